@@ -43,10 +43,10 @@
 extern "C" {
 #endif
 
-#define LKL_ABI_VERSION 6
+#define LKL_ABI_VERSION 7
 
-/* element types of q/k tensors */
-enum lkl_dtype { LKL_F16 = 0, LKL_BF16 = 1 };
+/* element types of q/k tensors; LKL_F32 for logits only (ABI version 7) */
+enum lkl_dtype { LKL_F16 = 0, LKL_BF16 = 1, LKL_F32 = 2 };
 
 /* element types accepted for the [B, T] padding mask (kernel_A.py:215-217) */
 enum lkl_mask_dtype { LKL_MASK_BOOL = 0, LKL_MASK_U8 = 1, LKL_MASK_I32 = 2, LKL_MASK_I64 = 3 };
@@ -299,6 +299,123 @@ void lkl_set_force_generic(int32_t force);
 int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, const void* kt,
                             const void* mask, const lkl_problem* p,
                             float* lse_s, float* lse_t, float* loss, void* stream);
+
+/* ---- Attention with a recomputing backward pass (ABI version 7) ----
+ * The attention of the distillation step itself.  For query head h of batch b
+ * and its kv head g = h / (Hq / Hkv), over the keys j valid for row i:
+ *   S_ij = sm_scale q_i . k_j,  lse_i = log sum_j e^S_ij,
+ *   P_ij = e^(S_ij - lse_i),    out_i = sum_j P_ij v_j.
+ * The backward keeps no n x n map: it recomputes P from q, k and lse;
+ *   delta_i = dout_i . out_i,  dS_ij = P_ij (dout_i . v_j - delta_i),
+ *   dq_i = sm_scale sum_j dS_ij k_j,  dk_j = sm_scale sum_i dS_ij q_i,
+ *   dv_j = sum_i P_ij dout_i   (dk, dv: over the query heads of the kv head).
+ * The mask is the [B, T] padding mask of the calls above: a token that it
+ * removes is neither a query nor a key.  Its row of out, lse, dq, dk and dv is
+ * 0, and what its rows of q, k, v, out and dout hold (NaN included) reaches no
+ * other row.
+ *
+ * All tensors are 16-bit of one type except lse (fp32 [B, Hq, T], contiguous).
+ * `strides` gives the element strides (b, h, t) of every 16-bit tensor in the
+ * order of its index below, each with a d stride of 1; NULL: all contiguous
+ * [B, H, T, D].  Input strides may be any non-negative number (0 where a tensor is
+ * broadcast), output strides are positive.  Head dims 8, 16, 32, 64 and 128 run on the tensor cores when
+ * every pointer is 16-byte aligned and every stride a positive multiple of 8
+ * elements; everything else runs on CUDA-core kernels.  lkl_last_path() tells which.
+ * Sums and softmax statistics are fp32; P and dS are rounded to the tensors'
+ * type before their products on the tensor cores.  Results are reproducible
+ * bit for bit: every output row has one writer.
+ * May be captured into CUDA graphs. */
+typedef struct lkl_attn_problem {
+  int32_t B, Hq, Hkv, T, D;
+  int32_t dtype;      /* LKL_F16 or LKL_BF16                                   */
+  int32_t causal;     /* nonzero: keep j <= i                                  */
+  int32_t mask_dtype; /* lkl_mask_dtype, ignored when mask == NULL             */
+  float sm_scale;     /* <= 0 selects 1/sqrt(D)                                */
+} lkl_attn_problem;
+
+enum lkl_attn_tensor {
+  LKL_ATTN_Q = 0, LKL_ATTN_K = 1, LKL_ATTN_V = 2, LKL_ATTN_OUT = 3, /* forward: 4 */
+  LKL_ATTN_DOUT = 4, LKL_ATTN_DQ = 5, LKL_ATTN_DK = 6, LKL_ATTN_DV = 7 /* backward: 8 */
+};
+
+/* Bytes of scratch of the forward (the packed mask; 0 without one). */
+size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);
+
+/* Bytes of scratch of the backward: the packed mask, 8 bytes per (batch, head,
+ * row) and, on the tensor cores, the 16-bit dS tiles that the key-stationary
+ * launch hands to the dq launch: all of them up to 8 GiB, beyond that the
+ * backward runs in chunks. */
+size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);
+
+int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_strides* strides,
+                         const void* mask, const lkl_attn_problem* p, void* out, float* lse,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const void* out,
+                          const float* lse, const void* dout, const lkl_strides* strides,
+                          const void* mask, const lkl_attn_problem* p, void* dq, void* dk,
+                          void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Logits (ABI version 7) ----
+ * Rows of logits: a [B, T, V] tensor with element strides (sb, st, 1), e.g.
+ * the logits of all positions but the last.  Type LKL_F16, LKL_BF16 or LKL_F32;
+ * pointers need only their element's alignment.  Every statistic is fp32. */
+typedef struct lkl_logits {
+  int64_t B, T, V;
+  int64_t sb, st;     /* element strides of the batch and token dims            */
+  int32_t dtype;      /* lkl_dtype                                              */
+} lkl_logits;
+
+#define LKL_MAX_TOP_K 32
+
+/* Log probabilities of given tokens, in one pass over the logits.  Per row:
+ *   lse = log sum_j e^x_j;  logprob = x_target - lse;
+ *   entropy = lse - sum_j p_j x_j;  the top_k largest log probabilities and
+ *   their indices, largest first, equal logits by the lowest index first.
+ * targets: int64 [B, T], contiguous.  A target equal to ignore_index gives
+ * logprob 0 (its entropy and alternatives are still given); any other target
+ * outside [0, V) gives logprob NaN.  logprob, entropy, lse: fp32 [B, T];
+ * top_logprobs fp32 and top_indices int64 [B, T, top_k], 0 <= top_k <=
+ * min(V, LKL_MAX_TOP_K) (both may be NULL when top_k == 0).  Logits of -inf
+ * have probability 0; a row with a NaN, with +inf or with nothing above -inf
+ * gives NaN (and its indices are valid but say nothing). */
+int32_t lkl_token_logprobs(const void* logits, const lkl_logits* l, const int64_t* targets,
+                           int64_t ignore_index, int32_t top_k, float* logprob, float* entropy,
+                           float* lse, float* top_logprobs, int64_t* top_indices, void* stream);
+
+/* d_logits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy), g =
+ * d_logprob (0 for an ignored target, NaN for one outside [0, V)), h =
+ * d_entropy; NULL means 0.  d_logits: contiguous [B, T, V] of the logits' type. */
+int32_t lkl_token_logprobs_backward(const void* logits, const lkl_logits* l,
+                                    const int64_t* targets, int64_t ignore_index,
+                                    const float* lse, const float* entropy,
+                                    const float* d_logprob, const float* d_entropy,
+                                    void* d_logits, void* stream);
+
+/* KL between the teacher's and the student's softened distributions, summed
+ * over the rows that the mask keeps:
+ *   *loss = sum_rows sum_j pt_j (log pt_j - log ps_j),  p = softmax(x / temperature).
+ * Replaces the logits term of the training loop (train.py:413-423), which
+ * divides the sum itself.  s and t have the same B, T, V and dtype; mask as
+ * above.  lse_s, lse_t (fp32 [B, T], of x / temperature; 0 where the mask
+ * removes the row) are what the backward needs.  A logit of -inf has
+ * probability 0 and a zero teacher probability adds nothing.
+ * The rows' sums are joined in a fixed order.  Workspace:
+ * lkl_logits_kl_workspace_size(). */
+size_t lkl_logits_kl_workspace_size(const lkl_logits* s);
+
+int32_t lkl_logits_kl_forward(const void* s_logits, const lkl_logits* s, const void* t_logits,
+                              const lkl_logits* t, const void* mask, int32_t mask_dtype,
+                              float temperature, float* lse_s, float* lse_t, float* loss,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ds[j] = *dloss (ps_j - pt_j) / temperature, 0 in the rows that the mask
+ * removes; contiguous [B, T, V] of the logits' type.  dloss: a device fp32
+ * scalar, NULL means 1. */
+int32_t lkl_logits_kl_backward(const void* s_logits, const lkl_logits* s, const void* t_logits,
+                               const lkl_logits* t, const void* mask, int32_t mask_dtype,
+                               float temperature, const float* lse_s, const float* lse_t,
+                               const float* dloss, void* ds, void* stream);
 
 #ifdef __cplusplus
 }

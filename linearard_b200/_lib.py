@@ -13,9 +13,9 @@ import threading
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "liblinearard_b200.so")
 
 __all__ = ["LKLProblem", "LKLStrides", "LKLGroupItem", "lib", "check", "LKLError",
-           "LKL_F16", "LKL_BF16", "MASK_DTYPES", "STATUS"]
+           "LKLAttnProblem", "LKLLogits", "LKL_F16", "LKL_BF16", "LKL_F32", "MASK_DTYPES", "STATUS"]
 
-LKL_F16, LKL_BF16 = 0, 1
+LKL_F16, LKL_BF16, LKL_F32 = 0, 1, 2
 LKL_MASK_BOOL, LKL_MASK_U8, LKL_MASK_I32, LKL_MASK_I64 = 0, 1, 2, 3
 STATUS = {
     0: "LKL_OK", 1: "LKL_ERR_NULL_POINTER", 2: "LKL_ERR_BAD_SHAPE", 3: "LKL_ERR_BAD_HEAD_DIM",
@@ -33,7 +33,10 @@ EXPORTS = ("lkl_abi_version", "lkl_status_string", "lkl_workspace_size", "lkl_ls
            "lkl_last_cuda_error", "lkl_backward_workspace_size", "lkl_forward_strided",
            "lkl_backward_strided", "lkl_grouped_workspace_size", "lkl_forward_grouped",
            "lkl_backward_grouped", "lkl_backward_plan", "lkl_forward_workspace_size",
-           "lkl_selftest_bounded_wait")
+           "lkl_selftest_bounded_wait", "lkl_attn_forward_workspace_size",
+           "lkl_attn_backward_workspace_size", "lkl_attn_forward", "lkl_attn_backward",
+           "lkl_token_logprobs", "lkl_token_logprobs_backward", "lkl_logits_kl_workspace_size",
+           "lkl_logits_kl_forward", "lkl_logits_kl_backward")
 
 
 class LKLProblem(ctypes.Structure):
@@ -59,6 +62,20 @@ class LKLGroupItem(ctypes.Structure):
                 ("lse_s", ctypes.c_void_p), ("lse_t", ctypes.c_void_p),
                 ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p),
                 ("strides", LKLStrides * 4)]
+
+
+class LKLAttnProblem(ctypes.Structure):
+    """Shape and options of an attention call (struct lkl_attn_problem)."""
+    _fields_ = [("B", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+                ("T", ctypes.c_int32), ("D", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("mask_dtype", ctypes.c_int32),
+                ("sm_scale", ctypes.c_float)]
+
+
+class LKLLogits(ctypes.Structure):
+    """Rows of logits, [B, T, V] with element strides (sb, st, 1) (struct lkl_logits)."""
+    _fields_ = [("B", ctypes.c_int64), ("T", ctypes.c_int64), ("V", ctypes.c_int64),
+                ("sb", ctypes.c_int64), ("st", ctypes.c_int64), ("dtype", ctypes.c_int32)]
 
 
 class LKLError(RuntimeError):
@@ -118,6 +135,27 @@ def _declare(L):
     L.lkl_backward_grouped.argtypes = [_i32, _G, _vp, _P, _vp, _vp, _sz, _vp]
     L.lkl_backward_plan.restype = _i32
     L.lkl_backward_plan.argtypes = [_P, _i32, _sz, _i32, ctypes.POINTER(ctypes.c_int32)]
+    _A, _R, _i64 = ctypes.POINTER(LKLAttnProblem), ctypes.POINTER(LKLLogits), ctypes.c_int64
+    for name in ("lkl_attn_forward_workspace_size", "lkl_attn_backward_workspace_size"):
+        getattr(L, name).restype = _sz
+        getattr(L, name).argtypes = [_A, _i32]
+    L.lkl_attn_forward.restype = _i32
+    L.lkl_attn_forward.argtypes = [_vp, _vp, _vp, _S, _vp, _A, _vp, _vp, _vp, _sz, _vp]
+    L.lkl_attn_backward.restype = _i32
+    L.lkl_attn_backward.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _S, _vp, _A, _vp, _vp, _vp, _vp,
+                                    _sz, _vp]
+    L.lkl_token_logprobs.restype = _i32
+    L.lkl_token_logprobs.argtypes = [_vp, _R, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp]
+    L.lkl_token_logprobs_backward.restype = _i32
+    L.lkl_token_logprobs_backward.argtypes = [_vp, _R, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]
+    L.lkl_logits_kl_workspace_size.restype = _sz
+    L.lkl_logits_kl_workspace_size.argtypes = [_R]
+    L.lkl_logits_kl_forward.restype = _i32
+    L.lkl_logits_kl_forward.argtypes = [_vp, _R, _vp, _R, _vp, _i32, ctypes.c_float, _vp, _vp, _vp,
+                                        _vp, _sz, _vp]
+    L.lkl_logits_kl_backward.restype = _i32
+    L.lkl_logits_kl_backward.argtypes = [_vp, _R, _vp, _R, _vp, _i32, ctypes.c_float, _vp, _vp,
+                                         _vp, _vp, _vp]
     L.lkl_forward_noalloc.restype = _i32
     L.lkl_forward_noalloc.argtypes = [_vp, _vp, _vp, _vp, _vp, _P, _vp, _vp, _vp, _vp]
 

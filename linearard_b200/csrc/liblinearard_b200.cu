@@ -2,5 +2,8 @@
 // sm_100a kernels and the C ABI share the device error word.
 #include "lkl_generic.cu"
 #include "lkl_sm100.cu"
+#include "lkl_attn_generic.cu"
+#include "lkl_logits.cu"
 #include "lkl_api.cu"
+#include "lkl_ops_api.cu"
 #include "lkl_noalloc.cu"

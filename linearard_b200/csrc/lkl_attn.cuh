@@ -1,0 +1,34 @@
+// Host-side description of one attention call, shared by its launchers.
+#pragma once
+
+#include "lkl_common.cuh"
+
+namespace lkl {
+
+struct AttnProblem {
+  int B, Hq, Hkv, T, D;
+  int dtype, causal;
+  float sc;
+};
+
+// Tensors of a call and their element strides; out, lse, ... as in lkl_attn_backward.
+struct AttnTensors {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const void* dout;
+  void *dq, *dk, *dv;
+  TensorStrides sq, sk, sv, so, sdo, sdq, sdk, sdv;
+};
+
+// CUDA-core kernels: every head dim of the set, any strides and alignment.
+cudaError_t launch_attn_generic_forward(const AttnProblem& p, const AttnTensors& t,
+                                        const uint32_t* bits, cudaStream_t st);
+// rows[b, h, i] = (-lse log2(e), delta_i); (-inf, 0) for a row the mask removes.
+cudaError_t launch_attn_delta(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
+                              float2* rows, cudaStream_t st);
+cudaError_t launch_attn_generic_backward(const AttnProblem& p, const AttnTensors& t,
+                                         const uint32_t* bits, const float2* rows,
+                                         cudaStream_t st);
+
+}  // namespace lkl

@@ -1,0 +1,111 @@
+"""KL between the teacher's and the student's logits.
+
+``logits_kl_align(s_logits, t_logits, attn_mask=None, temperature=1.0)`` returns
+the 0-d fp32 **sum** over the rows that the mask keeps of
+``KL(softmax(t / temperature) || softmax(s / temperature))``; the caller
+divides, as with ``attn_kl_align``.  This is the ``lam_l`` term of the training
+loop (``train.py:413-423``) without its [B, T, V] tensors of log probabilities:
+the forward reads both logits once, the backward once more
+(``lkl_logits_kl_forward`` / ``lkl_logits_kl_backward``).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+from ..attention_KL._common import prepare_mask, ptr, stream_of
+from ._common import check_logits, rows_of
+
+__all__ = ["logits_kl_align", "logits_kl_forward", "logits_kl_backward", "LogitsKLAlignFn"]
+
+
+def _check(s, t, temperature):
+    check_logits(s, "s_logits")
+    check_logits(t, "t_logits")
+    assert s.shape == t.shape, "student/teacher logits shape must match"
+    assert s.dtype == t.dtype, "student/teacher logits dtype must match"
+    assert s.device == t.device, "student/teacher must be on the same device"
+    assert isinstance(temperature, (float, int)), "temperature must be a scalar"
+    # single precision has to hold the temperature and what it divides by
+    assert 1e-30 < temperature < 1e30, "temperature must be positive"
+
+
+def _mask(attn_mask, s):
+    if attn_mask is None:
+        return prepare_mask(None, 0, 0, s.device)
+    assert isinstance(attn_mask, torch.Tensor), "attn_mask must be a torch.Tensor"
+    assert attn_mask.shape == s.shape[:-1], "attn_mask shape must be that of the logits' rows"
+    mask = attn_mask.contiguous()
+    mask = mask[None] if s.ndim == 2 else mask
+    return prepare_mask(mask, mask.shape[0], mask.shape[1], s.device)
+
+
+def logits_kl_forward(s_logits, t_logits, attn_mask=None, temperature=1.0):
+    """(loss 0-d fp32, lse_s, lse_t fp32 of the rows' shape: the log-sum-exp of
+    logits / temperature, 0 where the mask removes the row)."""
+    _check(s_logits, t_logits, temperature)
+    dev, shape = s_logits.device, tuple(s_logits.shape[:-1])
+    mask, mdt = _mask(attn_mask, s_logits)
+    rs, rt = rows_of(s_logits), rows_of(t_logits)
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        lse_s, lse_t = torch.empty((2,) + shape, device=dev, dtype=torch.float32).unbind(0)
+        loss = torch.empty((), device=dev, dtype=torch.float32)
+        n = int(L.lkl_logits_kl_workspace_size(ctypes.byref(rs)))
+        ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
+        st = L.lkl_logits_kl_forward(ptr(s_logits), ctypes.byref(rs), ptr(t_logits),
+                                     ctypes.byref(rt), ptr(mask), mdt, float(temperature),
+                                     ptr(lse_s), ptr(lse_t), ptr(loss), ptr(ws), n, stream_of(dev))
+    _lib.check(st, "lkl_logits_kl_forward")
+    return loss, lse_s, lse_t
+
+
+def logits_kl_backward(s_logits, t_logits, lse_s, lse_t, attn_mask=None, temperature=1.0,
+                       dloss=None):
+    """Gradient of the student's logits, contiguous, of their type.  dloss: a
+    device fp32 scalar, default 1."""
+    _check(s_logits, t_logits, temperature)
+    dev, shape = s_logits.device, tuple(s_logits.shape[:-1])
+    for z in (lse_s, lse_t):
+        assert isinstance(z, torch.Tensor) and tuple(z.shape) == shape, \
+            "lse shape must be that of the logits' rows"
+        assert z.dtype == torch.float32 and z.is_contiguous() and z.device == dev, \
+            "lse must be contiguous float32 on the device of the logits"
+    if dloss is not None:
+        assert isinstance(dloss, torch.Tensor) and dloss.numel() == 1 and dloss.device == dev \
+            and dloss.dtype == torch.float32, "dloss must be a float32 scalar on the device"
+    mask, mdt = _mask(attn_mask, s_logits)
+    rs, rt = rows_of(s_logits), rows_of(t_logits)
+    with torch.cuda.device(dev):
+        ds = torch.empty(s_logits.shape, device=dev, dtype=s_logits.dtype)
+        st = _lib.lib().lkl_logits_kl_backward(
+            ptr(s_logits), ctypes.byref(rs), ptr(t_logits), ctypes.byref(rt), ptr(mask), mdt,
+            float(temperature), ptr(lse_s), ptr(lse_t), ptr(dloss), ptr(ds), stream_of(dev))
+    _lib.check(st, "lkl_logits_kl_backward")
+    return ds
+
+
+class LogitsKLAlignFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, s_logits, t_logits, attn_mask, temperature):
+        loss, lse_s, lse_t = logits_kl_forward(s_logits, t_logits, attn_mask, temperature)
+        ctx.save_for_backward(s_logits, t_logits, lse_s, lse_t, attn_mask)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        s_logits, t_logits, lse_s, lse_t, mask = ctx.saved_tensors
+        ds = logits_kl_backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.temperature,
+                                dloss.to(torch.float32))
+        return ds, None, None, None      # the teacher gets no gradient
+
+
+def logits_kl_align(s_logits, t_logits, attn_mask=None, temperature=1.0):
+    """s_logits, t_logits: [B,T,V] (or [N,V]), fp16, bf16 or fp32 of one type, last
+    stride 1, read in place; attn_mask: [B,T] (or [N]), nonzero = kept, or None.
+    Gradients flow to the student's logits only."""
+    return LogitsKLAlignFn.apply(s_logits, t_logits, attn_mask, temperature)

@@ -1,0 +1,89 @@
+"""Log probabilities of given tokens, with entropy and top alternatives.
+
+``token_logprobs(logits, targets, top_k=0, ignore_index=-100)`` reads the
+logits once and never writes a [.., V] tensor of probabilities.  It takes views
+such as ``logits[:, :-1]`` as they are.  ``-logprob.sum()`` is the next-token
+loss; the gradients of logprob and entropy flow to the logits
+(``lkl_token_logprobs`` / ``lkl_token_logprobs_backward``).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import _lib
+from ..attention_KL._common import ptr, stream_of
+from ._common import check_logits, rows_of
+
+__all__ = ["token_logprobs", "TokenLogprobs", "TokenLogprobsFn", "MAX_TOP_K"]
+
+MAX_TOP_K = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """fp32 [B, T] each; the alternatives [B, T, top_k] (None without them)."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k: int, ignore_index: int):
+        rows, shape, dev = rows_of(logits), tuple(targets.shape), logits.device
+        with torch.cuda.device(dev):
+            stats = torch.empty((3,) + shape, device=dev, dtype=torch.float32)
+            logprob, entropy, lse = stats.unbind(0)
+            top_v = top_i = None
+            if top_k:
+                top_v = torch.empty(shape + (top_k,), device=dev, dtype=torch.float32)
+                top_i = torch.empty(shape + (top_k,), device=dev, dtype=torch.int64)
+            st = _lib.lib().lkl_token_logprobs(
+                ptr(logits), ctypes.byref(rows), ptr(targets), ignore_index, top_k, ptr(logprob),
+                ptr(entropy), ptr(lse), ptr(top_v), ptr(top_i), stream_of(dev))
+        _lib.check(st, "lkl_token_logprobs")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, targets, lse, entropy)
+        ctx.ignore_index = ignore_index
+        if top_k:
+            ctx.mark_non_differentiable(top_v, top_i)
+        return logprob, entropy, top_v, top_i
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logprob, d_entropy, _top_v, _top_i):
+        if d_logprob is None and d_entropy is None:
+            return None, None, None, None
+        logits, targets, lse, entropy = ctx.saved_tensors
+        rows, dev = rows_of(logits), logits.device
+        with torch.cuda.device(dev):
+            g, h = (None if d is None else d.to(torch.float32).contiguous()
+                    for d in (d_logprob, d_entropy))
+            dx = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+            st = _lib.lib().lkl_token_logprobs_backward(
+                ptr(logits), ctypes.byref(rows), ptr(targets), ctx.ignore_index, ptr(lse),
+                ptr(entropy), ptr(g), ptr(h), ptr(dx), stream_of(dev))
+        _lib.check(st, "lkl_token_logprobs_backward")
+        return dx, None, None, None
+
+
+def token_logprobs(logits, targets, top_k=0, ignore_index=-100) -> TokenLogprobs:
+    """logits: [B,T,V] (or [N,V]) fp16, bf16 or fp32 on CUDA, last stride 1;
+    targets: int64 [B,T] (or [N]).  logprob is 0 where the target is
+    ignore_index and NaN where it is any other number outside [0, V).
+    top_k: up to 32 alternatives, largest first, equal logits by the lowest
+    index.  logprob and entropy carry gradients to the logits; the
+    alternatives carry none."""
+    check_logits(logits)
+    assert isinstance(targets, torch.Tensor), "targets must be a torch.Tensor"
+    assert targets.device == logits.device, "targets must be on the device of the logits"
+    assert targets.dtype == torch.int64, "targets must be int64"
+    assert targets.shape == logits.shape[:-1], "targets shape must be that of the logits' rows"
+    assert isinstance(top_k, int) and 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]), \
+        "top_k must be from 0 to min(V, 32)"
+    assert isinstance(ignore_index, int), "ignore_index must be an integer"
+    return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets.contiguous(), top_k,
+                                                ignore_index))
