@@ -23,7 +23,7 @@ LIB_NAME = "liblinearard_b200.so"
 LIB_PATH = os.path.join(OUT_DIR, LIB_NAME)
 
 SOURCES = ["liblinearard_b200.cu", "lkl_api.cu", "lkl_generic.cu", "lkl_sm100.cu", "lkl_noalloc.cu",
-           "lkl_attn_generic.cu", "lkl_attn.cuh", "lkl_logits.cu", "lkl_logits.cuh", "lkl_ops_api.cu",
+           "lkl_attn_generic.cu", "lkl_attn_sm100.cu", "lkl_attn.cuh", "lkl_logits.cu", "lkl_logits.cuh", "lkl_ops_api.cu",
            "lkl_common.cuh", "sm100_ptx.cuh"]
 
 NVCC_FLAGS = [

@@ -3,6 +3,7 @@
 #include "lkl_generic.cu"
 #include "lkl_sm100.cu"
 #include "lkl_attn_generic.cu"
+#include "lkl_attn_sm100.cu"
 #include "lkl_logits.cu"
 #include "lkl_api.cu"
 #include "lkl_ops_api.cu"

@@ -31,4 +31,10 @@ cudaError_t launch_attn_generic_backward(const AttnProblem& p, const AttnTensors
                                          const uint32_t* bits, const float2* rows,
                                          cudaStream_t st);
 
+// Tensor-core kernels: head dims up to 128, 16-byte aligned pointers, strides
+// that are positive multiples of 8 elements.
+bool attn_sm100_supports(const AttnProblem& p, const AttnTensors& t);
+cudaError_t launch_attn_sm100_forward(const AttnProblem& p, const AttnTensors& t,
+                                      const uint32_t* bits, cudaStream_t st);
+
 }  // namespace lkl

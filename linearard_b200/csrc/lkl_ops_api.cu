@@ -132,8 +132,9 @@ int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_
   t.sv = attn_strides(strides, LKL_ATTN_V, p);
   t.so = attn_strides(strides, LKL_ATTN_OUT, p);
   const AttnProblem a = to_attn(p);
-  t_last_path = 0;
-  return launch_status(lkl::launch_attn_generic_forward(a, t, bits, st));
+  t_last_path = !g_force_generic.load() && lkl::attn_sm100_supports(a, t) ? 1 : 0;
+  return launch_status(t_last_path ? lkl::launch_attn_sm100_forward(a, t, bits, st)
+                                   : lkl::launch_attn_generic_forward(a, t, bits, st));
 }
 
 int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const void* out,
