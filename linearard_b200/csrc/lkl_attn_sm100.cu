@@ -1,6 +1,6 @@
-// sm_100a tensor-core attention: the forward.
+// sm_100a tensor-core attention, forward and recomputing backward.
 //
-// One CTA owns 256 query rows of one head as two tiles of 128 and walks the
+// Forward: one CTA owns 256 query rows of one head as two tiles of 128 and walks the
 // 128-key tiles from the diagonal down.  Per tile and key tile, two GEMMs
 // (S = Q K^T, O += P V) and one exponential per score.  At head dim 128 the
 // 16,384 exponentials of a tile take 1024 cycles of the SM's MUFU pipe and its
@@ -411,6 +411,786 @@ cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const u
   return cudaGetLastError();
 }
 
+// ============================================================== backward
+// Two launches per chunk of the dS buffer and no reductions.
+//
+// dkv launch (key-stationary): one CTA owns 128 keys of one kv head and walks
+// the query tiles of the group's heads.  Scores are computed transposed (lanes
+// = keys, columns = queries), so that P^T and dS^T, written to TMEM as 16-bit
+// values, are the A operands of dV += P^T dO and dK += dS^T Q.  dS^T also goes to
+// the dS buffer in HBM.
+// dq launch (persistent GEMM): dq_i = sm_scale sum_j dS_ij K_j from that buffer.
+//
+// The hand-over costs 32 KB of HBM writes and reads a tile pair (10 ns of the
+// whole GPU) and saves the second recomputation of S and dP: two GEMMs and
+// 16,384 exponentials.  Reducing dq in L2 instead would move 64 KB of fp32 a
+// pair, in an order that changes from run to run.
+//
+// Bound of the dkv launch: four GEMMs of 512 cycles a tile pair against 1024
+// cycles of exponentials.  The issue order dV(i), S(i+1), dK(i), dP(i+1) keeps the
+// tensor pipe busy: dS(i) is computed under dV(i) and S(i+1), P(i+1) under dK(i)
+// and dP(i+1).  All 512 TMEM columns are in use (S, dP, dV, dK at head dim 128;
+// P and dS overwrite the first half of what they come from).
+constexpr int kFbThreads = 384;
+constexpr int kFbProducer = 8, kFbMma = 9, kFbCleaner = 10, kFbStats = 11;
+
+// One backward chunk: kv groups [g0, g1), key tiles [j0, j1).  `split`: not all
+// key tiles, so that dq is summed over launches in fp32.
+struct FbChunk {
+  int g0, g1, j0, j1;
+  int split;
+  int band;            // kv groups per band of work items
+  long long tph;       // dS tiles per query head
+};
+
+__host__ __device__ __forceinline__ long long fb_tile(const FbChunk& c, int causal, int n_t, int i,
+                                                      int j) {
+  if (c.split) return (long long)(i - (causal ? c.j0 : 0)) * (c.j1 - c.j0) + (j - c.j0);
+  return causal ? (long long)i * (i + 1) / 2 + j : (long long)i * n_t + j;
+}
+
+// Query rows' statistics as the dkv launch reads them: per (head, query tile)
+// 128 exponent offsets -lse log2(e) (-inf for a row without gradient), then
+// 128 delta_i = dout_i . out_i.
+constexpr int kFbStatBytes = 2 * kBM * 4;
+
+// A block takes one tile of 128 rows; D / 8 neighbouring lanes share a row.
+__global__ void __launch_bounds__(256)
+attn_sm100_delta_kernel(const AttnProblem p, const AttnTensors a,
+                        const uint32_t* __restrict__ bits, float* __restrict__ stats) {
+  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5;
+  const int bh = blockIdx.x / n_t, qt = blockIdx.x % n_t, b = bh / p.Hq, h = bh % p.Hq;
+  const int lanes = p.D / 8, sub = threadIdx.x % lanes;
+  float* dst = stats + (size_t)blockIdx.x * 2 * kBM;
+  for (int r = threadIdx.x / lanes; r < kBM; r += 256 / lanes) {
+    const int i = qt * kBM + r;
+    const bool on = i < p.T && token_valid(bits, words, b, i);
+    float s = 0.f;
+    if (on) {
+      const uint4 x = *reinterpret_cast<const uint4*>(
+          static_cast<const uint16_t*>(a.out) + (size_t)b * a.so.b + (size_t)h * a.so.h +
+          (size_t)i * a.so.t + sub * 8);
+      const uint4 y = *reinterpret_cast<const uint4*>(
+          static_cast<const uint16_t*>(a.dout) + (size_t)b * a.sdo.b + (size_t)h * a.sdo.h +
+          (size_t)i * a.sdo.t + sub * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        s = fmaf(load_elem(&x, e, p.dtype), load_elem(&y, e, p.dtype), s);
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (sub == 0) {
+      dst[r] = on ? -a.lse[(size_t)bh * p.T + i] * kLog2e : -CUDART_INF_F;
+      dst[kBM + r] = s;
+    }
+  }
+}
+
+template <int D>
+struct FbLayout {
+  static constexpr int TILE = kBM * D * 2;
+  static constexpr int NS = D == 128 ? 5 : 8;   // ring of Q and dO tiles
+  static constexpr int OFF_K = 0, OFF_V = TILE, OFF_RING = 2 * TILE;
+  static constexpr int OFF_MISC = OFF_RING + NS * TILE;
+  static constexpr int MISC = 512;
+  // statistics: exponent offsets of two query tiles, delta of one
+  static constexpr int OFF_LSE = OFF_MISC + MISC, OFF_DELTA = OFF_LSE + kFbStatBytes;
+  static constexpr int BYTES = 1024 + OFF_DELTA + kFbStatBytes / 2;
+  static_assert(BYTES <= kMaxDynSmem, "shared memory");
+};
+
+struct FbMisc {
+  uint64_t kv_full;
+  uint64_t full[8], ready[8], empty[8];
+  uint64_t lse_full[2], lse_empty[2], delta_full, delta_empty;
+  uint64_t s_full, p_full, dp_full, ds_full, acc_full;
+  uint32_t tmem_base;
+  int abort;
+};
+static_assert(sizeof(FbMisc) <= 512, "misc region too small");
+
+// Next query tile at or above i with a token in it, or n_t.
+template <bool MASKED>
+__device__ __forceinline__ int live_tile_up(const uint32_t* bits, int words, int b, int i,
+                                            int n_t) {
+  if (MASKED)
+    while (i < n_t && !tile_bits<true>(bits, words, b, i).any()) ++i;
+  return i;
+}
+
+// The (query head, query tile) pairs of a dkv CTA, in the order every role takes them.
+template <bool MASKED>
+struct FbWalk {
+  const uint32_t* bits;
+  int words, b, n_t, first, h, h_end, i;
+  __device__ __forceinline__ FbWalk(const uint32_t* bits_, int words_, int b_, int n_t_, int first_,
+                                    int h0, int G)
+      : bits(bits_), words(words_), b(b_), n_t(n_t_), h(h0), h_end(h0 + G) {
+    first = live_tile_up<MASKED>(bits, words, b, first_, n_t);
+    i = first;
+    if (first >= n_t) h = h_end;
+  }
+  __device__ __forceinline__ bool on() const { return h < h_end; }
+  __device__ __forceinline__ void next() {
+    i = live_tile_up<MASKED>(bits, words, b, i + 1, n_t);
+    if (i >= n_t) {
+      i = first;
+      ++h;
+    }
+  }
+};
+
+// This thread's NC fp32 TMEM columns times `scale` as 16-bit values into row[0 .. n_valid).
+template <int NC, bool BF16>
+__device__ __forceinline__ void store_row16(uint32_t taddr, uint16_t* row, float scale, bool store,
+                                            bool zero, int n_valid) {
+#pragma unroll
+  for (int c = 0; c < NC; c += 32) {
+    float v[32];
+    tmem_ld32(taddr + c, v);
+    tmem_wait_ld_dep(v);
+    if (!store) continue;
+#pragma unroll
+    for (int k = 0; k < 32; k += 8) {
+      if (c + k >= n_valid) break;
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = zero ? 0u : pack2t<BF16>(v[k + 2 * e] * scale, v[k + 2 * e + 1] * scale);
+      *reinterpret_cast<uint4*>(row + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <int D, bool BF16, bool MASKED>
+__global__ void __launch_bounds__(kFbThreads, 1)
+attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
+                      const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ CUtensorMap tm_do, const AttnProblem p,
+                      const AttnTensors a, const FbChunk c, const uint32_t* __restrict__ bits,
+                      const float* __restrict__ stats, uint16_t* __restrict__ dsbuf) {
+  using L = FbLayout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  FbMisc* misc = reinterpret_cast<FbMisc*>(smem + L::OFF_MISC);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* err = &g_device_error;
+  volatile int* abort = &misc->abort;
+  constexpr uint32_t kColDp = 128, kColDv = 256, kColDk = 256 + D;
+
+  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5, G = p.Hq / p.Hkv;
+  // bands of kv groups, key tiles ascending (the longest first when causal)
+  int lg, j;
+  {
+    const int n_j = c.j1 - c.j0, n_g = c.g1 - c.g0, blk = blockIdx.x;
+    const int k = blk / (c.band * n_j), r = blk % (c.band * n_j);
+    const int size = min(c.band, n_g - k * c.band);
+    lg = k * c.band + r % size;
+    j = c.j0 + r / size;
+  }
+  const int grp = c.g0 + lg, b = grp / p.Hkv, g = grp % p.Hkv;
+  const TileBits keys = tile_bits<MASKED>(bits, words, b, j);
+  const FbWalk<MASKED> walk0(bits, words, b, n_t, p.causal ? j : 0, g * G, keys.any() ? G : 0);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&misc->kv_full, 1);
+    for (int s = 0; s < L::NS; ++s) {
+      mbar_init(&misc->full[s], 1);
+      mbar_init(&misc->ready[s], 1);
+      mbar_init(&misc->empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&misc->lse_full[s], 1);
+      mbar_init(&misc->lse_empty[s], 8);
+    }
+    mbar_init(&misc->delta_full, 1);
+    mbar_init(&misc->delta_empty, 8);
+    mbar_init(&misc->s_full, 1);
+    mbar_init(&misc->p_full, 8);
+    mbar_init(&misc->dp_full, 1);
+    mbar_init(&misc->ds_full, 8);
+    mbar_init(&misc->acc_full, 1);
+    misc->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kFbMma) {
+    tmem_alloc(&misc->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == kFbProducer && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_do);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc->tmem_base;
+
+  if (warp == kFbProducer) {
+    if (lane == 0 && walk0.on()) {
+      mbar_arrive_expect_tx(&misc->kv_full, 2 * L::TILE);
+      issue_tile_loads(smem + L::OFF_K, &tm_k, &misc->kv_full, D, j * kBN, g, b);
+      issue_tile_loads(smem + L::OFF_V, &tm_v, &misc->kv_full, D, j * kBN, g, b);
+      int n = 0;   // Q(0), dO(0), Q(1), dO(1), ...
+      bool ok = true;
+      for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next())
+        for (int o = 0; o < 2; ++o, ++n) {
+          const int s = n % L::NS;
+          if (n >= L::NS && !mbar_wait(&misc->empty[s], (n / L::NS - 1) & 1, abort, err)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&misc->full[s], L::TILE);
+          issue_tile_loads(smem + L::OFF_RING + s * L::TILE, o ? &tm_do : &tm_q, &misc->full[s], D,
+                           w.i * kBM, w.h, b);
+        }
+    }
+  } else if (warp == kFbStats) {
+    if (lane == 0 && walk0.on()) {
+      constexpr int kHalf = kFbStatBytes / 2;
+      auto src = [&](const FbWalk<MASKED>& w) {
+        return stats + ((size_t)(b * p.Hq + w.h) * n_t + w.i) * 2 * kBM;
+      };
+      auto load_lse = [&](const FbWalk<MASKED>& w, int it) {
+        const int e = it & 1;
+        if (it >= 2 && !mbar_wait(&misc->lse_empty[e], ((it >> 1) - 1) & 1, abort, err))
+          return false;
+        mbar_arrive_expect_tx(&misc->lse_full[e], kHalf);
+        bulk_load(smem + L::OFF_LSE + e * kHalf, src(w), kHalf, &misc->lse_full[e]);
+        return true;
+      };
+      FbWalk<MASKED> w = walk0;
+      bool ok = load_lse(w, 0);
+      for (int it = 0; ok && w.on(); ++it) {
+        if (it >= 1 && !mbar_wait(&misc->delta_empty, (it - 1) & 1, abort, err)) break;
+        mbar_arrive_expect_tx(&misc->delta_full, kHalf);
+        bulk_load(smem + L::OFF_DELTA, src(w) + kBM, kHalf, &misc->delta_full);
+        w.next();
+        if (w.on()) ok = load_lse(w, it + 1);
+      }
+    }
+  } else if (warp == kFbMma) {
+    if (lane == 0 && walk0.on()) {
+      const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
+      const uint32_t id_g = idesc_f16(kBM, D, BF16, BF16, 0, 1);
+      const uint32_t k_at = smem_u32(smem + L::OFF_K), v_at = smem_u32(smem + L::OFF_V);
+      const uint32_t ring = smem_u32(smem + L::OFF_RING);
+      uint64_t* loaded = MASKED ? misc->ready : misc->full;
+      auto wait_load = [&](int n) {
+        return mbar_wait(&loaded[n % L::NS], (n / L::NS) & 1, abort, err);
+      };
+      // S^T = K Q^T (n: load of Q) and dP^T = V dO^T (n: load of dO)
+      auto scores = [&](int n, uint32_t a_at, uint32_t col, uint64_t* bar) {
+        const uint32_t b_at = ring + (n % L::NS) * L::TILE;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_f16_ss(tmem + col, kmajor_desc(a_at, kk), kmajor_desc(b_at, kk), id_s, kk > 0);
+        umma_commit(bar);
+      };
+      // acc += A^T-from-TMEM x tile; the two warpgroups' halves of A lie 64 columns apart
+      auto grads = [&](int n, uint32_t acc, uint32_t col, bool first) {
+        const uint32_t b_at = ring + (n % L::NS) * L::TILE;
+#pragma unroll
+        for (int kk = 0; kk < kBM / 16; ++kk)
+          umma_f16_ts(tmem + acc, tmem + col + (kk >> 2) * 64 + (kk & 3) * 8,
+                      mnmajor_desc(b_at, kk), id_g, (!first || kk > 0) ? 1u : 0u);
+        umma_commit(&misc->empty[n % L::NS]);
+      };
+      bool ok = mbar_wait(&misc->kv_full, 0, abort, err) && wait_load(0);
+      if (ok) {
+        tc_fence_after();
+        scores(0, k_at, 0, &misc->s_full);
+        ok = wait_load(1);
+      }
+      if (ok) {
+        tc_fence_after();
+        scores(1, v_at, kColDp, &misc->dp_full);
+      }
+      int it = 0;
+      FbWalk<MASKED> w = walk0;
+      while (ok) {
+        w.next();
+        const bool more = w.on();
+        if (!(ok = mbar_wait(&misc->p_full, it & 1, abort, err))) break;
+        tc_fence_after();
+        grads(2 * it + 1, kColDv, 0, it == 0);
+        if (more) {
+          if (!(ok = wait_load(2 * it + 2))) break;
+          tc_fence_after();
+          scores(2 * it + 2, k_at, 0, &misc->s_full);
+        }
+        if (!(ok = mbar_wait(&misc->ds_full, it & 1, abort, err))) break;
+        tc_fence_after();
+        grads(2 * it, kColDk, kColDp, it == 0);
+        if (!more) break;
+        if (!(ok = wait_load(2 * it + 3))) break;
+        tc_fence_after();
+        scores(2 * it + 3, v_at, kColDp, &misc->dp_full);
+        ++it;
+      }
+      if (ok) umma_commit(&misc->acc_full);
+    }
+  } else if (warp == kFbCleaner) {
+    if (MASKED) {
+      int n = 0;
+      bool ok = true;
+      for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next()) {
+        const TileBits tb = tile_bits<MASKED>(bits, words, b, w.i);
+        for (int o = 0; o < 2; ++o, ++n) {
+          const int s = n % L::NS;
+          if (!mbar_wait(&misc->full[s], (n / L::NS) & 1, abort, err)) {
+            ok = false;
+            break;
+          }
+          if (!tb.all()) {
+            clear_rows<D>(smem + L::OFF_RING + s * L::TILE, tb, lane);
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&misc->ready[s]);
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ---------------- thread = key r; warpgroup wg owns 64 of the tile's 128 queries
+    const int wg = warp >> 2, r = (warp & 3) * 32 + lane, key = j * kBN + r;
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + wg * 64;
+    const float cs = p.sc * kLog2e;
+    const uint64_t cs2 = f2pack(cs, cs);
+    const bool key_ok = key < p.T && ((keys.w[warp & 3] >> lane) & 1u);
+    uint4* const buf = reinterpret_cast<uint4*>(dsbuf) + (size_t)(wg * 8) * kBM + r;
+    int it = 0;
+    bool ok = true;
+    for (FbWalk<MASKED> w = walk0; w.on(); w.next(), ++it) {
+      const float* nl =
+          reinterpret_cast<const float*>(smem + L::OFF_LSE + (it & 1) * (kFbStatBytes / 2)) +
+          wg * 64;
+      const float* dl = reinterpret_cast<const float*>(smem + L::OFF_DELTA) + wg * 64;
+      if (!mbar_wait(&misc->lse_full[it & 1], (it >> 1) & 1, abort, err) ||
+          !mbar_wait(&misc->s_full, it & 1, abort, err)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float pr[2][32];
+      tmem_ld32(lane_addr, pr[0]);
+      tmem_ld32(lane_addr + 32, pr[1]);
+      tmem_wait_ld_dep(pr[0]);
+      tmem_wait_ld_dep(pr[1]);
+      // causal: a query before this key takes no part (the diagonal tile only)
+      const int from = p.causal && w.i == j ? r - wg * 64 : 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(nl + h * 32 + k);
+          float* x = pr[h] + k;
+          f2unpack(ffma2(f2pack(x[0], x[1]), cs2, f2pack(z.x, z.y)), x[0], x[1]);
+          f2unpack(ffma2(f2pack(x[2], x[3]), cs2, f2pack(z.z, z.w)), x[2], x[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
+        }
+        if (!key_ok || from > 0) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (!key_ok || h * 32 + k < from) pr[h][k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) packed[k >> 1] = pack2t<BF16>(pr[h][k], pr[h][k + 1]);
+        tmem_st16(lane_addr + h * 16, packed);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&misc->p_full);
+        mbar_arrive(&misc->lse_empty[it & 1]);
+      }
+
+      if (!mbar_wait(&misc->delta_full, it & 1, abort, err) ||
+          !mbar_wait(&misc->dp_full, it & 1, abort, err)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t ds[2][16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x[32];
+        tmem_ld32(lane_addr + kColDp + h * 32, x);
+        tmem_wait_ld_dep(x);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(dl + h * 32 + k);
+          f2unpack(fmul2(f2pack(pr[h][k], pr[h][k + 1]),
+                         fsub2(f2pack(x[k], x[k + 1]), f2pack(z.x, z.y))), x[k], x[k + 1]);
+          f2unpack(fmul2(f2pack(pr[h][k + 2], pr[h][k + 3]),
+                         fsub2(f2pack(x[k + 2], x[k + 3]), f2pack(z.z, z.w))), x[k + 2], x[k + 3]);
+        }
+        if (MASKED && !key_ok) {   // 0 x what the removed key's v holds
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) ds[h][k >> 1] = pack2t<BF16>(x[k], x[k + 1]);
+      }
+      // both halves are loaded: dS may overwrite the first of them
+      tmem_st16(lane_addr + kColDp, ds[0]);
+      tmem_st16(lane_addr + kColDp + 16, ds[1]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&misc->ds_full);
+        mbar_arrive(&misc->delta_empty);
+      }
+      // 16 groups of 8 queries, each [128 keys][16 bytes]: the no-swizzle core-matrix
+      // layout that the dq GEMM reads; a warp's store covers 512 contiguous bytes
+      const long long head = (long long)lg * G + (w.h - g * G);
+      uint4* dst = buf + (size_t)(head * c.tph + fb_tile(c, p.causal, n_t, w.i, j)) *
+                             (kDTileElems / 8);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t* v = ds[k >> 2] + (k & 3) * 4;
+        dst[k * kBM] = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    if (ok && it > 0) ok = mbar_wait(&misc->acc_full, 0, abort, err);
+    tc_fence_after();
+    if (ok) {
+      const uint32_t row_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + wg * (D / 2);
+      const bool in = key < p.T, zero = !key_ok || it == 0;
+      const int first = wg * (D / 2);
+      uint16_t* dv = static_cast<uint16_t*>(a.dv) + (size_t)b * a.sdv.b + (size_t)g * a.sdv.h +
+                     (size_t)key * a.sdv.t + first;
+      uint16_t* dk = static_cast<uint16_t*>(a.dk) + (size_t)b * a.sdk.b + (size_t)g * a.sdk.h +
+                     (size_t)key * a.sdk.t + first;
+      store_row16<D / 2, BF16>(row_addr + kColDv, dv, 1.f, in && first < p.D, zero, p.D - first);
+      store_row16<D / 2, BF16>(row_addr + kColDk, dk, p.sc, in && first < p.D, zero, p.D - first);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kFbMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// dq launch: a pipelined GEMM, one persistent CTA per SM.  Work item = (query
+// head, query tile i): dq_i = sm_scale sum_j dS_ij K_j.  A = dS (one bulk copy of a
+// stored tile, no swizzle, MN-major), B = K (TMA, 128-byte swizzle, MN-major).
+// Bound by HBM: 32 KB of dS for 4.2 MFLOP.  Two accumulators, so that an item's
+// epilogue runs under the next item's GEMM.
+constexpr int kFqThreads = 224;   // producer, MMA, cleaner, four epilogue warps
+
+template <int D>
+struct FqLayout {
+  static constexpr int DS_BYTES = kDTileElems * 2, K_BYTES = kBM * D * 2;
+  static constexpr int STAGE = DS_BYTES + K_BYTES;
+  static constexpr int NS = D == 128 ? 3 : 4;
+  static constexpr int OFF_MISC = NS * STAGE;
+  static constexpr int BYTES = 1024 + OFF_MISC + kMisc;
+  static_assert(BYTES <= kMaxDynSmem, "shared memory");
+};
+
+struct FqMisc {
+  uint64_t full[4], ready[4], empty[4];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct FqWork {
+  int head, b, h, i, kt_last;   // head: within the chunk; kt_last: last key tile in it
+};
+__device__ __forceinline__ FqWork fq_work(const AttnProblem& p, const FbChunk& c, int n_t, int w) {
+  FqWork k;
+  const int G = p.Hq / p.Hkv, heads = (c.g1 - c.g0) * G;
+  const int i0 = p.causal ? c.j0 : 0, band = c.band * G, n_i = n_t - i0;
+  const int kb = w / (band * n_i), r = w % (band * n_i), size = min(band, heads - kb * band);
+  k.head = kb * band + r % size;
+  k.i = n_t - 1 - r / size;   // the longest first
+  const int gh = c.g0 * G + k.head;   // kv groups and query heads are both head-major
+  k.b = gh / p.Hq;
+  k.h = gh % p.Hq;
+  k.kt_last = (p.causal ? min(k.i, c.j1 - 1) : c.j1 - 1);
+  return k;
+}
+
+template <int D, bool BF16, bool MASKED>
+__global__ void __launch_bounds__(kFqThreads, 1)
+attn_sm100_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const AttnProblem p,
+                     const AttnTensors a, const FbChunk c, const uint32_t* __restrict__ bits,
+                     const uint16_t* __restrict__ dsbuf, float* __restrict__ acc32) {
+  using L = FqLayout<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  FqMisc* misc = reinterpret_cast<FqMisc*>(smem + L::OFF_MISC);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* err = &g_device_error;
+  volatile int* abort = &misc->abort;
+  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5, G = p.Hq / p.Hkv;
+  const int n_work = (c.g1 - c.g0) * G * (n_t - (p.causal ? c.j0 : 0));
+  // "snake" order over the CTAs: evens out the causal lengths
+  auto work_at = [&](int rd) {
+    const int n = (int)gridDim.x, k = (int)blockIdx.x;
+    return rd * n + ((rd & 1) ? n - 1 - k : k);
+  };
+  // key tiles of an item, from the last down (a query tile without a token has none)
+  auto first_kt = [&](const FqWork& k) {
+    if (MASKED && !tile_bits<MASKED>(bits, words, k.b, k.i).any()) return -1;
+    const int kt = live_tile<MASKED>(bits, words, k.b, k.kt_last);
+    return kt >= c.j0 ? kt : -1;
+  };
+  auto next_kt = [&](const FqWork& k, int kt) {
+    kt = live_tile<MASKED>(bits, words, k.b, kt - 1);
+    return kt >= c.j0 ? kt : -1;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&misc->full[s], 1);
+      mbar_init(&misc->ready[s], 1);
+      mbar_init(&misc->empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&misc->acc_full[s], 1);
+      mbar_init(&misc->acc_empty[s], 4);
+    }
+    misc->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&misc->tmem_base, 256);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) tma_prefetch_desc(&tm_k);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc->tmem_base;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int n = 0;
+      bool ok = true;
+      for (int rd = 0, w = work_at(0); ok && w < n_work; w = work_at(++rd)) {
+        const FqWork k = fq_work(p, c, n_t, w);
+        for (int kt = first_kt(k); kt >= 0; kt = next_kt(k, kt), ++n) {
+          const int s = n % L::NS;
+          if (n >= L::NS && !mbar_wait(&misc->empty[s], (n / L::NS - 1) & 1, abort, err)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * L::STAGE;
+          mbar_arrive_expect_tx(&misc->full[s], L::STAGE);
+          bulk_load(st,
+                    dsbuf + ((long long)k.head * c.tph + fb_tile(c, p.causal, n_t, k.i, kt)) *
+                                kDTileElems,
+                    L::DS_BYTES, &misc->full[s]);
+          issue_tile_loads(st + L::DS_BYTES, &tm_k, &misc->full[s], D, kt * kBN, k.h / G, k.b);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t id = idesc_f16(kBM, D, BF16, BF16, 1, 1);
+      uint64_t* loaded = MASKED ? misc->ready : misc->full;
+      int n = 0, it = 0;
+      bool ok = true;
+      for (int rd = 0, w = work_at(0); ok && w < n_work; w = work_at(++rd)) {
+        const FqWork k = fq_work(p, c, n_t, w);
+        int kt = first_kt(k);
+        if (kt < 0) continue;
+        const int ab = it & 1;
+        if (it >= 2 && !mbar_wait(&misc->acc_empty[ab], ((it >> 1) - 1) & 1, abort, err)) break;
+        tc_fence_after();
+        for (uint32_t more = 0; kt >= 0; kt = next_kt(k, kt), ++n, more = 1) {
+          const int s = n % L::NS;
+          if (!mbar_wait(&loaded[s], (n / L::NS) & 1, abort, err)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t at = smem_u32(smem + s * L::STAGE), bt = at + L::DS_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < kBN / 16; ++kk)
+            umma_f16_ss(tmem + ab * 128, desc_interleave(at + kk * 2 * 128, 128, kBM * 16),
+                        mnmajor_desc(bt, kk), id, (more || kk > 0) ? 1u : 0u);
+          umma_commit(&misc->empty[s]);
+        }
+        if (ok) umma_commit(&misc->acc_full[ab]);
+        ++it;
+      }
+    }
+  } else if (warp == 2) {
+    if (MASKED) {
+      int n = 0;
+      bool ok = true;
+      for (int rd = 0, w = work_at(0); ok && w < n_work; w = work_at(++rd)) {
+        const FqWork k = fq_work(p, c, n_t, w);
+        for (int kt = first_kt(k); kt >= 0; kt = next_kt(k, kt), ++n) {
+          const int s = n % L::NS;
+          if (!mbar_wait(&misc->full[s], (n / L::NS) & 1, abort, err)) {
+            ok = false;
+            break;
+          }
+          const TileBits tb = tile_bits<MASKED>(bits, words, k.b, kt);
+          if (!tb.all()) {
+            clear_rows<D>(smem + s * L::STAGE + L::DS_BYTES, tb, lane);
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&misc->ready[s]);
+        }
+      }
+    }
+  } else {
+    const int r = (warp & 3) * 32 + lane;
+    int it = 0;
+    for (int rd = 0, w = work_at(0); w < n_work; w = work_at(++rd)) {
+      const FqWork k = fq_work(p, c, n_t, w);
+      const bool any = first_kt(k) >= 0;
+      const int ab = it & 1, i = k.i * kBM + r;
+      if (any && !mbar_wait(&misc->acc_full[ab], (it >> 1) & 1, abort, err)) break;
+      tc_fence_after();
+      const bool in = i < p.T;
+      const bool live = any && in && token_valid(MASKED ? bits : nullptr, words, k.b, i);
+      uint16_t* row = static_cast<uint16_t*>(a.dq) + (size_t)k.b * a.sdq.b + (size_t)k.h * a.sdq.h +
+                      (size_t)i * a.sdq.t;
+      const uint32_t taddr = tmem + ab * 128 + ((uint32_t)((warp & 3) * 32) << 16);
+      // a split head: fp32 sums over its launches, rounded by the last of them
+      const bool first = c.j0 == 0, last = p.causal ? k.i < c.j1 : c.j1 == n_t;
+#pragma unroll
+      for (int col = 0; col < D; col += 32) {
+        float v[32];
+        if (any) {
+          tmem_ld32(taddr + col, v);
+          tmem_wait_ld_dep(v);
+        }
+        if (!in) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = live ? v[e] : 0.f;
+        if (c.split) {
+          float* sum = acc32 + ((size_t)k.head * p.T + i) * p.D + col;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            if (col + e >= p.D) break;
+            float4* at = reinterpret_cast<float4*>(sum + e);
+            if (!first) {
+              const float4 o = *at;
+              v[e] += o.x;
+              v[e + 1] += o.y;
+              v[e + 2] += o.z;
+              v[e + 3] += o.w;
+            }
+            if (!last) *at = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+          if (!last) continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (col + e >= p.D) break;
+          *reinterpret_cast<uint4*>(row + col + e) =
+              make_uint4(pack2t<BF16>(v[e] * p.sc, v[e + 1] * p.sc),
+                         pack2t<BF16>(v[e + 2] * p.sc, v[e + 3] * p.sc),
+                         pack2t<BF16>(v[e + 4] * p.sc, v[e + 5] * p.sc),
+                         pack2t<BF16>(v[e + 6] * p.sc, v[e + 7] * p.sc));
+        }
+      }
+      if (any) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&misc->acc_empty[ab]);
+        ++it;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+long long fb_tiles_per_head(const AttnProblem& p) {
+  const long long n_t = (p.T + kBM - 1) / kBM;
+  return p.causal ? n_t * (n_t + 1) / 2 : n_t * n_t;
+}
+
+// How the backward is cut: `per` whole kv groups a launch, or, when one
+// group's dS tiles exceed the buffer's upper bound, `keys` key tiles of one group.
+struct FbPlan {
+  int per, keys;
+  long long tiles;    // dS tiles that the buffer holds
+  bool split;
+};
+FbPlan fb_plan(const AttnProblem& p) {
+  const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
+  const long long cap = kDBufCapBytes / (kDTileElems * 2);
+  const long long group = (long long)G * fb_tiles_per_head(p);
+  if (group <= cap) {
+    // as few launches as fit, of near-equal size
+    const long long most = std::min<long long>(groups, cap / group);
+    const int n = (int)((groups + most - 1) / most), per = (groups + n - 1) / n;
+    return FbPlan{per, n_t, per * group, false};
+  }
+  const long long col = (long long)G * n_t;
+  const int keys = (int)std::max<long long>(1, std::min<long long>(n_t, cap / col));
+  return FbPlan{1, keys, keys * col, true};
+}
+
+template <int D, bool BF16, bool MASKED>
+cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
+                              float* stats, uint16_t* dsbuf, float* acc32, cudaStream_t st) {
+  CUtensorMap mq, mk, mv, mdo;
+  if (!attn_map(&mq, t.q, p, p.Hq, t.sq) || !attn_map(&mk, t.k, p, p.Hkv, t.sk) ||
+      !attn_map(&mv, t.v, p, p.Hkv, t.sv) || !attn_map(&mdo, t.dout, p, p.Hq, t.sdo))
+    return cudaErrorInvalidValue;
+  auto kkv = attn_sm100_dkv_kernel<D, BF16, MASKED>;
+  auto kq = attn_sm100_dq_kernel<D, BF16, MASKED>;
+  cudaError_t e;
+  int dev = 0, num_sms = 0;
+  if ((e = prep(kkv, FbLayout<D>::BYTES)) != cudaSuccess ||
+      (e = prep(kq, FqLayout<D>::BYTES)) != cudaSuccess ||
+      (e = cudaGetDevice(&dev)) != cudaSuccess ||
+      (e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
+    return e;
+  const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
+  attn_sm100_delta_kernel<<<p.B * p.Hq * n_t, 256, 0, st>>>(p, t, bits, stats);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const FbPlan plan = fb_plan(p);
+  const long long group_bytes = 4ll * G * p.T * p.D;   // queries and dO
+  for (int g0 = 0; g0 < groups; g0 += plan.per)
+    for (int j0 = 0; j0 < n_t; j0 += plan.keys) {
+      FbChunk c{};
+      c.g0 = g0;
+      c.g1 = std::min(groups, g0 + plan.per);
+      c.j0 = j0;
+      c.j1 = std::min(n_t, j0 + plan.keys);
+      c.split = plan.split;
+      c.band = (int)std::max<long long>(
+          1, std::min<long long>(c.g1 - g0, (64ll << 20) / std::max<long long>(group_bytes, 1)));
+      const int i0 = p.causal ? j0 : 0;
+      c.tph = plan.split ? (long long)(n_t - i0) * (c.j1 - j0) : fb_tiles_per_head(p);
+      kkv<<<(c.g1 - g0) * (c.j1 - j0), kFbThreads, FbLayout<D>::BYTES, st>>>(
+          mq, mk, mv, mdo, p, t, c, bits, stats, dsbuf);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      const int work = (c.g1 - g0) * G * (n_t - i0);
+      kq<<<std::min(work, num_sms), kFqThreads, FqLayout<D>::BYTES, st>>>(mk, p, t, c, bits, dsbuf,
+                                                                          acc32);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+  return cudaSuccess;
+}
+
 bool attn_readable(const void* x, const TensorStrides& s) {
   return reinterpret_cast<uintptr_t>(x) % 16 == 0 && s.b > 0 && s.h > 0 && s.t > 0 &&
          s.b % 8 == 0 && s.h % 8 == 0 && s.t % 8 == 0;
@@ -421,6 +1201,40 @@ bool attn_readable(const void* x, const TensorStrides& s) {
 bool attn_sm100_supports(const AttnProblem& p, const AttnTensors& t) {
   return p.D <= 128 && attn_readable(t.q, t.sq) && attn_readable(t.k, t.sk) &&
          attn_readable(t.v, t.sv) && attn_readable(t.out, t.so);
+}
+
+bool attn_sm100_backward_supports(const AttnProblem& p, const AttnTensors& t) {
+  return attn_sm100_supports(p, t) && attn_readable(t.dout, t.sdo) && attn_readable(t.dq, t.sdq) &&
+         attn_readable(t.dk, t.sdk) && attn_readable(t.dv, t.sdv);
+}
+
+size_t attn_stats_bytes(const AttnProblem& p) {
+  return (size_t)p.B * p.Hq * ((p.T + kBM - 1) / kBM) * kFbStatBytes;
+}
+
+size_t attn_sm100_ds_bytes(const AttnProblem& p) {
+  return p.D <= 128 ? (size_t)fb_plan(p).tiles * kDTileElems * 2 : 0;
+}
+
+size_t attn_sm100_acc_bytes(const AttnProblem& p) {
+  return p.D <= 128 && fb_plan(p).split ? (size_t)(p.Hq / p.Hkv) * p.T * p.D * 4 : 0;
+}
+
+cudaError_t launch_attn_sm100_backward(const AttnProblem& p, const AttnTensors& t,
+                                       const uint32_t* bits, float* stats, void* ds, float* acc,
+                                       cudaStream_t st) {
+  uint16_t* d = static_cast<uint16_t*>(ds);
+  const bool bf = p.dtype == LKL_BF16;
+  if (tc_dim(p.D) == 64) {
+    if (bits) return bf ? run_attn_backward<64, true, true>(p, t, bits, stats, d, acc, st)
+                        : run_attn_backward<64, false, true>(p, t, bits, stats, d, acc, st);
+    return bf ? run_attn_backward<64, true, false>(p, t, bits, stats, d, acc, st)
+              : run_attn_backward<64, false, false>(p, t, bits, stats, d, acc, st);
+  }
+  if (bits) return bf ? run_attn_backward<128, true, true>(p, t, bits, stats, d, acc, st)
+                      : run_attn_backward<128, false, true>(p, t, bits, stats, d, acc, st);
+  return bf ? run_attn_backward<128, true, false>(p, t, bits, stats, d, acc, st)
+            : run_attn_backward<128, false, false>(p, t, bits, stats, d, acc, st);
 }
 
 cudaError_t launch_attn_sm100_forward(const AttnProblem& p, const AttnTensors& t,

@@ -32,8 +32,18 @@ AttnProblem to_attn(const lkl_attn_problem* p) {
 inline size_t attn_bits_bytes(const lkl_attn_problem* p) {
   return round256((size_t)p->B * (size_t)((p->T + 31) / 32) * sizeof(uint32_t));
 }
-inline size_t attn_rows_bytes(const lkl_attn_problem* p) {
-  return round256((size_t)p->B * p->Hq * p->T * sizeof(float2));
+// Backward scratch: [mask bits][row statistics][fp32 dq sums][dS tiles].
+struct AttnScratch {
+  size_t stats, acc, ds, total;   // offsets of the last three, and the end
+};
+AttnScratch attn_scratch(const lkl_attn_problem* p, bool has_mask) {
+  const AttnProblem a = to_attn(p);
+  AttnScratch s;
+  s.stats = has_mask ? attn_bits_bytes(p) : 0;
+  s.acc = s.stats + round256(lkl::attn_stats_bytes(a));
+  s.ds = s.acc + round256(lkl::attn_sm100_acc_bytes(a));
+  s.total = s.ds + round256(lkl::attn_sm100_ds_bytes(a));
+  return s;
 }
 
 // Strides of tensor `which` (`strides` or the contiguous ones).
@@ -106,7 +116,7 @@ size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_ma
 
 size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask) {
   if (check_attn(p) != LKL_OK || p->B == 0 || p->T == 0) return 0;
-  return (has_mask ? attn_bits_bytes(p) : 0) + attn_rows_bytes(p);
+  return attn_scratch(p, has_mask != 0).total;
 }
 
 int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_strides* strides,
@@ -157,8 +167,8 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint32_t* bits;
   if ((s = attn_bits(p, mask, ws, &bits, st))) return s;
-  float2* rows = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) +
-                                           (mask ? attn_bits_bytes(p) : 0));
+  const AttnScratch at = attn_scratch(p, mask != nullptr);
+  uint8_t* const base = static_cast<uint8_t*>(ws);
   AttnTensors t{};
   t.q = q, t.k = k, t.v = v, t.out = const_cast<void*>(out), t.lse = const_cast<float*>(lse);
   t.dout = dout, t.dq = dq, t.dk = dk, t.dv = dv;
@@ -171,8 +181,13 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   t.sdk = attn_strides(strides, LKL_ATTN_DK, p);
   t.sdv = attn_strides(strides, LKL_ATTN_DV, p);
   const AttnProblem a = to_attn(p);
+  t_last_path = !g_force_generic.load() && lkl::attn_sm100_backward_supports(a, t) ? 1 : 0;
+  if (t_last_path)
+    return launch_status(lkl::launch_attn_sm100_backward(
+        a, t, bits, reinterpret_cast<float*>(base + at.stats), base + at.ds,
+        reinterpret_cast<float*>(base + at.acc), st));
+  float2* rows = reinterpret_cast<float2*>(base + at.stats);
   if ((s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;
-  t_last_path = 0;
   return launch_status(lkl::launch_attn_generic_backward(a, t, bits, rows, st));
 }
 
