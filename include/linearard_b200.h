@@ -341,10 +341,13 @@ enum lkl_attn_tensor {
 /* Bytes of scratch of the forward (the packed mask; 0 without one). */
 size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);
 
-/* Bytes of scratch of the backward: the packed mask, 8 bytes per (batch, head,
- * row) and, on the tensor cores, the 16-bit dS tiles that the key-stationary
+/* Bytes of scratch of the backward: the packed mask, 1 KB per (batch, head,
+ * 128 rows) and, on the tensor cores, the 16-bit dS tiles that the key-stationary
  * launch hands to the dq launch: all of them up to 8 GiB, beyond that the
- * backward runs in chunks. */
+ * backward runs in chunks of kv heads or, where one kv head's query heads need
+ * more, of key tiles.  Less also works, in more chunks, down to the dS tiles of
+ * one key tile ((Hq / Hkv) * ceil(T / 128) tiles of 32 KB) and one kv head's dq in fp32; below that
+ * LKL_ERR_WORKSPACE. */
 size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);
 
 int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_strides* strides,

@@ -37,13 +37,16 @@ bool attn_sm100_supports(const AttnProblem& p, const AttnTensors& t);
 cudaError_t launch_attn_sm100_forward(const AttnProblem& p, const AttnTensors& t,
                                       const uint32_t* bits, cudaStream_t st);
 bool attn_sm100_backward_supports(const AttnProblem& p, const AttnTensors& t);
-// Scratch of the backward: row statistics (either path), dS tiles, and the fp32
-// dq of one kv group's heads where its dS tiles take several launches.
+// Scratch of the backward: row statistics (either path); dS tiles: what it asks
+// for, the least it runs with, and what holds one kv group (below that, dq is
+// summed over launches in attn_sm100_acc_bytes of fp32).
 size_t attn_stats_bytes(const AttnProblem& p);
 size_t attn_sm100_ds_bytes(const AttnProblem& p);
+size_t attn_sm100_ds_min_bytes(const AttnProblem& p);
+size_t attn_sm100_group_bytes(const AttnProblem& p);
 size_t attn_sm100_acc_bytes(const AttnProblem& p);
 cudaError_t launch_attn_sm100_backward(const AttnProblem& p, const AttnTensors& t,
-                                       const uint32_t* bits, float* stats, void* ds, float* acc,
-                                       cudaStream_t st);
+                                       const uint32_t* bits, float* stats, void* ds,
+                                       size_t ds_bytes, float* acc, cudaStream_t st);
 
 }  // namespace lkl

@@ -1125,31 +1125,31 @@ long long fb_tiles_per_head(const AttnProblem& p) {
   return p.causal ? n_t * (n_t + 1) / 2 : n_t * n_t;
 }
 
-// How the backward is cut: `per` whole kv groups a launch, or, when one
-// group's dS tiles exceed the buffer's upper bound, `keys` key tiles of one group.
+// How the backward is cut: `per` whole kv groups a launch, or, where the buffer
+// does not hold one group's dS tiles, `keys` key tiles of one group (split).
 struct FbPlan {
   int per, keys;
-  long long tiles;    // dS tiles that the buffer holds
   bool split;
 };
-FbPlan fb_plan(const AttnProblem& p) {
+FbPlan fb_plan(const AttnProblem& p, long long cap_tiles) {
   const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
-  const long long cap = kDBufCapBytes / (kDTileElems * 2);
   const long long group = (long long)G * fb_tiles_per_head(p);
-  if (group <= cap) {
+  if (group <= cap_tiles) {
     // as few launches as fit, of near-equal size
-    const long long most = std::min<long long>(groups, cap / group);
-    const int n = (int)((groups + most - 1) / most), per = (groups + n - 1) / n;
-    return FbPlan{per, n_t, per * group, false};
+    const long long most = std::min<long long>(groups, cap_tiles / group);
+    const int n = (int)((groups + most - 1) / most);
+    return FbPlan{(groups + n - 1) / n, n_t, false};
   }
-  const long long col = (long long)G * n_t;
-  const int keys = (int)std::max<long long>(1, std::min<long long>(n_t, cap / col));
-  return FbPlan{1, keys, keys * col, true};
+  const long long keys = cap_tiles / ((long long)G * n_t);
+  return FbPlan{1, (int)std::min<long long>(n_t, keys), true};
 }
 
 template <int D, bool BF16, bool MASKED>
 cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
-                              float* stats, uint16_t* dsbuf, float* acc32, cudaStream_t st) {
+                              float* stats, uint16_t* dsbuf, size_t ds_bytes, float* acc32,
+                              cudaStream_t st) {
+  const FbPlan plan = fb_plan(p, (long long)(ds_bytes / (kDTileElems * 2)));
+  if (plan.keys <= 0) return cudaErrorInvalidValue;
   CUtensorMap mq, mk, mv, mdo;
   if (!attn_map(&mq, t.q, p, p.Hq, t.sq) || !attn_map(&mk, t.k, p, p.Hkv, t.sk) ||
       !attn_map(&mv, t.v, p, p.Hkv, t.sv) || !attn_map(&mdo, t.dout, p, p.Hq, t.sdo))
@@ -1166,7 +1166,6 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
   const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
   attn_sm100_delta_kernel<<<p.B * p.Hq * n_t, 256, 0, st>>>(p, t, bits, stats);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const FbPlan plan = fb_plan(p);
   const long long group_bytes = 4ll * G * p.T * p.D;   // queries and dO
   for (int g0 = 0; g0 < groups; g0 += plan.per)
     for (int j0 = 0; j0 < n_t; j0 += plan.keys) {
@@ -1212,29 +1211,38 @@ size_t attn_stats_bytes(const AttnProblem& p) {
   return (size_t)p.B * p.Hq * ((p.T + kBM - 1) / kBM) * kFbStatBytes;
 }
 
+size_t attn_sm100_group_bytes(const AttnProblem& p) {
+  return (size_t)(p.Hq / p.Hkv) * fb_tiles_per_head(p) * kDTileElems * 2;
+}
+
 size_t attn_sm100_ds_bytes(const AttnProblem& p) {
-  return p.D <= 128 ? (size_t)fb_plan(p).tiles * kDTileElems * 2 : 0;
+  const long long all = fb_tiles_per_head(p) * p.B * p.Hq * kDTileElems * 2;
+  const long long min = (long long)attn_sm100_ds_min_bytes(p);
+  return (size_t)std::min(all, std::max(kDBufCapBytes, min));
+}
+
+size_t attn_sm100_ds_min_bytes(const AttnProblem& p) {
+  return (size_t)(p.Hq / p.Hkv) * ((p.T + kBM - 1) / kBM) * kDTileElems * 2;
 }
 
 size_t attn_sm100_acc_bytes(const AttnProblem& p) {
-  return p.D <= 128 && fb_plan(p).split ? (size_t)(p.Hq / p.Hkv) * p.T * p.D * 4 : 0;
+  return (size_t)(p.Hq / p.Hkv) * p.T * p.D * 4;
 }
 
 cudaError_t launch_attn_sm100_backward(const AttnProblem& p, const AttnTensors& t,
-                                       const uint32_t* bits, float* stats, void* ds, float* acc,
-                                       cudaStream_t st) {
+                                       const uint32_t* bits, float* stats, void* ds,
+                                       size_t ds_bytes, float* acc, cudaStream_t st) {
   uint16_t* d = static_cast<uint16_t*>(ds);
   const bool bf = p.dtype == LKL_BF16;
+  auto run = [&](auto k) { return k(p, t, bits, stats, d, ds_bytes, acc, st); };
   if (tc_dim(p.D) == 64) {
-    if (bits) return bf ? run_attn_backward<64, true, true>(p, t, bits, stats, d, acc, st)
-                        : run_attn_backward<64, false, true>(p, t, bits, stats, d, acc, st);
-    return bf ? run_attn_backward<64, true, false>(p, t, bits, stats, d, acc, st)
-              : run_attn_backward<64, false, false>(p, t, bits, stats, d, acc, st);
+    if (bits) return bf ? run(run_attn_backward<64, true, true>)
+                        : run(run_attn_backward<64, false, true>);
+    return bf ? run(run_attn_backward<64, true, false>) : run(run_attn_backward<64, false, false>);
   }
-  if (bits) return bf ? run_attn_backward<128, true, true>(p, t, bits, stats, d, acc, st)
-                      : run_attn_backward<128, false, true>(p, t, bits, stats, d, acc, st);
-  return bf ? run_attn_backward<128, true, false>(p, t, bits, stats, d, acc, st)
-            : run_attn_backward<128, false, false>(p, t, bits, stats, d, acc, st);
+  if (bits) return bf ? run(run_attn_backward<128, true, true>)
+                      : run(run_attn_backward<128, false, true>);
+  return bf ? run(run_attn_backward<128, true, false>) : run(run_attn_backward<128, false, false>);
 }
 
 cudaError_t launch_attn_sm100_forward(const AttnProblem& p, const AttnTensors& t,

@@ -32,18 +32,24 @@ AttnProblem to_attn(const lkl_attn_problem* p) {
 inline size_t attn_bits_bytes(const lkl_attn_problem* p) {
   return round256((size_t)p->B * (size_t)((p->T + 31) / 32) * sizeof(uint32_t));
 }
-// Backward scratch: [mask bits][row statistics][fp32 dq sums][dS tiles].
+// Backward scratch: [mask bits][row statistics][fp32 dq sums][dS tiles]; the
+// sums only where the tiles of one kv group do not fit at once.
 struct AttnScratch {
-  size_t stats, acc, ds, total;   // offsets of the last three, and the end
+  size_t stats, acc, ds, ds_bytes;   // offsets, and the bytes left for dS
 };
-AttnScratch attn_scratch(const lkl_attn_problem* p, bool has_mask) {
+AttnScratch attn_scratch(const lkl_attn_problem* p, bool has_mask, size_t ws_bytes) {
   const AttnProblem a = to_attn(p);
   AttnScratch s;
   s.stats = has_mask ? attn_bits_bytes(p) : 0;
-  s.acc = s.stats + round256(lkl::attn_stats_bytes(a));
-  s.ds = s.acc + round256(lkl::attn_sm100_acc_bytes(a));
-  s.total = s.ds + round256(lkl::attn_sm100_ds_bytes(a));
+  s.acc = s.ds = s.stats + round256(lkl::attn_stats_bytes(a));
+  if (ws_bytes < s.ds + lkl::attn_sm100_group_bytes(a))
+    s.ds += round256(lkl::attn_sm100_acc_bytes(a));
+  s.ds_bytes = ws_bytes > s.ds ? ws_bytes - s.ds : 0;
   return s;
+}
+// What the CUDA-core backward needs; the tensor cores' add dS tiles.
+size_t attn_backward_base(const lkl_attn_problem* p, bool has_mask) {
+  return attn_scratch(p, has_mask, SIZE_MAX).ds;
 }
 
 // Strides of tensor `which` (`strides` or the contiguous ones).
@@ -116,7 +122,12 @@ size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_ma
 
 size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask) {
   if (check_attn(p) != LKL_OK || p->B == 0 || p->T == 0) return 0;
-  return attn_scratch(p, has_mask != 0).total;
+  const AttnProblem a = to_attn(p);
+  size_t n = attn_backward_base(p, has_mask != 0);
+  if (a.D > 128) return n;
+  const size_t ds = lkl::attn_sm100_ds_bytes(a);
+  if (ds < lkl::attn_sm100_group_bytes(a)) n += round256(lkl::attn_sm100_acc_bytes(a));
+  return n + round256(ds);
 }
 
 int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_strides* strides,
@@ -161,14 +172,7 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   if (!aligned(lse, 4)) return LKL_ERR_MISALIGNED;
   if (dq == dk || dq == dv || dk == dv) return LKL_ERR_BAD_ALIAS;
   if ((s = check_mask(mask, p->mask_dtype)) || (s = check_attn_strides(strides, 8))) return s;
-  if ((s = check_workspace(lkl_attn_backward_workspace_size(p, mask != nullptr), ws, ws_bytes)))
-    return s;
-  if (!bind_device_of(q) || !device_is_sm100()) return LKL_ERR_NO_DEVICE;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  uint32_t* bits;
-  if ((s = attn_bits(p, mask, ws, &bits, st))) return s;
-  const AttnScratch at = attn_scratch(p, mask != nullptr);
-  uint8_t* const base = static_cast<uint8_t*>(ws);
+  if ((s = check_workspace(attn_backward_base(p, mask != nullptr), ws, ws_bytes))) return s;
   AttnTensors t{};
   t.q = q, t.k = k, t.v = v, t.out = const_cast<void*>(out), t.lse = const_cast<float*>(lse);
   t.dout = dout, t.dq = dq, t.dk = dk, t.dv = dv;
@@ -181,10 +185,19 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   t.sdk = attn_strides(strides, LKL_ATTN_DK, p);
   t.sdv = attn_strides(strides, LKL_ATTN_DV, p);
   const AttnProblem a = to_attn(p);
-  t_last_path = !g_force_generic.load() && lkl::attn_sm100_backward_supports(a, t) ? 1 : 0;
-  if (t_last_path)
+  const bool tc = !g_force_generic.load() && lkl::attn_sm100_backward_supports(a, t);
+  const AttnScratch at = attn_scratch(p, mask != nullptr, ws_bytes);
+  if (tc && at.ds_bytes < lkl::attn_sm100_ds_min_bytes(a)) return LKL_ERR_WORKSPACE;
+  if (!bind_device_of(q) || !device_is_sm100()) return LKL_ERR_NO_DEVICE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint32_t* bits;
+  if ((s = attn_bits(p, mask, ws, &bits, st))) return s;
+  uint8_t* const base = static_cast<uint8_t*>(ws);
+  t_last_path = tc ? 1 : 0;
+  if (tc)
     return launch_status(lkl::launch_attn_sm100_backward(
         a, t, bits, reinterpret_cast<float*>(base + at.stats), base + at.ds,
+        std::min(at.ds_bytes, lkl::attn_sm100_ds_bytes(a)),
         reinterpret_cast<float*>(base + at.acc), st));
   float2* rows = reinterpret_cast<float2*>(base + at.stats);
   if ((s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;

@@ -227,6 +227,49 @@ def test_rows_behind_the_tensor_stay():
     assert (lse[B * H * T:] == 7).all() and (ws[nb:] == 9).all()
 
 
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (4, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("mask", [False, True])
+def test_chunks_of_the_backward(Hq, Hkv, causal, mask):
+    """Less scratch than asked for: fewer kv heads a launch, then key tiles of one
+    kv head with dq summed over launches.  dk and dv keep their bits; dq is summed in
+    another order."""
+    import ctypes
+
+    from linearard_b200 import _lib
+    from linearard_b200.attention import recompute as R
+    B, T, D = 2, 700, 128
+    q, k, v, g = make(B, Hq, Hkv, T, D, "bf16", "bhtd")
+    m = right_pad(B, T, [700, 290]) if mask else None
+    out, lse = attn_forward(q, k, v, m, causal)
+    want = attn_backward(g, q, k, v, out, lse, m, causal)
+    ref = AttnRef(q, k, v, m, causal, None, g)
+    prob = R._problem(q, k, causal, _lib.LKL_MASK_I64, None)
+    L = _lib.lib()
+    full = L.lkl_attn_backward_workspace_size(ctypes.byref(prob), int(mask))
+    n_t, G = 6, Hq // Hkv
+    tiles = n_t * (n_t + 1) // 2 if causal else n_t * n_t
+    base = full - B * Hq * tiles * 32768
+    acc = G * T * D * 4
+    sizes = [full, base + 3 * G * tiles * 32768, base + G * tiles * 32768,
+             base + acc + 4 * G * n_t * 32768, base + acc + 2 * G * n_t * 32768,
+             base + acc + G * n_t * 32768]
+    for n in sizes:
+        ws = torch.full((n + 256,), 0xFF, dtype=torch.uint8, device="cuda")
+        grads = [torch.empty_like(t) for t in (q, k, v)]
+        st = L.lkl_attn_backward(*(R.ptr(t) for t in (q, k, v, out, lse, g)), None, R.ptr(m),
+                                 ctypes.byref(prob), *(R.ptr(t) for t in grads), R.ptr(ws), n,
+                                 R.stream_of(q.device))
+        assert st == 0
+        assert (ws[n:] == 0xFF).all()
+        assert torch.equal(grads[1], want[1]) and torch.equal(grads[2], want[2])
+        assert_within(grads[0], ref.dq, ref.dq_tol, "dq")
+    assert L.lkl_attn_backward(*(R.ptr(t) for t in (q, k, v, out, lse, g)), None, R.ptr(m),
+                               ctypes.byref(prob), *(R.ptr(t) for t in grads), R.ptr(ws),
+                               sizes[-1] - 256, R.stream_of(q.device)) == 6
+    check_device_status()
+
+
 def test_captured_and_replayed():
     q, k, v, g = make(1, 4, 2, 300, 128, "bf16")
     m = right_pad(1, 300, [211])
