@@ -140,9 +140,9 @@ def _declare(L):
         getattr(L, name).restype = _sz
         getattr(L, name).argtypes = [_A, _i32]
     L.lkl_attn_forward.restype = _i32
-    L.lkl_attn_forward.argtypes = [_vp, _vp, _vp, _S, _vp, _A, _vp, _vp, _vp, _sz, _vp]
+    L.lkl_attn_forward.argtypes = [_vp, _vp, _vp, _vp, _vp, _A, _vp, _vp, _vp, _sz, _vp]
     L.lkl_attn_backward.restype = _i32
-    L.lkl_attn_backward.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _S, _vp, _A, _vp, _vp, _vp, _vp,
+    L.lkl_attn_backward.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _A, _vp, _vp, _vp, _vp,
                                     _sz, _vp]
     L.lkl_token_logprobs.restype = _i32
     L.lkl_token_logprobs.argtypes = [_vp, _R, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp]

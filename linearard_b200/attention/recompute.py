@@ -22,8 +22,9 @@ import ctypes
 import torch
 
 from .. import _lib
+from .._marshal import on_device, once_when_recorded, raw_stream
 from ..attention_KL._common import (_DT, SUPPORTED_HEAD_DIMS, TC_HEAD_DIMS, check_lse,
-                                    prepare_mask, ptr, scale_of, stream_of)
+                                    prepare_mask, scale_of)
 
 __all__ = ["attn", "attn_forward", "attn_backward", "AttnFn"]
 
@@ -32,47 +33,46 @@ def _check(q, k, v):
     for name, t in (("q", q), ("k", k), ("v", v)):
         assert isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor"
         assert t.is_cuda, "q/k/v must be on CUDA"
-        assert t.dtype in (torch.float16, torch.bfloat16), f"{name} dtype supports only fp16/bf16"
+        assert t.dtype in _DT, f"{name} dtype supports only fp16/bf16"
         assert t.ndim == 4, f"{name} shape must be [B,H,T,D]"
         assert t.stride(-1) == 1, f"{name} last-dim stride must be 1"
     assert q.dtype == k.dtype == v.dtype, "q/k/v dtype must match"
     assert q.device == k.device == v.device, "q/k/v must be on the same device"
-    assert k.shape == v.shape, "k/v shape must match"
-    assert (k.shape[0], k.shape[2], k.shape[3]) == (q.shape[0], q.shape[2], q.shape[3]), \
-        "q/k B/T/D must match"
-    assert k.shape[1] > 0 and q.shape[1] > 0, "there must be a head"
-    assert q.shape[1] % k.shape[1] == 0, "Hq must be divisible by Hkv"
-    assert q.shape[3] in SUPPORTED_HEAD_DIMS, "head_dim is not in the supported set"
-
-
-def _scale(sm_scale, D):
-    sc = scale_of(sm_scale, D, "sm_scale")
-    assert 0.0 < sc < float("inf"), "sm_scale must be positive"
-    return sc
+    (B, Hq, T, D), (Bk, Hkv, Tk, Dk) = q.shape, k.shape
+    assert v.shape == k.shape, "k/v shape must match"
+    assert (B, T, D) == (Bk, Tk, Dk), "q/k B/T/D must match"
+    assert Hkv > 0 and Hq > 0, "there must be a head"
+    assert Hq % Hkv == 0, "Hq must be divisible by Hkv"
+    assert D in SUPPORTED_HEAD_DIMS, "head_dim is not in the supported set"
 
 
 def _problem(q, k, causal, mask_dtype, sm_scale):
     B, Hq, T, D = q.shape
-    return _lib.LKLAttnProblem(B=B, Hq=Hq, Hkv=k.shape[1], T=T, D=D, dtype=_DT[q.dtype],
-                               causal=1 if causal else 0, mask_dtype=mask_dtype,
-                               sm_scale=_scale(sm_scale, D))
+    sc = scale_of(sm_scale, D, "sm_scale")
+    assert 0.0 < sc < float("inf"), "sm_scale must be positive"
+    return _lib.LKLAttnProblem(B, Hq, k.shape[1], T, D, _DT[q.dtype], 1 if causal else 0,
+                               mask_dtype, sc)
 
 
-def _stride(t):
+def _strides(t):
     """Element strides (b, h, t); a dim of size 1 gets one that any path can read."""
-    b, h, n = (t.stride(i) if t.shape[i] != 1 else t.shape[3] for i in range(3))
-    return _lib.LKLStrides(b=b, h=h, t=n)
+    (b, h, n, _), (B, H, T, D) = t.stride(), t.shape
+    return (b if B != 1 else D, h if H != 1 else D, n if T != 1 else D)
 
 
 def _readable(t):
-    """`t`, or a contiguous copy where the tensor-core kernels cannot read it in
-    place (their CUDA-core counterparts could, many times slower)."""
+    """(tensor, strides): t itself, or a contiguous copy where the tensor-core
+    kernels cannot read it in place (the CUDA-core ones could, many times slower)."""
+    s = _strides(t)
+    unit = t.stride(3) == 1
     if t.shape[3] in TC_HEAD_DIMS:
-        s = _stride(t)
-        if (t.data_ptr() % 16 or t.stride(3) != 1
-                or any(x <= 0 or x % 8 for x in (s.b, s.h, s.t))):
-            return t.clone(memory_format=torch.contiguous_format)
-    return t if t.stride(3) == 1 else t.contiguous()
+        b, h, n = s
+        unit = (unit and b > 0 and h > 0 and n > 0 and (b | h | n) % 8 == 0
+                and t.data_ptr() % 16 == 0)
+    if unit:
+        return t, s
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _strides(t)
 
 
 def _like(t):
@@ -83,33 +83,59 @@ def _like(t):
     return torch.empty((B, H, T, D), device=t.device, dtype=t.dtype)
 
 
-def _strides(*tensors):
-    return (_lib.LKLStrides * len(tensors))(*[_stride(t) for t in tensors])
-
-
 def _workspace(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    """(tensor to hold, its address)"""
+    if not n:
+        return None, None
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr()
+
+
+def _forward(q, k, v, mask, prob):
+    """out and lse of checked arguments; mask on the device or None."""
+    L, dev = _lib.lib(), q.device
+    with on_device(dev):
+        (q, sq), (k, sk), (v, sv) = _readable(q), _readable(k), _readable(v)
+        out = _like(q)
+        lse = torch.empty((prob.B, prob.Hq, prob.T), device=dev, dtype=torch.float32)
+        ref = ctypes.byref(prob)
+        n, ws, at = 0, None, None
+        if mask is not None:
+            n = L.lkl_attn_forward_workspace_size(ref, 1)
+            ws, at = _workspace(n, dev)
+        st = L.lkl_attn_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                (ctypes.c_int64 * 12)(*sq, *sk, *sv, *_strides(out)),
+                                None if mask is None else mask.data_ptr(), ref, out.data_ptr(),
+                                lse.data_ptr(), at, n, raw_stream(dev))
+    _lib.check(st, "lkl_attn_forward")
+    return out, lse
+
+
+def _backward(dout, q, k, v, out, lse, mask, prob):
+    L, dev = _lib.lib(), q.device
+    with on_device(dev):
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        (q, sq), (k, sk), (v, sv), (out, so), (dout, sd) = (_readable(t)
+                                                            for t in (q, k, v, out, dout))
+        ref = ctypes.byref(prob)
+        n = L.lkl_attn_backward_workspace_size(ref, 0 if mask is None else 1)
+        ws, at = _workspace(n, dev)
+        st = L.lkl_attn_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            dout.data_ptr(), (ctypes.c_int64 * 24)(*sq, *sk, *sv, *so, *sd, *_strides(dq),
+                                                   *_strides(dk), *_strides(dv)),
+            None if mask is None else mask.data_ptr(), ref, dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), at, n, raw_stream(dev))
+    _lib.check(st, "lkl_attn_backward")
+    return dq, dk, dv
 
 
 def attn_forward(q, k, v, attn_mask=None, causal=True, sm_scale=None):
     """q [B,Hq,T,D], k and v [B,Hkv,T,D] -> (out [B,Hq,T,D], lse [B,Hq,T] fp32).
     Rows that the mask removes have out 0 and lse 0."""
     _check(q, k, v)
-    B, Hq, T, _ = q.shape
-    mask, mdt = prepare_mask(attn_mask, B, T, q.device)
-    prob = _problem(q, k, causal, mdt, sm_scale)
-    L = _lib.lib()
-    with torch.cuda.device(q.device):
-        q, k, v = _readable(q), _readable(k), _readable(v)
-        out = _like(q)
-        lse = torch.empty((B, Hq, T), device=q.device, dtype=torch.float32)
-        n = int(L.lkl_attn_forward_workspace_size(ctypes.byref(prob), 1 if mask is not None else 0))
-        ws = _workspace(n, q.device)
-        st = L.lkl_attn_forward(ptr(q), ptr(k), ptr(v), _strides(q, k, v, out), ptr(mask),
-                                ctypes.byref(prob), ptr(out), ptr(lse), ptr(ws), n,
-                                stream_of(q.device))
-    _lib.check(st, "lkl_attn_forward")
-    return out, lse
+    mask, mdt = prepare_mask(attn_mask, q.shape[0], q.shape[2], q.device)
+    return _forward(q, k, v, mask, _problem(q, k, causal, mdt, sm_scale))
 
 
 def attn_backward(dout, q, k, v, out, lse, attn_mask=None, causal=True, sm_scale=None):
@@ -120,42 +146,25 @@ def attn_backward(dout, q, k, v, out, lse, attn_mask=None, causal=True, sm_scale
         assert isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor"
         assert t.shape == q.shape and t.dtype == q.dtype and t.device == q.device, \
             f"{name} must have the shape, dtype and device of q"
-    B, Hq, T, _ = q.shape
-    check_lse(lse, (B, Hq, T))
+    check_lse(lse, q.shape[:3])
     assert lse.device == q.device, "lse must be on the device of q"
-    mask, mdt = prepare_mask(attn_mask, B, T, q.device)
-    prob = _problem(q, k, causal, mdt, sm_scale)
-    L = _lib.lib()
-    with torch.cuda.device(q.device):
-        dq, dk, dv = _like(q), _like(k), _like(v)
-        q, k, v, out, dout = (_readable(t) for t in (q, k, v, out, dout))
-        n = int(L.lkl_attn_backward_workspace_size(ctypes.byref(prob),
-                                                   1 if mask is not None else 0))
-        ws = _workspace(n, q.device)
-        st = L.lkl_attn_backward(ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(dout),
-                                 _strides(q, k, v, out, dout, dq, dk, dv), ptr(mask),
-                                 ctypes.byref(prob), ptr(dq), ptr(dk), ptr(dv), ptr(ws), n,
-                                 stream_of(q.device))
-    _lib.check(st, "lkl_attn_backward")
-    return dq, dk, dv
+    mask, mdt = prepare_mask(attn_mask, q.shape[0], q.shape[2], q.device)
+    return _backward(dout, q, k, v, out, lse, mask, _problem(q, k, causal, mdt, sm_scale))
 
 
 class AttnFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, attn_mask, causal: bool, sm_scale):
-        _check(q, k, v)
-        mask, _ = prepare_mask(attn_mask, q.shape[0], q.shape[2], q.device)
-        out, lse = attn_forward(q, k, v, mask, causal, sm_scale)
+    def forward(ctx, q, k, v, mask, prob):
+        out, lse = _forward(q, k, v, mask, prob)
         ctx.save_for_backward(q, k, v, out, lse, mask)
-        ctx.causal, ctx.sm_scale = causal, sm_scale
+        ctx.prob = prob
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_when_recorded
     def backward(ctx, dout):
         q, k, v, out, lse, mask = ctx.saved_tensors
-        dq, dk, dv = attn_backward(dout, q, k, v, out, lse, mask, ctx.causal, ctx.sm_scale)
-        return dq, dk, dv, None, None, None
+        dq, dk, dv = _backward(dout, q, k, v, out, lse, mask, ctx.prob)
+        return dq, dk, dv, None, None
 
 
 def attn(q, k, v, attn_mask=None, causal=True, sm_scale=None):
@@ -164,4 +173,6 @@ def attn(q, k, v, attn_mask=None, causal=True, sm_scale=None):
     where they are not multiples of 8 elements); attn_mask: [B,T], nonzero =
     token, or None; sm_scale: default 1/sqrt(D).  Returns [B,Hq,T,D] in the
     memory order of q."""
-    return AttnFn.apply(q, k, v, attn_mask, causal, sm_scale)
+    _check(q, k, v)
+    mask, mdt = prepare_mask(attn_mask, q.shape[0], q.shape[2], q.device)
+    return AttnFn.apply(q, k, v, mask, _problem(q, k, causal, mdt, sm_scale))

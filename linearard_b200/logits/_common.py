@@ -20,7 +20,5 @@ def check_logits(x, name="logits"):
 def rows_of(x) -> _lib.LKLLogits:
     """The rows of [B, T, V] or [N, V] logits, read in place."""
     if x.ndim == 2:
-        return _lib.LKLLogits(B=1, T=x.shape[0], V=x.shape[1], sb=0, st=x.stride(0),
-                              dtype=_DT[x.dtype])
-    return _lib.LKLLogits(B=x.shape[0], T=x.shape[1], V=x.shape[2], sb=x.stride(0),
-                          st=x.stride(1), dtype=_DT[x.dtype])
+        return _lib.LKLLogits(1, x.shape[0], x.shape[1], 0, x.stride(0), _DT[x.dtype])
+    return _lib.LKLLogits(*x.shape, *x.stride()[:2], _DT[x.dtype])

@@ -15,7 +15,8 @@ import ctypes
 import torch
 
 from .. import _lib
-from ..attention_KL._common import prepare_mask, ptr, stream_of
+from .._marshal import on_device, once_when_recorded, raw_stream
+from ..attention_KL._common import prepare_mask
 from ._common import check_logits, rows_of
 
 __all__ = ["logits_kl_align", "logits_kl_forward", "logits_kl_backward", "LogitsKLAlignFn"]
@@ -42,24 +43,43 @@ def _mask(attn_mask, s):
     return prepare_mask(mask, mask.shape[0], mask.shape[1], s.device)
 
 
+def _forward(s, t, mask, mdt, temperature, rows):
+    dev, shape = s.device, s.shape[:-1]
+    L = _lib.lib()
+    with on_device(dev):
+        lse_s, lse_t = torch.empty((2, *shape), device=dev, dtype=torch.float32).unbind(0)
+        loss = torch.empty((), device=dev, dtype=torch.float32)
+        rs, rt = ctypes.byref(rows[0]), ctypes.byref(rows[1])
+        n = L.lkl_logits_kl_workspace_size(rs)
+        ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
+        st = L.lkl_logits_kl_forward(s.data_ptr(), rs, t.data_ptr(), rt,
+                                     None if mask is None else mask.data_ptr(), mdt, temperature,
+                                     lse_s.data_ptr(), lse_t.data_ptr(), loss.data_ptr(),
+                                     ws.data_ptr(), n, raw_stream(dev))
+    _lib.check(st, "lkl_logits_kl_forward")
+    return loss, lse_s, lse_t
+
+
+def _backward(s, t, lse_s, lse_t, mask, mdt, temperature, rows, dloss):
+    dev = s.device
+    with on_device(dev):
+        ds = torch.empty(s.shape, device=dev, dtype=s.dtype)
+        st = _lib.lib().lkl_logits_kl_backward(
+            s.data_ptr(), ctypes.byref(rows[0]), t.data_ptr(), ctypes.byref(rows[1]),
+            None if mask is None else mask.data_ptr(), mdt, temperature, lse_s.data_ptr(),
+            lse_t.data_ptr(), None if dloss is None else dloss.data_ptr(), ds.data_ptr(),
+            raw_stream(dev))
+    _lib.check(st, "lkl_logits_kl_backward")
+    return ds
+
+
 def logits_kl_forward(s_logits, t_logits, attn_mask=None, temperature=1.0):
     """(loss 0-d fp32, lse_s, lse_t fp32 of the rows' shape: the log-sum-exp of
     logits / temperature, 0 where the mask removes the row)."""
     _check(s_logits, t_logits, temperature)
-    dev, shape = s_logits.device, tuple(s_logits.shape[:-1])
     mask, mdt = _mask(attn_mask, s_logits)
-    rs, rt = rows_of(s_logits), rows_of(t_logits)
-    L = _lib.lib()
-    with torch.cuda.device(dev):
-        lse_s, lse_t = torch.empty((2,) + shape, device=dev, dtype=torch.float32).unbind(0)
-        loss = torch.empty((), device=dev, dtype=torch.float32)
-        n = int(L.lkl_logits_kl_workspace_size(ctypes.byref(rs)))
-        ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
-        st = L.lkl_logits_kl_forward(ptr(s_logits), ctypes.byref(rs), ptr(t_logits),
-                                     ctypes.byref(rt), ptr(mask), mdt, float(temperature),
-                                     ptr(lse_s), ptr(lse_t), ptr(loss), ptr(ws), n, stream_of(dev))
-    _lib.check(st, "lkl_logits_kl_forward")
-    return loss, lse_s, lse_t
+    return _forward(s_logits, t_logits, mask, mdt, float(temperature),
+                    (rows_of(s_logits), rows_of(t_logits)))
 
 
 def logits_kl_backward(s_logits, t_logits, lse_s, lse_t, attn_mask=None, temperature=1.0,
@@ -77,35 +97,31 @@ def logits_kl_backward(s_logits, t_logits, lse_s, lse_t, attn_mask=None, tempera
         assert isinstance(dloss, torch.Tensor) and dloss.numel() == 1 and dloss.device == dev \
             and dloss.dtype == torch.float32, "dloss must be a float32 scalar on the device"
     mask, mdt = _mask(attn_mask, s_logits)
-    rs, rt = rows_of(s_logits), rows_of(t_logits)
-    with torch.cuda.device(dev):
-        ds = torch.empty(s_logits.shape, device=dev, dtype=s_logits.dtype)
-        st = _lib.lib().lkl_logits_kl_backward(
-            ptr(s_logits), ctypes.byref(rs), ptr(t_logits), ctypes.byref(rt), ptr(mask), mdt,
-            float(temperature), ptr(lse_s), ptr(lse_t), ptr(dloss), ptr(ds), stream_of(dev))
-    _lib.check(st, "lkl_logits_kl_backward")
-    return ds
+    return _backward(s_logits, t_logits, lse_s, lse_t, mask, mdt, float(temperature),
+                     (rows_of(s_logits), rows_of(t_logits)), dloss)
 
 
 class LogitsKLAlignFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, s_logits, t_logits, attn_mask, temperature):
-        loss, lse_s, lse_t = logits_kl_forward(s_logits, t_logits, attn_mask, temperature)
-        ctx.save_for_backward(s_logits, t_logits, lse_s, lse_t, attn_mask)
-        ctx.temperature = temperature
+    def forward(ctx, s_logits, t_logits, mask, mdt, temperature, rows):
+        loss, lse_s, lse_t = _forward(s_logits, t_logits, mask, mdt, temperature, rows)
+        ctx.save_for_backward(s_logits, t_logits, lse_s, lse_t, mask)
+        ctx.mdt, ctx.temperature, ctx.rows = mdt, temperature, rows
         return loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_when_recorded
     def backward(ctx, dloss):
         s_logits, t_logits, lse_s, lse_t, mask = ctx.saved_tensors
-        ds = logits_kl_backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.temperature,
-                                dloss.to(torch.float32))
-        return ds, None, None, None      # the teacher gets no gradient
+        ds = _backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.mdt, ctx.temperature, ctx.rows,
+                       dloss.to(torch.float32))
+        return ds, None, None, None, None, None      # the teacher gets no gradient
 
 
 def logits_kl_align(s_logits, t_logits, attn_mask=None, temperature=1.0):
     """s_logits, t_logits: [B,T,V] (or [N,V]), fp16, bf16 or fp32 of one type, last
     stride 1, read in place; attn_mask: [B,T] (or [N]), nonzero = kept, or None.
     Gradients flow to the student's logits only."""
-    return LogitsKLAlignFn.apply(s_logits, t_logits, attn_mask, temperature)
+    _check(s_logits, t_logits, temperature)
+    mask, mdt = _mask(attn_mask, s_logits)
+    return LogitsKLAlignFn.apply(s_logits, t_logits, mask, mdt, float(temperature),
+                                 (rows_of(s_logits), rows_of(t_logits)))

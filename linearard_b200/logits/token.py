@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ..attention_KL._common import ptr, stream_of
+from .._marshal import on_device, once_when_recorded, raw_stream
 from ._common import check_logits, rows_of
 
 __all__ = ["token_logprobs", "TokenLogprobs", "TokenLogprobsFn", "MAX_TOP_K"]
@@ -30,44 +30,51 @@ class TokenLogprobs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
+def _forward(logits, rows, targets, top_k, ignore_index):
+    """(logprob, entropy, lse, top_logprobs, top_indices) of checked arguments."""
+    dev, shape = logits.device, targets.shape
+    with on_device(dev):
+        logprob, entropy, lse = torch.empty((3, *shape), device=dev, dtype=torch.float32).unbind(0)
+        top_v = top_i = None
+        if top_k:
+            top_v = torch.empty((*shape, top_k), device=dev, dtype=torch.float32)
+            top_i = torch.empty((*shape, top_k), device=dev, dtype=torch.int64)
+        st = _lib.lib().lkl_token_logprobs(
+            logits.data_ptr(), ctypes.byref(rows), targets.data_ptr(), ignore_index, top_k,
+            logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+            top_v.data_ptr() if top_k else None, top_i.data_ptr() if top_k else None,
+            raw_stream(dev))
+    _lib.check(st, "lkl_token_logprobs")
+    return logprob, entropy, lse, top_v, top_i
+
+
 class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, top_k: int, ignore_index: int):
-        rows, shape, dev = rows_of(logits), tuple(targets.shape), logits.device
-        with torch.cuda.device(dev):
-            stats = torch.empty((3,) + shape, device=dev, dtype=torch.float32)
-            logprob, entropy, lse = stats.unbind(0)
-            top_v = top_i = None
-            if top_k:
-                top_v = torch.empty(shape + (top_k,), device=dev, dtype=torch.float32)
-                top_i = torch.empty(shape + (top_k,), device=dev, dtype=torch.int64)
-            st = _lib.lib().lkl_token_logprobs(
-                ptr(logits), ctypes.byref(rows), ptr(targets), ignore_index, top_k, ptr(logprob),
-                ptr(entropy), ptr(lse), ptr(top_v), ptr(top_i), stream_of(dev))
-        _lib.check(st, "lkl_token_logprobs")
+    def forward(ctx, logits, rows, targets, top_k: int, ignore_index: int):
+        logprob, entropy, lse, top_v, top_i = _forward(logits, rows, targets, top_k, ignore_index)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, targets, lse, entropy)
-        ctx.ignore_index = ignore_index
+        ctx.rows, ctx.ignore_index = rows, ignore_index
         if top_k:
             ctx.mark_non_differentiable(top_v, top_i)
         return logprob, entropy, top_v, top_i
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_when_recorded
     def backward(ctx, d_logprob, d_entropy, _top_v, _top_i):
         if d_logprob is None and d_entropy is None:
-            return None, None, None, None
+            return None, None, None, None, None
         logits, targets, lse, entropy = ctx.saved_tensors
-        rows, dev = rows_of(logits), logits.device
-        with torch.cuda.device(dev):
+        dev = logits.device
+        with on_device(dev):
             g, h = (None if d is None else d.to(torch.float32).contiguous()
                     for d in (d_logprob, d_entropy))
             dx = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
             st = _lib.lib().lkl_token_logprobs_backward(
-                ptr(logits), ctypes.byref(rows), ptr(targets), ctx.ignore_index, ptr(lse),
-                ptr(entropy), ptr(g), ptr(h), ptr(dx), stream_of(dev))
+                logits.data_ptr(), ctypes.byref(ctx.rows), targets.data_ptr(), ctx.ignore_index,
+                lse.data_ptr(), entropy.data_ptr(), None if g is None else g.data_ptr(),
+                None if h is None else h.data_ptr(), dx.data_ptr(), raw_stream(dev))
         _lib.check(st, "lkl_token_logprobs_backward")
-        return dx, None, None, None
+        return dx, None, None, None, None
 
 
 def token_logprobs(logits, targets, top_k=0, ignore_index=-100) -> TokenLogprobs:
@@ -85,5 +92,8 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100) -> TokenLogprobs
     assert isinstance(top_k, int) and 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]), \
         "top_k must be from 0 to min(V, 32)"
     assert isinstance(ignore_index, int), "ignore_index must be an integer"
-    return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets.contiguous(), top_k,
-                                                ignore_index))
+    rows, targets = rows_of(logits), targets.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*TokenLogprobsFn.apply(logits, rows, targets, top_k, ignore_index))
+    logprob, entropy, _, top_v, top_i = _forward(logits, rows, targets, top_k, ignore_index)
+    return TokenLogprobs(logprob, entropy, top_v, top_i)

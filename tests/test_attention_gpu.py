@@ -246,6 +246,7 @@ def test_chunks_of_the_backward(Hq, Hkv, causal, mask):
     ref = AttnRef(q, k, v, m, causal, None, g)
     prob = R._problem(q, k, causal, _lib.LKL_MASK_I64, None)
     L = _lib.lib()
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     full = L.lkl_attn_backward_workspace_size(ctypes.byref(prob), int(mask))
     n_t, G = 6, Hq // Hkv
     tiles = n_t * (n_t + 1) // 2 if causal else n_t * n_t
@@ -257,16 +258,16 @@ def test_chunks_of_the_backward(Hq, Hkv, causal, mask):
     for n in sizes:
         ws = torch.full((n + 256,), 0xFF, dtype=torch.uint8, device="cuda")
         grads = [torch.empty_like(t) for t in (q, k, v)]
-        st = L.lkl_attn_backward(*(R.ptr(t) for t in (q, k, v, out, lse, g)), None, R.ptr(m),
-                                 ctypes.byref(prob), *(R.ptr(t) for t in grads), R.ptr(ws), n,
-                                 R.stream_of(q.device))
+        st = L.lkl_attn_backward(*(t.data_ptr() for t in (q, k, v, out, lse, g)), None, at(m),
+                                 ctypes.byref(prob), *(t.data_ptr() for t in grads), ws.data_ptr(), n,
+                                 R.raw_stream(q.device))
         assert st == 0
         assert (ws[n:] == 0xFF).all()
         assert torch.equal(grads[1], want[1]) and torch.equal(grads[2], want[2])
         assert_within(grads[0], ref.dq, ref.dq_tol, "dq")
-    assert L.lkl_attn_backward(*(R.ptr(t) for t in (q, k, v, out, lse, g)), None, R.ptr(m),
-                               ctypes.byref(prob), *(R.ptr(t) for t in grads), R.ptr(ws),
-                               sizes[-1] - 256, R.stream_of(q.device)) == 6
+    assert L.lkl_attn_backward(*(t.data_ptr() for t in (q, k, v, out, lse, g)), None, at(m),
+                               ctypes.byref(prob), *(t.data_ptr() for t in grads), ws.data_ptr(),
+                               sizes[-1] - 256, R.raw_stream(q.device)) == 6
     check_device_status()
 
 
