@@ -32,25 +32,26 @@ static_assert(2 * kFaSoftmaxRegs + kFaOtherRegs <= 3 * kFaRegs, "register split"
 static_assert(kFaThreads * kFaRegs <= 65536, "register file");
 constexpr int kFaProducer = 8, kFaMma = 9, kFaCleaner = 10;
 // A row's exponent offset is its running maximum as of the last rescale; it
-// moves only when the maximum has grown by more than 2^8.  P then stays below
-// 256, exact in neither type more or less than below 1 (the rounding is relative).
-constexpr float kFaSlack = 8.f;
+// moves only when the maximum has grown by more than this power of two.  P then
+// stays below 2^slack, where its rounding is as exact as below 1.  fp16 ends at 2^16.
+template <bool BF16>
+constexpr float kFaSlack = BF16 ? 40.f : 8.f;
 constexpr float kMaskedScore = -1.0e30f;
 
 template <int D>
 struct FaLayout {
   static constexpr int TILE = kBM * D * 2;      // one 128-row tile
-  static constexpr int NS = D == 128 ? 5 : 8;   // ring of K and V tiles
-  static constexpr int OFF_Q = 0, OFF_KV = 2 * TILE;
-  static constexpr int OFF_MISC = OFF_KV + NS * TILE;
+  static constexpr int NK = D == 128 ? 2 : 4, NV = D == 128 ? 3 : 4;   // rings of K, V tiles
+  static constexpr int OFF_Q = 0, OFF_K = 2 * TILE, OFF_V = OFF_K + NK * TILE;
+  static constexpr int OFF_MISC = OFF_V + NV * TILE;
   static constexpr int BYTES = 1024 + OFF_MISC + kMisc;
   static_assert(BYTES <= kMaxDynSmem, "shared memory");
 };
 
 struct FaMisc {
   uint64_t q_full;
-  uint64_t full[8], ready[8], empty[8];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_ready[4], v_empty[4];
+  uint64_t s_full[2], p_full[2][2], o_full[2];   // p_full: keys 0-95, 96-127
   uint32_t tmem_base;
   int abort;
 };
@@ -102,6 +103,33 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, const TileBits& t, int
   }
 }
 
+// 32 16-bit columns from `col` on of row r into a [128][D] tile of 128-byte
+// swizzled [128][64] chunks.
+__device__ __forceinline__ void stage_row32(uint8_t* tile, int r, int col,
+                                            const uint32_t (&w)[16]) {
+  uint8_t* row = tile + (col >> 6) * kChunk + r * 128;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    *reinterpret_cast<uint4*>(row + (((((col & 63) >> 3) + e) ^ (r & 7)) << 4)) =
+        make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+}
+
+// Writes a warp's 32 rows of such a tile through a map with a {64, 32} box; rows
+// past T and columns past the head dim are left as they are.
+template <int D>
+__device__ __forceinline__ void store_rows_tma(const CUtensorMap* map, const uint8_t* tile, int w,
+                                               int lane, int row0, int T, int h, int b) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && row0 + w * 32 < T) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      tma_store_4d(map, tile + c * kChunk + w * 32 * 128, c * 64, row0 + w * 32, h, b);
+    bulk_commit_group();
+    bulk_wait_read();
+  }
+}
+
 // Query tiles in bands of heads whose keys and values stay in L2, the longest
 // rows of a band first.
 struct FaWork {
@@ -117,9 +145,9 @@ template <int D, bool BF16, bool MASKED>
 __global__ void __launch_bounds__(kFaThreads, 1)
 attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
                           const __grid_constant__ CUtensorMap tm_k,
-                          const __grid_constant__ CUtensorMap tm_v, const AttnProblem p,
-                          const TensorStrides so, const uint32_t* __restrict__ bits,
-                          uint16_t* __restrict__ out, float* __restrict__ lse, int band) {
+                          const __grid_constant__ CUtensorMap tm_v,
+                          const __grid_constant__ CUtensorMap tm_o, const AttnProblem p,
+                          const uint32_t* __restrict__ bits, float* __restrict__ lse, int band) {
   using L = FaLayout<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
@@ -144,14 +172,18 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
 
   if (threadIdx.x == 0) {
     mbar_init(&misc->q_full, 1);
-    for (int s = 0; s < L::NS; ++s) {
-      mbar_init(&misc->full[s], 1);
-      mbar_init(&misc->ready[s], 1);
-      mbar_init(&misc->empty[s], 1);
+    const int users = 4 * ((n_ct[0] > 0) + (n_ct[1] > 0));   // softmax warps
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&misc->k_full[s], 1);
+      mbar_init(&misc->k_empty[s], users);
+      mbar_init(&misc->v_full[s], 1);
+      mbar_init(&misc->v_ready[s], 1);
+      mbar_init(&misc->v_empty[s], users);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&misc->s_full[t], 1);
-      mbar_init(&misc->p_full[t], 4);
+      mbar_init(&misc->p_full[t][0], 4);
+      mbar_init(&misc->p_full[t][1], 4);
       mbar_init(&misc->o_full[t], 1);
     }
     misc->abort = 0;
@@ -177,91 +209,119 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
     if (warp == kFaProducer) {
       if (lane == 0 && kt0 >= 0) {
         mbar_arrive_expect_tx(&misc->q_full, ((n_ct[0] > 0) + (n_ct[1] > 0)) * L::TILE);
-  #pragma unroll
+#pragma unroll
         for (int t = 0; t < 2; ++t)
           if (n_ct[t] > 0)
             issue_tile_loads(smem + L::OFF_Q + t * L::TILE, &tm_q, &misc->q_full, D,
                              (wk.m * 2 + t) * kBM, h, b);
-        int n = 0;   // K(0), V(0), K(1), V(1), ...
-        bool ok = true;
-        for (int kt = kt0; ok && kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1))
-          for (int v = 0; v < 2; ++v, ++n) {
-            const int s = n % L::NS;
-            if (n >= L::NS && !mbar_wait(&misc->empty[s], (n / L::NS - 1) & 1, abort, err)) {
-              ok = false;
-              break;
-            }
-            mbar_arrive_expect_tx(&misc->full[s], L::TILE);
-            issue_tile_loads(smem + L::OFF_KV + s * L::TILE, v ? &tm_v : &tm_k, &misc->full[s], D,
-                             kt * kBN, g, b);
-          }
+        int n = 0;
+        for (int kt = kt0; kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1), ++n) {
+          const int sk = n % L::NK, sv = n % L::NV;
+          if (n >= L::NK && !mbar_wait(&misc->k_empty[sk], (n / L::NK - 1) & 1, abort, err)) break;
+          mbar_arrive_expect_tx(&misc->k_full[sk], L::TILE);
+          issue_tile_loads(smem + L::OFF_K + sk * L::TILE, &tm_k, &misc->k_full[sk], D, kt * kBN,
+                           g, b);
+          if (n >= L::NV && !mbar_wait(&misc->v_empty[sv], (n / L::NV - 1) & 1, abort, err)) break;
+          mbar_arrive_expect_tx(&misc->v_full[sv], L::TILE);
+          issue_tile_loads(smem + L::OFF_V + sv * L::TILE, &tm_v, &misc->v_full[sv], D, kt * kBN,
+                           g, b);
+        }
       }
     } else if (warp == kFaMma) {
+      // One thread issues both tiles' GEMMs, in turns: that keeps the tiles half a period
+      // apart, so that one's softmax runs under the other's GEMMs.  (A thread a tile lets
+      // them fall into step: 679 us instead of 541.)  The pipe waits for this thread, so
+      // the loop keeps ring positions and descriptors in registers.
       if (lane == 0 && kt0 >= 0) {
         const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
         const uint32_t id_o = idesc_f16(kBM, D, BF16, BF16, 0, 1);
-        const uint32_t q_at = smem_u32(smem + L::OFF_Q), kv_at = smem_u32(smem + L::OFF_KV);
-        uint64_t* loaded = MASKED ? misc->ready : misc->full;
-        int done[2] = {0, 0};   // score tiles issued
-        auto pv = [&](int t, int n_v) {   // O_t += P_t V with the V tile of load n_v
-          const uint32_t v_at = kv_at + (n_v % L::NS) * L::TILE;
-          if (!mbar_wait(&misc->p_full[t], (done[t] - 1) & 1, abort, err)) return false;
-          tc_fence_after();
-  #pragma unroll
-          for (int kk = 0; kk < kBN / 16; ++kk)
-            umma_f16_ts(tmem + kColO + t * D, tmem + t * 128 + kk * 8, mnmajor_desc(v_at, kk), id_o,
-                        (done[t] > 1 || kk > 0) ? 1u : 0u);
+        const uint64_t q_desc = kmajor_desc(smem_u32(smem + L::OFF_Q), 0);
+        const uint64_t k_desc = kmajor_desc(smem_u32(smem + L::OFF_K), 0);
+        const uint64_t v_desc = mnmajor_desc(smem_u32(smem + L::OFF_V), 0);
+        constexpr uint64_t kTile = L::TILE >> 4;   // descriptors count 16 bytes
+        uint64_t* v_loaded = MASKED ? misc->v_ready : misc->v_full;
+        int k_slot = 0, v_slot = 0;   // ring positions of the next K and V, and their phases
+        uint32_t k_phase = 0, v_phase = 0;
+        auto step = [](int& slot, uint32_t& phase, int n) {
+          if (++slot == n) {
+            slot = 0;
+            phase ^= 1;
+          }
+        };
+        auto score = [&](int t, uint64_t kd) {   // S_t = Q_t K^T
+          const uint64_t qd = q_desc + t * kTile;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off = (uint64_t)((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
+            umma_f16_ss(tmem + t * 128, qd + off, kd + off, id_s, kk > 0);
+          }
+          umma_commit(&misc->s_full[t]);
+        };
+        // O_t += P_t V, in the order in which P arrives
+        auto sum = [&](int t, uint64_t vd, uint32_t parity, bool first) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!mbar_wait(&misc->p_full[t][half], parity, abort, err)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = half * 6; kk < 6 + half * 2; ++kk)
+              umma_f16_ts(tmem + kColO + t * D, tmem + t * 128 + kk * 8,
+                          vd + (uint64_t)(kk * 16 * 128 >> 4), id_o,
+                          (!first || kk > 0) ? 1u : 0u);
+          }
           return true;
         };
-        bool ok = mbar_wait(&misc->q_full, 0, abort, err);
-        int n = 0;
-        for (int kt = kt0; ok && kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1), n += 2) {
-          ok = mbar_wait(&loaded[n % L::NS], (n / L::NS) & 1, abort, err);
-          if (ok && n > 0)
-            ok = mbar_wait(&loaded[(n - 1) % L::NS], ((n - 1) / L::NS) & 1, abort, err);
-          if (!ok) break;
+        bool ok = mbar_wait(&misc->q_full, 0, abort, err) &&
+                  mbar_wait(&misc->k_full[0], 0, abort, err);
+        uint32_t par[2] = {0, 0};
+        bool on[2] = {false, false}, fresh[2] = {true, true};
+        if (ok) {
           tc_fence_after();
-          const uint32_t k_at = kv_at + (n % L::NS) * L::TILE;
-  #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (kt >= n_ct[t]) continue;
-            if (done[t] > 0 && !(ok = pv(t, n - 1))) break;
-  #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              umma_f16_ss(tmem + t * 128, kmajor_desc(q_at + t * L::TILE, kk),
-                          kmajor_desc(k_at, kk), id_s, kk > 0);
-            umma_commit(&misc->s_full[t]);
-            ++done[t];
-          }
-          if (!ok) break;
-          umma_commit(&misc->empty[n % L::NS]);
-          if (n > 0) umma_commit(&misc->empty[(n - 1) % L::NS]);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if ((on[t] = kt0 < n_ct[t])) score(t, k_desc);
+          step(k_slot, k_phase, L::NK);
         }
-        if (ok) ok = mbar_wait(&loaded[(n - 1) % L::NS], ((n - 1) / L::NS) & 1, abort, err);
-        tc_fence_after();
-  #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && done[t] > 0 && (ok = pv(t, n - 1))) umma_commit(&misc->o_full[t]);
+        int kt = kt0;
+        while (ok) {
+          kt = live_tile<MASKED>(bits, words, b, kt - 1);
+          const bool more = kt >= 0;
+          if (!(ok = mbar_wait(&v_loaded[v_slot], v_phase, abort, err) &&
+                     (!more || mbar_wait(&misc->k_full[k_slot], k_phase, abort, err))))
+            break;
+          tc_fence_after();
+          const uint64_t vd = v_desc + v_slot * kTile, kd = k_desc + k_slot * kTile;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (ok && on[t]) {
+              ok = sum(t, vd, par[t], fresh[t]);
+              par[t] ^= 1;
+              fresh[t] = false;
+              if (ok && !more) umma_commit(&misc->o_full[t]);
+            }
+            if (ok && more && kt < n_ct[t]) {
+              score(t, kd);
+              on[t] = true;
+            }
+          }
+          if (!ok || !more) break;
+          step(k_slot, k_phase, L::NK);
+          step(v_slot, v_phase, L::NV);
+        }
       }
     } else if (warp == kFaCleaner) {
       if (MASKED) {
         int n = 0;
-        bool ok = true;
-        for (int kt = kt0; ok && kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1)) {
+        for (int kt = kt0; kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1), ++n) {
           const TileBits tb = tile_bits<MASKED>(bits, words, b, kt);
-          for (int v = 0; v < 2; ++v, ++n) {
-            const int s = n % L::NS;
-            if (!mbar_wait(&misc->full[s], (n / L::NS) & 1, abort, err)) {
-              ok = false;
-              break;
-            }
-            if (v && !tb.all()) {
-              clear_rows<D>(smem + L::OFF_KV + s * L::TILE, tb, lane);
-              fence_proxy_async_smem();
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&misc->ready[s]);
+          const int s = n % L::NV;
+          if (!mbar_wait(&misc->v_full[s], (n / L::NV) & 1, abort, err)) break;
+          if (!tb.all()) {
+            clear_rows<D>(smem + L::OFF_V + s * L::TILE, tb, lane);
+            fence_proxy_async_smem();
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&misc->v_ready[s]);
         }
       }
     }
@@ -275,15 +335,30 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
     const uint64_t cs2 = f2pack(cs, cs);
     float ref = -CUDART_INF_F, l = 0.f;   // exponent offset and sum of 2^(x cs - ref)
     const int my_ct = t ? n_ct[1] : n_ct[0];
-    int n = 0;
+    // rows that are not written take no part in the warp's decisions
+    const bool live = i < p.T && my_ct > 0 && token_valid(MASKED ? bits : nullptr, words, b, i);
+    int n = 0, skip = 0;   // key tiles taken; those before them that are the other tile's alone
     bool ok = true;
-    for (int kt = live_tile<MASKED>(bits, words, b, my_ct - 1); kt >= 0;
-         kt = live_tile<MASKED>(bits, words, b, kt - 1), ++n) {
+    int kt = live_tile<MASKED>(bits, words, b, my_ct - 1);
+    if (my_ct > 0 && kt != kt0) {
+      skip = 1;
+      if (lane == 0) {
+        mbar_arrive(&misc->k_empty[0]);
+        mbar_arrive(&misc->v_empty[0]);
+      }
+    }
+    for (; kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1), ++n) {
       if (!mbar_wait(&misc->s_full[t], n & 1, abort, err)) {
         ok = false;
         break;
       }
       tc_fence_after();
+      // S(n) is complete, and with it all that was issued before: K(n) and V(n - 1) are
+      // free.  (Commits of their own in the MMA thread cost it 250 cycles each.)
+      if (lane == 0) {
+        mbar_arrive(&misc->k_empty[(n + skip) % L::NK]);
+        if (n > 0) mbar_arrive(&misc->v_empty[(n + skip - 1) % L::NV]);
+      }
       float x[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(lane_addr + t * 128 + c * 32, x[c]);
@@ -298,13 +373,18 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
           for (int k = 0; k < 32; ++k)
             if (!(c * 32 + k <= lim && ((tb.w[c] >> k) & 1u))) x[c][k] = kMaskedScore;
       }
-      float mx = x[0][0];
+      float mx[8];   // eight chains: a single one would wait 64 times for the last maximum
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 8; ++c) {
+        const float* y = x[c >> 1] + (c & 1) * 16;
+        mx[c] = y[0];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) mx = fmax3(mx, x[c][k], x[c][k + 1]);
-      const float m_new = fmaxf(ref, mx * cs);
-      if (__any_sync(0xffffffffu, m_new > ref + kFaSlack)) {
+        for (int k = 1; k < 15; k += 2) mx[c] = fmax3(mx[c], y[k], y[k + 1]);
+        mx[c] = fmaxf(mx[c], y[15]);
+      }
+      const float m_new = fmaxf(ref, fmaxf(fmax3(fmax3(mx[0], mx[1], mx[2]), mx[3], mx[4]),
+                                           fmax3(mx[5], mx[6], mx[7])) * cs);
+      if (__any_sync(0xffffffffu, live && m_new > ref + kFaSlack<BF16>)) {
         if (n > 0) {
           const float f = ex2(ref - m_new);
           const uint64_t f2 = f2pack(f, f);
@@ -337,11 +417,13 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
           packed[k >> 1] = pack2t<BF16>(a0, a1);
         }
         tmem_st16(lane_addr + t * 128 + c * 16, packed);
+        if (c >= 2) {   // O += P V starts with the first 96 keys
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&misc->p_full[t][c - 2]);
+        }
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&misc->p_full[t]);
       float s0, s1;
       f2unpack(fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3])), s0, s1);
       l += s0 + s1;
@@ -350,9 +432,9 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
     tc_fence_after();
     if (ok) {
       const bool in = i < p.T;
-      const bool live = in && my_ct > 0 && token_valid(MASKED ? bits : nullptr, words, b, i);
       const float inv = live ? 1.f / l : 0.f;
-      uint16_t* row = out + (size_t)b * so.b + (size_t)h * so.h + (size_t)i * so.t;
+      // through the query tile's shared memory, which no GEMM reads any more
+      uint8_t* const tile = smem + L::OFF_Q + t * L::TILE;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float o[32];
@@ -360,17 +442,13 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
           tmem_ld32(lane_addr + kColO + t * D + c, o);
           tmem_wait_ld_dep(o);
         }
-        if (!in) continue;
+        uint32_t w[16];
 #pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          if (c + k >= p.D) break;   // head dims below 64 run zero-padded
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = live ? pack2t<BF16>(o[k + 2 * e] * inv, o[k + 2 * e + 1] * inv) : 0u;
-          *reinterpret_cast<uint4*>(row + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int k = 0; k < 32; k += 2)
+          w[k >> 1] = live ? pack2t<BF16>(o[k] * inv, o[k + 1] * inv) : 0u;
+        stage_row32(tile, r, c, w);
       }
+      store_rows_tma<D>(&tm_o, tile, warp & 3, lane, qt * kBM, p.T, h, b);
       if (in) lse[(size_t)wk.bh * p.T + i] = live ? (ref + lg2(l)) * kLn2 : 0.f;
     }
   }
@@ -390,24 +468,24 @@ int fa_band(const AttnProblem& p) {
   return (int)std::min<long long>(groups * G, (long long)p.B * p.Hq);
 }
 
-bool attn_map(CUtensorMap* m, const void* x, const AttnProblem& p, int H, const TensorStrides& s) {
-  return make_map(m, x, p.dtype, p.D, p.T, H, p.B, s);
+bool attn_map(CUtensorMap* m, const void* x, const AttnProblem& p, int H, const TensorStrides& s,
+              int box_rows = kBM) {
+  return make_map(m, x, p.dtype, p.D, p.T, H, p.B, s, box_rows);
 }
 
 template <int D, bool BF16, bool MASKED>
 cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
                              cudaStream_t st) {
   using L = FaLayout<D>;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   if (!attn_map(&mq, t.q, p, p.Hq, t.sq) || !attn_map(&mk, t.k, p, p.Hkv, t.sk) ||
-      !attn_map(&mv, t.v, p, p.Hkv, t.sv))
+      !attn_map(&mv, t.v, p, p.Hkv, t.sv) || !attn_map(&mo, t.out, p, p.Hq, t.so, 32))
     return cudaErrorInvalidValue;
   auto k = attn_sm100_forward_kernel<D, BF16, MASKED>;
   const cudaError_t e = prep(k, L::BYTES);
   if (e != cudaSuccess) return e;
   const int grid = p.B * p.Hq * ((p.T + 2 * kBM - 1) / (2 * kBM));
-  k<<<grid, kFaThreads, L::BYTES, st>>>(mq, mk, mv, p, t.so, bits, static_cast<uint16_t*>(t.out),
-                                        t.lse, fa_band(p));
+  k<<<grid, kFaThreads, L::BYTES, st>>>(mq, mk, mv, mo, p, bits, t.lse, fa_band(p));
   return cudaGetLastError();
 }
 
@@ -539,35 +617,15 @@ struct FbWalk {
   }
 };
 
-// This thread's NC fp32 TMEM columns times `scale` as 16-bit values into row[0 .. n_valid).
-template <int NC, bool BF16>
-__device__ __forceinline__ void store_row16(uint32_t taddr, uint16_t* row, float scale, bool store,
-                                            bool zero, int n_valid) {
-#pragma unroll
-  for (int c = 0; c < NC; c += 32) {
-    float v[32];
-    tmem_ld32(taddr + c, v);
-    tmem_wait_ld_dep(v);
-    if (!store) continue;
-#pragma unroll
-    for (int k = 0; k < 32; k += 8) {
-      if (c + k >= n_valid) break;
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = zero ? 0u : pack2t<BF16>(v[k + 2 * e] * scale, v[k + 2 * e + 1] * scale);
-      *reinterpret_cast<uint4*>(row + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-}
-
 template <int D, bool BF16, bool MASKED>
 __global__ void __launch_bounds__(kFbThreads, 1)
 attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v,
-                      const __grid_constant__ CUtensorMap tm_do, const AttnProblem p,
-                      const AttnTensors a, const FbChunk c, const uint32_t* __restrict__ bits,
+                      const __grid_constant__ CUtensorMap tm_do,
+                      const __grid_constant__ CUtensorMap tm_dk,
+                      const __grid_constant__ CUtensorMap tm_dv, const AttnProblem p,
+                      const FbChunk c, const uint32_t* __restrict__ bits,
                       const float* __restrict__ stats, uint16_t* __restrict__ dsbuf) {
   using L = FbLayout<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -861,15 +919,24 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
     if (ok && it > 0) ok = mbar_wait(&misc->acc_full, 0, abort, err);
     tc_fence_after();
     if (ok) {
-      const uint32_t row_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + wg * (D / 2);
-      const bool in = key < p.T, zero = !key_ok || it == 0;
-      const int first = wg * (D / 2);
-      uint16_t* dv = static_cast<uint16_t*>(a.dv) + (size_t)b * a.sdv.b + (size_t)g * a.sdv.h +
-                     (size_t)key * a.sdv.t + first;
-      uint16_t* dk = static_cast<uint16_t*>(a.dk) + (size_t)b * a.sdk.b + (size_t)g * a.sdk.h +
-                     (size_t)key * a.sdk.t + first;
-      store_row16<D / 2, BF16>(row_addr + kColDv, dv, 1.f, in && first < p.D, zero, p.D - first);
-      store_row16<D / 2, BF16>(row_addr + kColDk, dk, p.sc, in && first < p.D, zero, p.D - first);
+      // warpgroup 0 writes dv, 1 dk, through the tiles of V and K, which no GEMM reads any more
+      const uint32_t row_addr =
+          tmem + ((uint32_t)((warp & 3) * 32) << 16) + (wg ? kColDk : kColDv);
+      uint8_t* const tile = smem + (wg ? L::OFF_K : L::OFF_V);
+      const float scale = wg ? p.sc : 1.f;
+      const bool live = key_ok && it > 0;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float v[32];
+        tmem_ld32(row_addr + c, v);
+        tmem_wait_ld_dep(v);
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2)
+          w[k >> 1] = live ? pack2t<BF16>(v[k] * scale, v[k + 1] * scale) : 0u;
+        stage_row32(tile, r, c, w);
+      }
+      store_rows_tma<D>(wg ? &tm_dk : &tm_dv, tile, warp & 3, lane, j * kBN, p.T, g, b);
     }
   }
 
@@ -1150,9 +1217,10 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
                               cudaStream_t st) {
   const FbPlan plan = fb_plan(p, (long long)(ds_bytes / (kDTileElems * 2)));
   if (plan.keys <= 0) return cudaErrorInvalidValue;
-  CUtensorMap mq, mk, mv, mdo;
+  CUtensorMap mq, mk, mv, mdo, mdk, mdv;
   if (!attn_map(&mq, t.q, p, p.Hq, t.sq) || !attn_map(&mk, t.k, p, p.Hkv, t.sk) ||
-      !attn_map(&mv, t.v, p, p.Hkv, t.sv) || !attn_map(&mdo, t.dout, p, p.Hq, t.sdo))
+      !attn_map(&mv, t.v, p, p.Hkv, t.sv) || !attn_map(&mdo, t.dout, p, p.Hq, t.sdo) ||
+      !attn_map(&mdk, t.dk, p, p.Hkv, t.sdk, 32) || !attn_map(&mdv, t.dv, p, p.Hkv, t.sdv, 32))
     return cudaErrorInvalidValue;
   auto kkv = attn_sm100_dkv_kernel<D, BF16, MASKED>;
   auto kq = attn_sm100_dq_kernel<D, BF16, MASKED>;
@@ -1180,7 +1248,7 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
       const int i0 = p.causal ? j0 : 0;
       c.tph = plan.split ? (long long)(n_t - i0) * (c.j1 - j0) : fb_tiles_per_head(p);
       kkv<<<(c.g1 - g0) * (c.j1 - j0), kFbThreads, FbLayout<D>::BYTES, st>>>(
-          mq, mk, mv, mdo, p, t, c, bits, stats, dsbuf);
+          mq, mk, mv, mdo, mdk, mdv, p, c, bits, stats, dsbuf);
       if ((e = cudaGetLastError()) != cudaSuccess) return e;
       const int work = (c.g1 - g0) * G * (n_t - i0);
       kq<<<std::min(work, num_sms), kFqThreads, FqLayout<D>::BYTES, st>>>(mk, p, t, c, bits, dsbuf,

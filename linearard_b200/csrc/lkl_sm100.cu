@@ -1223,12 +1223,12 @@ EncodeTiledFn get_encoder() {
 int tc_dim(int d) { return d <= 64 ? 64 : 128; }
 
 bool make_map(CUtensorMap* m, const void* ptr, int dtype, int D, int T, int H, int B,
-              const TensorStrides& s) {
+              const TensorStrides& s, int box_rows = 128) {
   EncodeTiledFn enc = get_encoder();
   if (!enc) return false;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)s.t * 2, (cuuint64_t)s.h * 2, (cuuint64_t)s.b * 2};
-  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(m, dtype == LKL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
