@@ -112,6 +112,7 @@ __device__ __forceinline__ void stage_row32(uint8_t* tile, int r, int col,
   for (int e = 0; e < 4; ++e)
     *reinterpret_cast<uint4*>(row + (((((col & 63) >> 3) + e) ^ (r & 7)) << 4)) =
         make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+  fence_proxy_async_smem();
 }
 
 // Writes a warp's 32 rows of such a tile through a map with a {64, 32} box; rows
@@ -119,7 +120,6 @@ __device__ __forceinline__ void stage_row32(uint8_t* tile, int r, int col,
 template <int D>
 __device__ __forceinline__ void store_rows_tma(const CUtensorMap* map, const uint8_t* tile, int w,
                                                int lane, int row0, int T, int h, int b) {
-  fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0 && row0 + w * 32 < T) {
 #pragma unroll
@@ -509,8 +509,18 @@ cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const u
 // tensor pipe busy: dS(i) is computed under dV(i) and S(i+1), P(i+1) under dK(i)
 // and dP(i+1).  All 512 TMEM columns are in use (S, dP, dV, dK at head dim 128;
 // P and dS overwrite the first half of what they come from).
-constexpr int kFbThreads = 384;
-constexpr int kFbProducer = 8, kFbMma = 9, kFbCleaner = 10, kFbStats = 11;
+//
+// Sixteen row warps, 32 queries of 128 each (eight warps with 64 queries left the
+// exponentials of a tile at 1800 cycles for want of independent work; ring slots are
+// released by the row warps, since a commit costs the MMA thread some 250 cycles).
+// P is handed over in two parts, so that half of dV's GEMM runs under its second part.
+constexpr int kFbRowWarps = 16;
+constexpr int kFbThreads = 640;
+constexpr int kFbProducer = 16, kFbMma = 17, kFbCleaner = 18, kFbStats = 19;
+// Registers a thread of the five warpgroups: 96 at launch
+constexpr int kFbRegs = 96, kFbRowRegs = 104, kFbOtherRegs = 64;
+static_assert(4 * kFbRowRegs + kFbOtherRegs <= 5 * kFbRegs, "register split");
+static_assert(kFbThreads * kFbRegs <= 65536, "register file");
 
 // One backward chunk: kv groups [g0, g1), key tiles [j0, j1).  `split`: not all
 // key tiles, so that dq is summed over launches in fp32.
@@ -580,7 +590,7 @@ struct FbMisc {
   uint64_t kv_full;
   uint64_t full[8], ready[8], empty[8];
   uint64_t lse_full[2], lse_empty[2], delta_full, delta_empty;
-  uint64_t s_full, p_full, dp_full, ds_full, acc_full;
+  uint64_t s_full, p_full[2], dp_full, ds_full, acc_full;
   uint32_t tmem_base;
   int abort;
 };
@@ -655,18 +665,18 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
     for (int s = 0; s < L::NS; ++s) {
       mbar_init(&misc->full[s], 1);
       mbar_init(&misc->ready[s], 1);
-      mbar_init(&misc->empty[s], 1);
+      mbar_init(&misc->empty[s], kFbRowWarps);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&misc->lse_full[s], 1);
-      mbar_init(&misc->lse_empty[s], 8);
+      mbar_init(&misc->lse_empty[s], kFbRowWarps);
+      mbar_init(&misc->p_full[s], kFbRowWarps);
     }
     mbar_init(&misc->delta_full, 1);
-    mbar_init(&misc->delta_empty, 8);
+    mbar_init(&misc->delta_empty, kFbRowWarps);
     mbar_init(&misc->s_full, 1);
-    mbar_init(&misc->p_full, 8);
     mbar_init(&misc->dp_full, 1);
-    mbar_init(&misc->ds_full, 8);
+    mbar_init(&misc->ds_full, kFbRowWarps);
     mbar_init(&misc->acc_full, 1);
     misc->abort = 0;
     fence_barrier_init();
@@ -686,186 +696,207 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
   tc_fence_after();
   const uint32_t tmem = misc->tmem_base;
 
-  if (warp == kFbProducer) {
-    if (lane == 0 && walk0.on()) {
-      mbar_arrive_expect_tx(&misc->kv_full, 2 * L::TILE);
-      issue_tile_loads(smem + L::OFF_K, &tm_k, &misc->kv_full, D, j * kBN, g, b);
-      issue_tile_loads(smem + L::OFF_V, &tm_v, &misc->kv_full, D, j * kBN, g, b);
-      int n = 0;   // Q(0), dO(0), Q(1), dO(1), ...
-      bool ok = true;
-      for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next())
-        for (int o = 0; o < 2; ++o, ++n) {
-          const int s = n % L::NS;
-          if (n >= L::NS && !mbar_wait(&misc->empty[s], (n / L::NS - 1) & 1, abort, err)) {
-            ok = false;
-            break;
+  if (warp >= kFbRowWarps) {
+    reg_dec<kFbOtherRegs>();
+    if (warp == kFbProducer) {
+      if (lane == 0 && walk0.on()) {
+        mbar_arrive_expect_tx(&misc->kv_full, 2 * L::TILE);
+        issue_tile_loads(smem + L::OFF_K, &tm_k, &misc->kv_full, D, j * kBN, g, b);
+        issue_tile_loads(smem + L::OFF_V, &tm_v, &misc->kv_full, D, j * kBN, g, b);
+        int n = 0;   // Q(0), dO(0), Q(1), dO(1), ...
+        bool ok = true;
+        for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next())
+          for (int o = 0; o < 2; ++o, ++n) {
+            const int s = n % L::NS;
+            if (n >= L::NS && !mbar_wait(&misc->empty[s], (n / L::NS - 1) & 1, abort, err)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&misc->full[s], L::TILE);
+            issue_tile_loads(smem + L::OFF_RING + s * L::TILE, o ? &tm_do : &tm_q, &misc->full[s], D,
+                             w.i * kBM, w.h, b);
           }
-          mbar_arrive_expect_tx(&misc->full[s], L::TILE);
-          issue_tile_loads(smem + L::OFF_RING + s * L::TILE, o ? &tm_do : &tm_q, &misc->full[s], D,
-                           w.i * kBM, w.h, b);
+      }
+    } else if (warp == kFbStats) {
+      if (lane == 0 && walk0.on()) {
+        constexpr int kHalf = kFbStatBytes / 2;
+        auto src = [&](const FbWalk<MASKED>& w) {
+          return stats + ((size_t)(b * p.Hq + w.h) * n_t + w.i) * 2 * kBM;
+        };
+        auto load_lse = [&](const FbWalk<MASKED>& w, int it) {
+          const int e = it & 1;
+          if (it >= 2 && !mbar_wait(&misc->lse_empty[e], ((it >> 1) - 1) & 1, abort, err))
+            return false;
+          mbar_arrive_expect_tx(&misc->lse_full[e], kHalf);
+          bulk_load(smem + L::OFF_LSE + e * kHalf, src(w), kHalf, &misc->lse_full[e]);
+          return true;
+        };
+        FbWalk<MASKED> w = walk0;
+        bool ok = load_lse(w, 0);
+        for (int it = 0; ok && w.on(); ++it) {
+          if (it >= 1 && !mbar_wait(&misc->delta_empty, (it - 1) & 1, abort, err)) break;
+          mbar_arrive_expect_tx(&misc->delta_full, kHalf);
+          bulk_load(smem + L::OFF_DELTA, src(w) + kBM, kHalf, &misc->delta_full);
+          w.next();
+          if (w.on()) ok = load_lse(w, it + 1);
         }
-    }
-  } else if (warp == kFbStats) {
-    if (lane == 0 && walk0.on()) {
-      constexpr int kHalf = kFbStatBytes / 2;
-      auto src = [&](const FbWalk<MASKED>& w) {
-        return stats + ((size_t)(b * p.Hq + w.h) * n_t + w.i) * 2 * kBM;
-      };
-      auto load_lse = [&](const FbWalk<MASKED>& w, int it) {
-        const int e = it & 1;
-        if (it >= 2 && !mbar_wait(&misc->lse_empty[e], ((it >> 1) - 1) & 1, abort, err))
-          return false;
-        mbar_arrive_expect_tx(&misc->lse_full[e], kHalf);
-        bulk_load(smem + L::OFF_LSE + e * kHalf, src(w), kHalf, &misc->lse_full[e]);
-        return true;
-      };
-      FbWalk<MASKED> w = walk0;
-      bool ok = load_lse(w, 0);
-      for (int it = 0; ok && w.on(); ++it) {
-        if (it >= 1 && !mbar_wait(&misc->delta_empty, (it - 1) & 1, abort, err)) break;
-        mbar_arrive_expect_tx(&misc->delta_full, kHalf);
-        bulk_load(smem + L::OFF_DELTA, src(w) + kBM, kHalf, &misc->delta_full);
-        w.next();
-        if (w.on()) ok = load_lse(w, it + 1);
       }
-    }
-  } else if (warp == kFbMma) {
-    if (lane == 0 && walk0.on()) {
-      const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
-      const uint32_t id_g = idesc_f16(kBM, D, BF16, BF16, 0, 1);
-      const uint32_t k_at = smem_u32(smem + L::OFF_K), v_at = smem_u32(smem + L::OFF_V);
-      const uint32_t ring = smem_u32(smem + L::OFF_RING);
-      uint64_t* loaded = MASKED ? misc->ready : misc->full;
-      auto wait_load = [&](int n) {
-        return mbar_wait(&loaded[n % L::NS], (n / L::NS) & 1, abort, err);
-      };
-      // S^T = K Q^T (n: load of Q) and dP^T = V dO^T (n: load of dO)
-      auto scores = [&](int n, uint32_t a_at, uint32_t col, uint64_t* bar) {
-        const uint32_t b_at = ring + (n % L::NS) * L::TILE;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_f16_ss(tmem + col, kmajor_desc(a_at, kk), kmajor_desc(b_at, kk), id_s, kk > 0);
-        umma_commit(bar);
-      };
-      // acc += A^T-from-TMEM x tile; the two warpgroups' halves of A lie 64 columns apart
-      auto grads = [&](int n, uint32_t acc, uint32_t col, bool first) {
-        const uint32_t b_at = ring + (n % L::NS) * L::TILE;
-#pragma unroll
-        for (int kk = 0; kk < kBM / 16; ++kk)
-          umma_f16_ts(tmem + acc, tmem + col + (kk >> 2) * 64 + (kk & 3) * 8,
-                      mnmajor_desc(b_at, kk), id_g, (!first || kk > 0) ? 1u : 0u);
-        umma_commit(&misc->empty[n % L::NS]);
-      };
-      bool ok = mbar_wait(&misc->kv_full, 0, abort, err) && wait_load(0);
-      if (ok) {
-        tc_fence_after();
-        scores(0, k_at, 0, &misc->s_full);
-        ok = wait_load(1);
-      }
-      if (ok) {
-        tc_fence_after();
-        scores(1, v_at, kColDp, &misc->dp_full);
-      }
-      int it = 0;
-      FbWalk<MASKED> w = walk0;
-      while (ok) {
-        w.next();
-        const bool more = w.on();
-        if (!(ok = mbar_wait(&misc->p_full, it & 1, abort, err))) break;
-        tc_fence_after();
-        grads(2 * it + 1, kColDv, 0, it == 0);
-        if (more) {
-          if (!(ok = wait_load(2 * it + 2))) break;
+    } else if (warp == kFbMma) {
+      if (lane == 0 && walk0.on()) {
+        const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
+        const uint32_t id_g = idesc_f16(kBM, D, BF16, BF16, 0, 1);
+        const uint64_t k_desc = kmajor_desc(smem_u32(smem + L::OFF_K), 0);
+        const uint64_t v_desc = kmajor_desc(smem_u32(smem + L::OFF_V), 0);
+        const uint64_t km_desc = kmajor_desc(smem_u32(smem + L::OFF_RING), 0);
+        const uint64_t mn_desc = mnmajor_desc(smem_u32(smem + L::OFF_RING), 0);
+        constexpr uint64_t kTile = L::TILE >> 4;   // descriptors count 16 bytes
+        uint64_t* loaded = MASKED ? misc->ready : misc->full;
+        int slot = 0;            // ring position of the next load, and its phase
+        uint32_t phase = 0;
+        auto take = [&] {        // waits for the next load; its position, or -1
+          const int at = slot;
+          const bool got = mbar_wait(&loaded[slot], phase, abort, err);
+          if (++slot == L::NS) {
+            slot = 0;
+            phase ^= 1;
+          }
           tc_fence_after();
-          scores(2 * it + 2, k_at, 0, &misc->s_full);
-        }
-        if (!(ok = mbar_wait(&misc->ds_full, it & 1, abort, err))) break;
-        tc_fence_after();
-        grads(2 * it, kColDk, kColDp, it == 0);
-        if (!more) break;
-        if (!(ok = wait_load(2 * it + 3))) break;
-        tc_fence_after();
-        scores(2 * it + 3, v_at, kColDp, &misc->dp_full);
-        ++it;
-      }
-      if (ok) umma_commit(&misc->acc_full);
-    }
-  } else if (warp == kFbCleaner) {
-    if (MASKED) {
-      int n = 0;
-      bool ok = true;
-      for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next()) {
-        const TileBits tb = tile_bits<MASKED>(bits, words, b, w.i);
-        for (int o = 0; o < 2; ++o, ++n) {
-          const int s = n % L::NS;
-          if (!mbar_wait(&misc->full[s], (n / L::NS) & 1, abort, err)) {
-            ok = false;
-            break;
+          return got ? at : -1;
+        };
+        // S^T = K Q^T (ring tile: Q) and dP^T = V dO^T (ring tile: dO)
+        auto scores = [&](uint64_t ad, int at, uint32_t col, uint64_t* bar) {
+          const uint64_t bd = km_desc + at * kTile;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off = (uint64_t)((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
+            umma_f16_ss(tmem + col, ad + off, bd + off, id_s, kk > 0);
           }
-          if (!tb.all()) {
-            clear_rows<D>(smem + L::OFF_RING + s * L::TILE, tb, lane);
-            fence_proxy_async_smem();
+          umma_commit(bar);
+        };
+        // One 16-query step of acc += A^T-from-TMEM x ring tile; the 32 queries of
+        // warpgroup w have their 16-bit values from column 32 w on
+        auto grad = [&](int at, uint32_t acc, uint32_t col, int kk, bool start) {
+          umma_f16_ts(tmem + acc, tmem + col + (kk >> 1) * 32 + (kk & 1) * 8,
+                      mn_desc + at * kTile + (uint64_t)(kk * 16 * 128 >> 4), id_g, start ? 0u : 1u);
+        };
+        bool ok = mbar_wait(&misc->kv_full, 0, abort, err);
+        int q_at = ok ? take() : -1, do_at = -1;
+        if ((ok = q_at >= 0)) {
+          scores(k_desc, q_at, 0, &misc->s_full);
+          do_at = take();
+          if ((ok = do_at >= 0)) scores(v_desc, do_at, kColDp, &misc->dp_full);
+        }
+        uint32_t par = 0;
+        bool first = true;
+        FbWalk<MASKED> w = walk0;
+        while (ok) {
+          w.next();
+          const bool more = w.on();
+          for (int part = 0; part < 2; ++part) {
+            if (!(ok = mbar_wait(&misc->p_full[part], par, abort, err))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              grad(do_at, kColDv, 0, 2 * k + part, first && part == 0 && k == 0);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&misc->ready[s]);
+          if (!ok) break;
+          int q_next = 0;
+          if (more) {
+            if (!(ok = (q_next = take()) >= 0)) break;
+            scores(k_desc, q_next, 0, &misc->s_full);
+          }
+          if (!(ok = mbar_wait(&misc->ds_full, par, abort, err))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) grad(q_at, kColDk, kColDp, k, first && k == 0);
+          if (!more) break;
+          q_at = q_next;
+          if (!(ok = (do_at = take()) >= 0)) break;
+          scores(v_desc, do_at, kColDp, &misc->dp_full);
+          par ^= 1;
+          first = false;
+        }
+        if (ok) umma_commit(&misc->acc_full);
+      }
+    } else if (warp == kFbCleaner) {
+      if (MASKED) {
+        int n = 0;
+        bool ok = true;
+        for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next()) {
+          const TileBits tb = tile_bits<MASKED>(bits, words, b, w.i);
+          for (int o = 0; o < 2; ++o, ++n) {
+            const int s = n % L::NS;
+            if (!mbar_wait(&misc->full[s], (n / L::NS) & 1, abort, err)) {
+              ok = false;
+              break;
+            }
+            if (!tb.all()) {
+              clear_rows<D>(smem + L::OFF_RING + s * L::TILE, tb, lane);
+              fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&misc->ready[s]);
+          }
         }
       }
     }
-  } else if (warp < 8) {
-    // ---------------- thread = key r; warpgroup wg owns 64 of the tile's 128 queries
+  } else {
+    reg_inc<kFbRowRegs>();
+    // ---------------- thread = key r; warpgroup wg owns 32 of the tile's 128 queries
     const int wg = warp >> 2, r = (warp & 3) * 32 + lane, key = j * kBN + r;
-    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + wg * 64;
+    const uint32_t row_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t lane_addr = row_addr + wg * 32;
     const float cs = p.sc * kLog2e;
     const uint64_t cs2 = f2pack(cs, cs);
     const bool key_ok = key < p.T && ((keys.w[warp & 3] >> lane) & 1u);
-    uint4* const buf = reinterpret_cast<uint4*>(dsbuf) + (size_t)(wg * 8) * kBM + r;
-    int it = 0;
+    uint4* const buf = reinterpret_cast<uint4*>(dsbuf) + (size_t)(wg * 4) * kBM + r;
+    const float* const dl = reinterpret_cast<const float*>(smem + L::OFF_DELTA) + wg * 32;
+    int it = 0, ring = 0;   // ring: position of the previous query tile's Q, dO behind it
     bool ok = true;
     for (FbWalk<MASKED> w = walk0; w.on(); w.next(), ++it) {
       const float* nl =
           reinterpret_cast<const float*>(smem + L::OFF_LSE + (it & 1) * (kFbStatBytes / 2)) +
-          wg * 64;
-      const float* dl = reinterpret_cast<const float*>(smem + L::OFF_DELTA) + wg * 64;
+          wg * 32;
       if (!mbar_wait(&misc->lse_full[it & 1], (it >> 1) & 1, abort, err) ||
           !mbar_wait(&misc->s_full, it & 1, abort, err)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      float pr[2][32];
-      tmem_ld32(lane_addr, pr[0]);
-      tmem_ld32(lane_addr + 32, pr[1]);
-      tmem_wait_ld_dep(pr[0]);
-      tmem_wait_ld_dep(pr[1]);
+      // S(i) was issued behind dV(i - 1), which read dO(i - 1) last
+      if (it > 0 && lane == 0) mbar_arrive(&misc->empty[(ring + 1) % L::NS]);
+      float pr[32];
+      tmem_ld32(lane_addr, pr);
+      tmem_wait_ld_dep(pr);
       // causal: a query before this key takes no part (the diagonal tile only)
-      const int from = p.causal && w.i == j ? r - wg * 64 : 0;
+      const int from = p.causal && w.i == j ? r - wg * 32 : 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t packed[16];
+      for (int half = 0; half < 2; ++half) {
+        float* x = pr + half * 16;
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          const float4 z = *reinterpret_cast<const float4*>(nl + h * 32 + k);
-          float* x = pr[h] + k;
-          f2unpack(ffma2(f2pack(x[0], x[1]), cs2, f2pack(z.x, z.y)), x[0], x[1]);
-          f2unpack(ffma2(f2pack(x[2], x[3]), cs2, f2pack(z.z, z.w)), x[2], x[3]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = ex2(x[e]);
+        for (int k = 0; k < 16; k += 4) {
+          const float4 z = *reinterpret_cast<const float4*>(nl + half * 16 + k);
+          f2unpack(ffma2(f2pack(x[k], x[k + 1]), cs2, f2pack(z.x, z.y)), x[k], x[k + 1]);
+          f2unpack(ffma2(f2pack(x[k + 2], x[k + 3]), cs2, f2pack(z.z, z.w)), x[k + 2], x[k + 3]);
         }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = ex2(x[k]);
         if (!key_ok || from > 0) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (!key_ok || h * 32 + k < from) pr[h][k] = 0.f;
+          for (int k = 0; k < 16; ++k)
+            if (!key_ok || half * 16 + k < from) x[k] = 0.f;
         }
+        uint32_t packed[8];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) packed[k >> 1] = pack2t<BF16>(pr[h][k], pr[h][k + 1]);
-        tmem_st16(lane_addr + h * 16, packed);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&misc->p_full);
-        mbar_arrive(&misc->lse_empty[it & 1]);
+        for (int k = 0; k < 16; k += 2) packed[k >> 1] = pack2t<BF16>(x[k], x[k + 1]);
+        tmem_st8(lane_addr + half * 8, packed);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&misc->p_full[half]);
+          if (half == 1) mbar_arrive(&misc->lse_empty[it & 1]);
+        }
       }
 
       if (!mbar_wait(&misc->delta_full, it & 1, abort, err) ||
@@ -874,18 +905,22 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         break;
       }
       tc_fence_after();
-      uint32_t ds[2][16];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      // dP(i) was issued behind dK(i - 1), which read Q(i - 1) last
+      if (it > 0) {
+        if (lane == 0) mbar_arrive(&misc->empty[ring]);
+        ring = (ring + 2) % L::NS;
+      }
+      uint32_t ds[16];
+      {
         float x[32];
-        tmem_ld32(lane_addr + kColDp + h * 32, x);
+        tmem_ld32(lane_addr + kColDp, x);
         tmem_wait_ld_dep(x);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
-          const float4 z = *reinterpret_cast<const float4*>(dl + h * 32 + k);
-          f2unpack(fmul2(f2pack(pr[h][k], pr[h][k + 1]),
+          const float4 z = *reinterpret_cast<const float4*>(dl + k);
+          f2unpack(fmul2(f2pack(pr[k], pr[k + 1]),
                          fsub2(f2pack(x[k], x[k + 1]), f2pack(z.x, z.y))), x[k], x[k + 1]);
-          f2unpack(fmul2(f2pack(pr[h][k + 2], pr[h][k + 3]),
+          f2unpack(fmul2(f2pack(pr[k + 2], pr[k + 3]),
                          fsub2(f2pack(x[k + 2], x[k + 3]), f2pack(z.z, z.w))), x[k + 2], x[k + 3]);
         }
         if (MASKED && !key_ok) {   // 0 x what the removed key's v holds
@@ -893,11 +928,9 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
           for (int k = 0; k < 32; ++k) x[k] = 0.f;
         }
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) ds[h][k >> 1] = pack2t<BF16>(x[k], x[k + 1]);
+        for (int k = 0; k < 32; k += 2) ds[k >> 1] = pack2t<BF16>(x[k], x[k + 1]);
       }
-      // both halves are loaded: dS may overwrite the first of them
-      tmem_st16(lane_addr + kColDp, ds[0]);
-      tmem_st16(lane_addr + kColDp + 16, ds[1]);
+      tmem_st16(lane_addr + kColDp, ds);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -911,32 +944,32 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
       uint4* dst = buf + (size_t)(head * c.tph + fb_tile(c, p.causal, n_t, w.i, j)) *
                              (kDTileElems / 8);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t* v = ds[k >> 2] + (k & 3) * 4;
-        dst[k * kBM] = make_uint4(v[0], v[1], v[2], v[3]);
-      }
+      for (int k = 0; k < 4; ++k)
+        dst[k * kBM] = make_uint4(ds[4 * k], ds[4 * k + 1], ds[4 * k + 2], ds[4 * k + 3]);
     }
     if (ok && it > 0) ok = mbar_wait(&misc->acc_full, 0, abort, err);
     tc_fence_after();
     if (ok) {
-      // warpgroup 0 writes dv, 1 dk, through the tiles of V and K, which no GEMM reads any more
-      const uint32_t row_addr =
-          tmem + ((uint32_t)((warp & 3) * 32) << 16) + (wg ? kColDk : kColDv);
-      uint8_t* const tile = smem + (wg ? L::OFF_K : L::OFF_V);
-      const float scale = wg ? p.sc : 1.f;
+      // warpgroups 0 and 1 write dv, 2 and 3 dk (half of the columns each), through the
+      // tiles of V and K, which no GEMM reads any more
+      const int which = wg >> 1, col0 = (wg & 1) * (D / 2);
+      uint8_t* const tile = smem + (which ? L::OFF_K : L::OFF_V);
+      const float scale = which ? p.sc : 1.f;
       const bool live = key_ok && it > 0;
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c2 = 0; c2 < D / 2; c2 += 32) {
         float v[32];
-        tmem_ld32(row_addr + c, v);
+        tmem_ld32(row_addr + (which ? kColDk : kColDv) + col0 + c2, v);
         tmem_wait_ld_dep(v);
-        uint32_t w[16];
+        uint32_t u[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2)
-          w[k >> 1] = live ? pack2t<BF16>(v[k] * scale, v[k + 1] * scale) : 0u;
-        stage_row32(tile, r, c, w);
+          u[k >> 1] = live ? pack2t<BF16>(v[k] * scale, v[k + 1] * scale) : 0u;
+        stage_row32(tile, r, col0 + c2, u);
       }
-      store_rows_tma<D>(wg ? &tm_dk : &tm_dv, tile, warp & 3, lane, j * kBN, p.T, g, b);
+      named_bar(1 + which, 256);
+      if ((wg & 1) == 0)
+        store_rows_tma<D>(which ? &tm_dk : &tm_dv, tile, warp & 3, lane, j * kBN, p.T, g, b);
     }
   }
 
