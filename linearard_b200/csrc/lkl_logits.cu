@@ -18,15 +18,17 @@
 #include <math_constants.h>
 
 #include "lkl_logits.cuh"
+#include "sm100_ptx.cuh"
 
 namespace lkl {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLThreads = 256;
+using namespace sm100;
+
+constexpr int kLThreads = 128;      // a row's block: small, so that many rows overlap
 constexpr int kLWarps = kLThreads / 32;
-constexpr int kLBatch = 4;          // 16-byte loads in flight a thread and stream
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kAll = 0xffffffffu;
 
@@ -46,6 +48,9 @@ struct Elem<float> {
   static __device__ __forceinline__ float get(const uint4& v, int e) {
     return __uint_as_float(reinterpret_cast<const uint32_t*>(&v)[e]);
   }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    return max_nan(max_nan(get(v, 0), get(v, 1)), max_nan(get(v, 2), get(v, 3)));
+  }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ void put(uint4& v, int e, float x) {
     reinterpret_cast<uint32_t*>(&v)[e] = __float_as_uint(x);
@@ -58,6 +63,11 @@ struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ float get(const uint4& v, int e) {
     const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[e >> 1];
     return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {   // the largest; NaN if one is
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) {
     return __bfloat162float(*p);
@@ -74,6 +84,11 @@ struct Elem<__half> {
   static constexpr int N = 8;
   static __device__ __forceinline__ float get(const uint4& v, int e) {
     return __half2float(reinterpret_cast<const __half*>(&v)[e]);
+  }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void put(uint4& v, int e, float x) {
@@ -132,94 +147,109 @@ __device__ __forceinline__ bool same_offset(const T* a, const T* b) {
 
 // ---------------------------------------------------------------- statistics
 // Running sums relative to a maximum; c scales differences to exponents of two.
-// Nothing above -inf so far: m = -inf, l = a = 0.
+// Nothing above -inf so far: m = -inf and sums of 0.
 struct TokenStat {
-  float m, l, a;
-  __device__ __forceinline__ void move(float to, float c) {   // to >= m, to > -inf
-    const float d = m - to, f = ex2(d * c);
-    a = f == 0.f ? 0.f : f * fmaf(l, d, a);
-    l *= f;
-    m = to;
-  }
-  __device__ __forceinline__ void join(TokenStat o, float c) {
-    const float to = max_nan(m, o.m);
-    if (to == -CUDART_INF_F) return;
-    if (m == -CUDART_INF_F) m = to;
-    else move(to, c);
-    if (o.m == -CUDART_INF_F) o.m = to;
-    else o.move(to, c);
-    l += o.l;
-    a += o.a;
+  static constexpr int kSums = 2;
+  float m[1], sum[2];   // l, a
+  __device__ __forceinline__ void move(const float* to, float c) {   // to >= m
+    if (to[0] == -CUDART_INF_F || to[0] == m[0]) return;
+    if (m[0] != -CUDART_INF_F) {
+      const float d = m[0] - to[0], f = ex2(d * c);
+      sum[1] = f == 0.f ? 0.f : f * fmaf(sum[0], d, sum[1]);
+      sum[0] *= f;
+    }
+    m[0] = to[0];
   }
 };
 struct KLStat {
-  float ms, ls, mt, lt, a;
-  __device__ __forceinline__ void move(float ns, float nt, float c) {
-    if (ns != -CUDART_INF_F) {
-      ls *= ms == -CUDART_INF_F ? 1.f : ex2((ms - ns) * c);
-      ms = ns;
+  static constexpr int kSums = 3;
+  float m[2], sum[3];   // m_s, m_t; l_s, l_t, A
+  __device__ __forceinline__ void move(const float* to, float c) {
+    if (to[0] != -CUDART_INF_F && to[0] != m[0]) {
+      sum[0] *= m[0] == -CUDART_INF_F ? 1.f : ex2((m[0] - to[0]) * c);
+      m[0] = to[0];
     }
-    if (nt != -CUDART_INF_F) {
-      const float f = mt == -CUDART_INF_F ? 1.f : ex2((mt - nt) * c);
-      lt *= f;
-      // a may be +inf, where the student excludes what the teacher gives
-      a = f == 0.f && !isnan(a) ? 0.f : a * f;
-      mt = nt;
+    if (to[1] != -CUDART_INF_F && to[1] != m[1]) {
+      const float f = m[1] == -CUDART_INF_F ? 1.f : ex2((m[1] - to[1]) * c);
+      sum[1] *= f;
+      // A may be +inf, where the student excludes what the teacher gives
+      sum[2] = f == 0.f && !isnan(sum[2]) ? 0.f : sum[2] * f;
+      m[1] = to[1];
     }
-  }
-  __device__ __forceinline__ void join(KLStat o, float c) {
-    const float ns = max_nan(ms, o.ms), nt = max_nan(mt, o.mt);
-    move(ns, nt, c);
-    o.move(ns, nt, c);
-    ls += o.ls;
-    lt += o.lt;
-    a += o.a;
   }
 };
 
-template <typename S>
-__device__ __forceinline__ S shfl_stat(const S& s, int lane_xor) {
-  S o;
-  const float* a = reinterpret_cast<const float*>(&s);
-  float* b = reinterpret_cast<float*>(&o);
-#pragma unroll
-  for (int k = 0; k < (int)(sizeof(S) / 4); ++k) b[k] = __shfl_xor_sync(kAll, a[k], lane_xor);
-  return o;
-}
+// What a block shows the others of its cluster.
+struct Joint {
+  float warp[kLWarps][4];
+  float block[2][4];   // maxima, sums
+};
 
-// Joins the statistics of a cluster's threads; every thread gets the result.
-// `shared`: kLWarps + 1 entries of this block.
+// Joins the statistics of a cluster's threads, in a fixed order: the maxima
+// first, so that every thread rescales its sums once; every thread gets the result.
 template <typename S>
-__device__ __forceinline__ S join_all(S s, S* shared, float c) {
+__device__ __forceinline__ S join_all(S s, Joint& shared, float c) {
+  constexpr int NM = S::kSums - 1, NS = S::kSums;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const S other = shfl_stat(s, o);
-    // the same operand order in both lanes: the same bits
-    if (lane & o) {
-      S t = other;
-      t.join(s, c);
-      s = t;
-    } else {
-      s.join(other, c);
-    }
-  }
-  if (lane == 0) shared[warp] = s;
-  __syncthreads();
-  s = shared[0];
-#pragma unroll
-  for (int w = 1; w < kLWarps; ++w) s.join(shared[w], c);
   cg::cluster_group cluster = cg::this_cluster();
   const int n = (int)cluster.num_blocks();
+  float top[NM];
+#pragma unroll
+  for (int k = 0; k < NM; ++k) {
+    top[k] = s.m[k];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top[k] = max_nan(top[k], __shfl_xor_sync(kAll, top[k], o));
+    if (lane == 0) shared.warp[warp][k] = top[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NM; ++k) {
+    top[k] = shared.warp[0][k];
+#pragma unroll
+    for (int w = 1; w < kLWarps; ++w) top[k] = max_nan(top[k], shared.warp[w][k]);
+  }
   if (n > 1) {
-    if (threadIdx.x == 0) shared[kLWarps] = s;
+    if (threadIdx.x == 0)
+      for (int k = 0; k < NM; ++k) shared.block[0][k] = top[k];
     cluster.sync();
-    s = *cluster.map_shared_rank(shared + kLWarps, 0);
-    for (int r = 1; r < n; ++r) s.join(*cluster.map_shared_rank(shared + kLWarps, r), c);
+    for (int r = 0; r < n; ++r) {
+      const Joint* other = cluster.map_shared_rank(&shared, r);
+#pragma unroll
+      for (int k = 0; k < NM; ++k) top[k] = max_nan(top[k], other->block[0][k]);
+    }
+  }
+  __syncthreads();
+  s.move(top, c);
+#pragma unroll
+  for (int k = 0; k < NS; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.sum[k] += __shfl_xor_sync(kAll, s.sum[k], o);
+    if (lane == 0) shared.warp[warp][k] = s.sum[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NS; ++k) {
+    s.sum[k] = shared.warp[0][k];
+#pragma unroll
+    for (int w = 1; w < kLWarps; ++w) s.sum[k] += shared.warp[w][k];
+  }
+  if (n > 1) {
+    if (threadIdx.x == 0)
+      for (int k = 0; k < NS; ++k) shared.block[1][k] = s.sum[k];
+    cluster.sync();
+#pragma unroll
+    for (int k = 0; k < NS; ++k) s.sum[k] = 0.f;
+    for (int r = 0; r < n; ++r) {
+      const Joint* other = cluster.map_shared_rank(&shared, r);
+#pragma unroll
+      for (int k = 0; k < NS; ++k) s.sum[k] += other->block[1][k];
+    }
     cluster.sync();   // the entries are free, and no block has left
   } else {
     __syncthreads();
   }
+#pragma unroll
+  for (int k = 0; k < NM; ++k) s.m[k] = top[k];
   return s;
 }
 
@@ -262,109 +292,148 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k, int lane) {
 }
 
 // ---------------------------------------------------------------- token forward
+// Adds the pair x (two values as one register pair) to sums relative to m2.
+template <bool GUARD>
+__device__ __forceinline__ void token_pair(uint64_t x, uint64_t m2, uint64_t c2, uint64_t& l,
+                                           uint64_t& a) {
+  uint64_t d = fsub2(x, m2);
+  if (GUARD) {
+    float d0, d1;
+    f2unpack(d, d0, d1);
+    d = f2pack(max_nan(d0, -200.f), max_nan(d1, -200.f));   // e^-200 is 0 in fp32
+  }
+  float e0, e1;
+  f2unpack(fmul2(d, c2), e0, e1);
+  const uint64_t e = f2pack(ex2(e0), ex2(e1));
+  l = fadd2(l, e);
+  a = ffma2(e, d, a);
+}
+
+// The warps' bounds on the alternatives, and room for one lane's elements a warp.
+struct TopShared {
+  float kth[kLWarps], part[kLWarps];
+  float lane[kLWarps][32];
+};
+
 // Sums over this block's share of the row.  GUARD: -inf logits add exactly 0 to
 // a, where the plain form gives 0 x -inf = NaN; only rows that met one need it.
+//
+// TOP: an element can be among the best k only if it reaches the k-th best of any
+// warp, and also the least of the warps' (k / warps)-th best.  Few elements do after
+// the first batch; a batch's maximum, known for the sums, rules most batches out.
 template <typename T, bool GUARD, bool TOP>
 __device__ __forceinline__ TokenStat token_pass(const T* row, long long V, int top_k, TopList& top,
-                                                volatile float* thr) {
-  constexpr int N = Elem<T>::N;
+                                                TopShared& ts) {
+  constexpr int N = Elem<T>::N, U = 4, E = U * N;
   const RowCut<T> cut(row, V);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), n_blocks = (int)cluster.num_blocks();
   const int v0 = (int)((long long)cut.nv * rank / n_blocks);
   const int v1 = (int)((long long)cut.nv * (rank + 1) / n_blocks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  TokenStat s{-CUDART_INF_F, 0.f, 0.f};
+  const uint4* vec = reinterpret_cast<const uint4*>(row + cut.lead);
+  volatile float* kth = ts.kth;
+  volatile float* part = ts.part;
+  const int share_k = (top_k + kLWarps - 1) / kLWarps;
+  TokenStat s{{-CUDART_INF_F}, {0.f, 0.f}};
+  const uint64_t c2 = f2pack(kLog2e, kLog2e);
   bool fresh = true;
-  auto add = [&](const float* x, int n) {   // n <= kLBatch * N values, unrolled by the caller
-    float bm = x[0];
+  auto add = [&](const uint4* raw, int n) {   // n vectors; the sums, given their maximum
+    float bm = Elem<T>::top(raw[0]);
 #pragma unroll
-    for (int e = 1; e < n; ++e) bm = max_nan(bm, x[e]);
-    const float to = max_nan(s.m, bm);
+    for (int u = 1; u < n; ++u) bm = max_nan(bm, Elem<T>::top(raw[u]));
+    const float to = max_nan(s.m[0], bm);
     if (to == -CUDART_INF_F) return bm;
-    if (!(to == s.m)) {
-      if (s.m == -CUDART_INF_F) s.m = to;
-      else s.move(to, kLog2e);
-    }
-    float l0 = 0.f, l1 = 0.f, a0 = 0.f, a1 = 0.f;
+    if (!(to == s.m[0])) s.move(&to, kLog2e);
+    const uint64_t m2 = f2pack(to, to);
+    uint64_t l[2] = {0, 0}, a[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < n; e += 2) {
-      float d0 = x[e] - s.m, d1 = e + 1 < n ? x[e + 1] - s.m : -CUDART_INF_F;
-      if (GUARD || n == 1) {
-        d0 = max_nan(d0, -200.f);   // e^-200 is 0 in fp32
-        d1 = max_nan(d1, -200.f);
-      }
-      const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
-      l0 += e0;
-      l1 += e1;
-      a0 = fmaf(e0, d0, a0);
-      a1 = fmaf(e1, d1, a1);
-    }
-    s.l += l0 + l1;
-    s.a += a0 + a1;
+    for (int u = 0; u < n; ++u)
+#pragma unroll
+      for (int e = 0; e < N; e += 2)
+        token_pair<GUARD>(f2pack(Elem<T>::get(raw[u], e), Elem<T>::get(raw[u], e + 1)), m2, c2,
+                          l[(e >> 1) & 1], a[(e >> 1) & 1]);
+    float x, y;
+    f2unpack(fadd2(l[0], l[1]), x, y);
+    s.sum[0] += x + y;
+    f2unpack(fadd2(a[0], a[1]), x, y);
+    s.sum[1] += x + y;
     return bm;
   };
-  for (int v = v0 + threadIdx.x - lane; v < v1; v += kLBatch * kLThreads) {
-    uint4 raw[kLBatch];
-    bool in[kLBatch];
+  for (int v = v0 + warp * 32; v < v1; v += U * kLThreads) {
+    uint4 raw[U];
+    const int mine = v + lane;
+    const bool full = mine + (U - 1) * kLThreads < v1;
 #pragma unroll
-    for (int u = 0; u < kLBatch; ++u) {
-      const int at = v + lane + u * kLThreads;
-      in[u] = at < v1;
-      if (in[u]) raw[u] = __ldg(reinterpret_cast<const uint4*>(row + cut.lead) + at);
-    }
-    float x[kLBatch * N];
+    for (int u = 0; u < U; ++u)
+      if (full || mine + u * kLThreads < v1) raw[u] = __ldg(vec + mine + u * kLThreads);
     float bm = -CUDART_INF_F;
-    if (in[kLBatch - 1]) {
-#pragma unroll
-      for (int e = 0; e < kLBatch * N; ++e) x[e] = Elem<T>::get(raw[e / N], e % N);
-      bm = add(x, kLBatch * N);
+    if (full) {
+      bm = add(raw, U);
     } else {
 #pragma unroll
-      for (int u = 0; u < kLBatch; ++u)
-        if (in[u]) {
-#pragma unroll
-          for (int e = 0; e < N; ++e) x[u * N + e] = Elem<T>::get(raw[u], e);
-          bm = max_nan(bm, add(x + u * N, N));
-        }
+      for (int u = 0; u < U; ++u)
+        if (mine + u * kLThreads < v1) bm = max_nan(bm, add(raw + u, 1));
     }
-    if (TOP) {
-      __syncwarp();
-      float need = top.threshold(top_k);
+    if (!TOP) continue;
+    __syncwarp();
+    float need = top.threshold(top_k), least = part[0];
 #pragma unroll
-      for (int w = 0; w < kLWarps; ++w) need = fmaxf(need, thr[w]);
-      if (fresh) need = fmaxf(need, kth_of_lanes(in[0] ? bm : -CUDART_INF_F, top_k, lane));
-      fresh = false;
-      if (__any_sync(kAll, in[0] && !(bm < need))) {
+    for (int w = 0; w < kLWarps; ++w) {
+      need = fmaxf(need, kth[w]);
+      least = fminf(least, part[w]);
+    }
+    need = fmaxf(need, least);
+    const bool in = mine < v1;
+    if (fresh) need = fmaxf(need, kth_of_lanes(in ? bm : -CUDART_INF_F, top_k, lane));
+    fresh = false;
+    uint32_t lanes = __ballot_sync(kAll, in && !(bm < need));
+    if (!lanes) continue;
+    // the elements of one lane after the other, one a lane
+    while (lanes) {
+      const int from = __ffs(lanes) - 1;
+      lanes &= lanes - 1;
+      if (lane == from) {
 #pragma unroll
-        for (int e = 0; e < kLBatch * N; ++e) {
-          uint32_t hit = __ballot_sync(kAll, in[e / N] && x[e] >= need);
-          if (!hit) continue;
-          while (hit) {
-            const int from = __ffs(hit) - 1;
-            hit &= hit - 1;
-            const float best = __shfl_sync(kAll, x[e], from);
-            const uint32_t idx =
-                (uint32_t)(cut.lead + (v + from + (e / N) * kLThreads) * N + e % N);
-            top.insert(top_key(best, idx), lane);
-          }
-          need = fmaxf(need, top.threshold(top_k));
-        }
-        if (lane == 0) thr[warp] = need;
+        for (int e = 0; e < E; ++e) ts.lane[warp][e] = Elem<T>::get(raw[e / N], e % N);
       }
+      __syncwarp();
+      const int at = v + from + (lane / N) * kLThreads;   // vector of this lane's element
+      const float x = ts.lane[warp][lane];
+      uint32_t hit = __ballot_sync(kAll, lane < E && at < v1 && x >= need);
+      const uint64_t key = top_key(x, (uint32_t)(cut.lead + at * N + lane % N));
+      while (hit) {
+        const int h = __ffs(hit) - 1;
+        hit &= hit - 1;
+        top.insert(__shfl_sync(kAll, key, h), lane);
+      }
+      need = fmaxf(need, top.threshold(top_k));
+      lanes &= __ballot_sync(kAll, !(bm < need));
+      __syncwarp();
+    }
+    const float a_k = top.threshold(top_k), a_part = top.threshold(share_k);
+    if (lane == 0) {
+      kth[warp] = a_k;
+      part[warp] = a_part;
     }
   }
   if (rank == 0 && warp == 0) {   // at most 14 elements
     const long long c = cut.end_elem(lane, V);
     const float x = c >= 0 ? Elem<T>::one(row + c) : -CUDART_INF_F;
-    add(&x, 1);
+    const float to = max_nan(s.m[0], x);
+    if (to != -CUDART_INF_F) {
+      if (!(to == s.m[0])) s.move(&to, kLog2e);
+      const float d = max_nan(x - to, -200.f), e = ex2(d * kLog2e);
+      s.sum[0] += e;
+      s.sum[1] = fmaf(e, d, s.sum[1]);
+    }
     if (TOP) {
       uint32_t hit = __ballot_sync(kAll, c >= 0 && !isnan(x));
+      const uint64_t key = top_key(x, (uint32_t)c);
       while (hit) {
-        const int from = __ffs(hit) - 1;
+        const int h = __ffs(hit) - 1;
         hit &= hit - 1;
-        top.insert(top_key(__shfl_sync(kAll, x, from),
-                           (uint32_t)__shfl_sync(kAll, (int)c, from)), lane);
+        top.insert(__shfl_sync(kAll, key, h), lane);
       }
     }
   }
@@ -377,8 +446,8 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
                       int top_k, float* __restrict__ logprob, float* __restrict__ entropy,
                       float* __restrict__ lse_out, float* __restrict__ top_v,
                       int64_t* __restrict__ top_i) {
-  __shared__ TokenStat stat[kLWarps + 1];
-  __shared__ float thr[kLWarps];
+  __shared__ Joint joint;
+  __shared__ TopShared ts;
   __shared__ uint64_t lists[TOP ? kLWarps : 1][32];
   cg::cluster_group cluster = cg::this_cluster();
   const int n = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -387,24 +456,24 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   TopList top{0};
   if (TOP) {
-    if (lane == 0) thr[warp] = -CUDART_INF_F;
+    if (lane == 0) ts.kth[warp] = ts.part[warp] = -CUDART_INF_F;
     __syncthreads();
   }
-  TokenStat s = join_all(token_pass<T, false, TOP>(x, view.V, top_k, top, thr), stat, kLog2e);
-  if (isnan(s.a) && !isnan(s.l) && s.l > 0.f) {   // the same in every thread of the cluster
+  TokenStat s = join_all(token_pass<T, false, TOP>(x, view.V, top_k, top, ts), joint, kLog2e);
+  if (isnan(s.sum[1]) && s.sum[0] > 0.f) {   // the same in every thread of the cluster
     TopList none{0};
-    s = join_all(token_pass<T, true, false>(x, view.V, 0, none, thr), stat, kLog2e);
+    s = join_all(token_pass<T, true, false>(x, view.V, 0, none, ts), joint, kLog2e);
   }
-  const bool empty = s.m == -CUDART_INF_F;
-  const float log_l = empty ? CUDART_NAN_F : logf(s.l);
+  const bool empty = s.m[0] == -CUDART_INF_F;
+  const float log_l = empty ? CUDART_NAN_F : logf(s.sum[0]);
   if (rank == 0 && threadIdx.x == 0) {
     const int64_t y = targets[row];
     float lp = CUDART_NAN_F;
     if (y == ignore) lp = 0.f;
-    else if (y >= 0 && y < view.V) lp = (Elem<T>::one(x + y) - s.m) - log_l;
+    else if (y >= 0 && y < view.V) lp = (Elem<T>::one(x + y) - s.m[0]) - log_l;
     logprob[row] = lp;
-    entropy[row] = log_l - s.a / s.l;
-    lse_out[row] = s.m + log_l;
+    entropy[row] = log_l - s.sum[1] / s.sum[0];
+    lse_out[row] = s.m[0] + log_l;
   }
   if (TOP) {
     lists[warp][lane] = top.key;
@@ -423,7 +492,8 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
       }
       if (lane < top_k) {
         const long long idx = (uint32_t)~(uint32_t)top.key;
-        top_v[row * top_k + lane] = top.key ? (top_value(top.key) - s.m) - log_l : CUDART_NAN_F;
+        top_v[row * top_k + lane] =
+            top.key ? (top_value(top.key) - s.m[0]) - log_l : CUDART_NAN_F;
         top_i[row * top_k + lane] = top.key ? idx : view.V - 1;   // a row of NaN
       }
     }
@@ -442,31 +512,47 @@ __device__ __forceinline__ KLStat kl_pass(const T* s, const T* t, long long V, f
   const int rank = (int)cluster.block_rank(), n_blocks = (int)cluster.num_blocks();
   const int v0 = (int)((long long)cut.nv * rank / n_blocks);
   const int v1 = (int)((long long)cut.nv * (rank + 1) / n_blocks);
-  KLStat st{-CUDART_INF_F, 0.f, -CUDART_INF_F, 0.f, 0.f};
-  auto add = [&](const float* x, const float* y, int n) {
-    float bs = x[0], bt = y[0];
+  KLStat st{{-CUDART_INF_F, -CUDART_INF_F}, {0.f, 0.f, 0.f}};
+  const uint64_t c2 = f2pack(c, c);
+  auto add = [&](const uint4* x, const uint4* y, int n) {
+    float to[2] = {st.m[0], st.m[1]};
 #pragma unroll
-    for (int e = 1; e < n; ++e) {
-      bs = max_nan(bs, x[e]);
-      bt = max_nan(bt, y[e]);
+    for (int u = 0; u < n; ++u) {
+      to[0] = max_nan(to[0], Elem<T>::top(x[u]));
+      to[1] = max_nan(to[1], Elem<T>::top(y[u]));
     }
-    const float ns = max_nan(st.ms, bs), nt = max_nan(st.mt, bt);
-    if (!(ns == st.ms && nt == st.mt)) st.move(ns, nt, c);
-    const float ms = ns == -CUDART_INF_F ? 0.f : ns, mt = nt == -CUDART_INF_F ? 0.f : nt;
-    float ls = 0.f, lt = 0.f, a0 = 0.f, a1 = 0.f;
+    if (!(to[0] == st.m[0] && to[1] == st.m[1])) st.move(to, c);
+    const float ms = to[0] == -CUDART_INF_F ? 0.f : to[0], mt = to[1] == -CUDART_INF_F ? 0.f : to[1];
+    const uint64_t ms2 = f2pack(ms, ms), mt2 = f2pack(mt, mt);
+    uint64_t ls = 0, lt = 0, a = 0;
 #pragma unroll
-    for (int e = 0; e < n; ++e) {
-      const float es = ex2((x[e] - ms) * c), et = ex2((y[e] - mt) * c);
-      ls += es;
-      lt += et;
-      float d = y[e] - x[e];
-      if (GUARD && et == 0.f) d = 0.f;
-      if (e & 1) a1 = fmaf(et, d, a1);
-      else a0 = fmaf(et, d, a0);
-    }
-    st.ls += ls;
-    st.lt += lt;
-    st.a += a0 + a1;
+    for (int u = 0; u < n; ++u)
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        const uint64_t xs = f2pack(Elem<T>::get(x[u], e), Elem<T>::get(x[u], e + 1));
+        const uint64_t xt = f2pack(Elem<T>::get(y[u], e), Elem<T>::get(y[u], e + 1));
+        float s0, s1, t0, t1;
+        f2unpack(fmul2(fsub2(xs, ms2), c2), s0, s1);
+        f2unpack(fmul2(fsub2(xt, mt2), c2), t0, t1);
+        const uint64_t es = f2pack(ex2(s0), ex2(s1)), et = f2pack(ex2(t0), ex2(t1));
+        ls = fadd2(ls, es);
+        lt = fadd2(lt, et);
+        uint64_t d = fsub2(xt, xs);
+        if (GUARD) {   // no teacher probability, nothing added
+          float e0, e1, d0, d1;
+          f2unpack(et, e0, e1);
+          f2unpack(d, d0, d1);
+          d = f2pack(e0 == 0.f ? 0.f : d0, e1 == 0.f ? 0.f : d1);
+        }
+        a = ffma2(et, d, a);
+      }
+    float u0, u1;
+    f2unpack(ls, u0, u1);
+    st.sum[0] += u0 + u1;
+    f2unpack(lt, u0, u1);
+    st.sum[1] += u0 + u1;
+    f2unpack(a, u0, u1);
+    st.sum[2] += u0 + u1;
   };
   const uint4* sv = reinterpret_cast<const uint4*>(s + cut.lead);
   const T* tv = t + cut.lead;
@@ -478,29 +564,23 @@ __device__ __forceinline__ KLStat kl_pass(const T* s, const T* t, long long V, f
       a[u] = __ldg(sv + v + u * kLThreads);
       b[u] = load_vec(tv + (size_t)(v + u * kLThreads) * N, vec);
     }
-    float x[U * N], y[U * N];
-#pragma unroll
-    for (int e = 0; e < U * N; ++e) {
-      x[e] = Elem<T>::get(a[e / N], e % N);
-      y[e] = Elem<T>::get(b[e / N], e % N);
-    }
-    add(x, y, U * N);
+    add(a, b, U);
   }
   for (; v < v1; v += kLThreads) {
     const uint4 a = __ldg(sv + v), b = load_vec(tv + (size_t)v * N, vec);
-    float x[N], y[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      x[e] = Elem<T>::get(a, e);
-      y[e] = Elem<T>::get(b, e);
-    }
-    add(x, y, N);
+    add(&a, &b, 1);
   }
   if (rank == 0) {
     const long long k = cut.end_elem(threadIdx.x, V);
     if (k >= 0) {
       const float x = Elem<T>::one(s + k), y = Elem<T>::one(t + k);
-      add(&x, &y, 1);
+      const float to[2] = {max_nan(st.m[0], x), max_nan(st.m[1], y)};
+      st.move(to, c);
+      const float es = to[0] == -CUDART_INF_F ? 0.f : ex2((x - to[0]) * c);
+      const float et = to[1] == -CUDART_INF_F ? 0.f : ex2((y - to[1]) * c);
+      st.sum[0] += es;
+      st.sum[1] += et;
+      st.sum[2] = fmaf(et, GUARD && et == 0.f ? 0.f : y - x, st.sum[2]);
     }
   }
   return st;
@@ -511,7 +591,7 @@ __global__ void __launch_bounds__(kLThreads)
 logits_kl_forward_kernel(const LogitsView sv, const LogitsView tv, const void* __restrict__ mask,
                          int mdt, float inv_tau, float* __restrict__ lse_s,
                          float* __restrict__ lse_t, float* __restrict__ row_kl) {
-  __shared__ KLStat stat[kLWarps + 1];
+  __shared__ Joint joint;
   cg::cluster_group cluster = cg::this_cluster();
   const long long row = blockIdx.x / cluster.num_blocks();
   const bool first = cluster.block_rank() == 0 && threadIdx.x == 0;
@@ -521,23 +601,23 @@ logits_kl_forward_kernel(const LogitsView sv, const LogitsView tv, const void* _
   }
   const T *s = row_ptr<T>(sv, row), *t = row_ptr<T>(tv, row);
   const float c = inv_tau * kLog2e;
-  KLStat k = join_all(kl_pass<T, false>(s, t, sv.V, c), stat, c);
-  if (isnan(k.a) && !isnan(k.ls) && !isnan(k.lt))
-    k = join_all(kl_pass<T, true>(s, t, sv.V, c), stat, c);
+  KLStat k = join_all(kl_pass<T, false>(s, t, sv.V, c), joint, c);
+  if (isnan(k.sum[2]) && !isnan(k.sum[0]) && !isnan(k.sum[1]))
+    k = join_all(kl_pass<T, true>(s, t, sv.V, c), joint, c);
   if (first) {
     // in 64 bits: the loss is what is left of the difference of the two LSEs
-    const bool none = k.ms == -CUDART_INF_F || k.mt == -CUDART_INF_F;
-    const double zs = none ? CUDART_NAN : (double)k.ms * inv_tau + log((double)k.ls);
-    const double zt = none ? CUDART_NAN : (double)k.mt * inv_tau + log((double)k.lt);
+    const bool none = k.m[0] == -CUDART_INF_F || k.m[1] == -CUDART_INF_F;
+    const double zs = none ? CUDART_NAN : (double)k.m[0] * inv_tau + log((double)k.sum[0]);
+    const double zt = none ? CUDART_NAN : (double)k.m[1] * inv_tau + log((double)k.sum[1]);
     lse_s[row] = (float)zs;
     lse_t[row] = (float)zt;
-    row_kl[row] = (float)((double)k.a * inv_tau / k.lt + (zs - zt));
+    row_kl[row] = (float)((double)k.sum[2] * inv_tau / k.sum[1] + (zs - zt));
   }
 }
 
 // ---------------------------------------------------------------- gradients
-// Elements [begin, end) of a row of V: a block's share, cut at vectors.
-constexpr int kLShare = 4 * kLThreads;   // vectors a block
+constexpr int kGThreadsL = 256;
+constexpr int kLShare = 4 * kGThreadsL;   // vectors a block
 
 // d = f(x, element) over a row: vectors in this block's share, the ends by the first block.
 template <typename T, typename Load, typename F>
@@ -547,15 +627,15 @@ __device__ __forceinline__ void map_row(const T* cut_by, T* out, long long V, in
   const RowCut<T> cut(cut_by, V);
   const bool vec = same_offset(cut_by, out);
   const int end = min(cut.nv, (share + 1) * kLShare);
-  for (int v = share * kLShare + threadIdx.x; v < end; v += 2 * kLThreads) {
-    const bool two = v + kLThreads < end;
+  for (int v = share * kLShare + threadIdx.x; v < end; v += 2 * kGThreadsL) {
+    const bool two = v + kGThreadsL < end;
     auto a = load(cut.lead + (long long)v * N);
     auto b = a;
-    if (two) b = load(cut.lead + (long long)(v + kLThreads) * N);
+    if (two) b = load(cut.lead + (long long)(v + kGThreadsL) * N);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (h == 1 && !two) break;
-      const long long at = cut.lead + (long long)(v + h * kLThreads) * N;
+      const long long at = cut.lead + (long long)(v + h * kGThreadsL) * N;
       uint4 d;
 #pragma unroll
       for (int e = 0; e < N; ++e) Elem<T>::put(d, e, f(h ? b : a, e, at + e));
@@ -582,7 +662,7 @@ struct LoadOne {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kLThreads)
+__global__ void __launch_bounds__(kGThreadsL)
 token_logprobs_backward_kernel(const LogitsView view, const int64_t* __restrict__ targets,
                                int64_t ignore, const float* __restrict__ lse,
                                const float* __restrict__ entropy, const float* __restrict__ g_lp,
@@ -620,7 +700,7 @@ struct LoadPair {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kLThreads)
+__global__ void __launch_bounds__(kGThreadsL)
 logits_kl_backward_kernel(const LogitsView sv, const LogitsView tv, const void* __restrict__ mask,
                           int mdt, float inv_tau, const float* __restrict__ lse_s,
                           const float* __restrict__ lse_t, const float* __restrict__ dloss,
@@ -647,20 +727,21 @@ logits_kl_backward_kernel(const LogitsView sv, const LogitsView tv, const void* 
 }
 
 // ---------------------------------------------------------------- launches
-// Blocks a row: enough that all rows together fill the GPU twice, as long as a
-// block keeps 2048 elements (below that, joining costs more than it saves).
+// Blocks a row: enough that all rows together give four blocks an SM, as long as a
+// block keeps 1024 elements (below that, joining costs more than it saves).
 int cluster_of(long long rows, long long V) {
   int n = 1;
-  while (n < kMaxCluster && rows * n < 296 && V / (2 * n) >= 2048) n *= 2;
+  while (n < kMaxCluster && rows * n < 592 && V / (2 * n) >= 1024) n *= 2;
   return n;
 }
 
 template <typename K, typename... A>
-cudaError_t launch_rows(K kernel, long long rows, int cluster, cudaStream_t st, A... args) {
+cudaError_t launch_rows(K kernel, int threads, long long rows, int cluster, cudaStream_t st,
+                        A... args) {
   if (rows * cluster > INT32_MAX) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
-  cfg.blockDim = dim3(kLThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -693,7 +774,7 @@ cudaError_t launch_token_logprobs(const LogitsView& x, long long rows, const int
   return with_type(x.dtype, [&](auto t) {
     using T = decltype(t);
     return launch_rows(top_k ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>,
-                       rows, n, st, x, targets, ignore, top_k, logprob, entropy, lse, top_v,
+                       kLThreads, rows, n, st, x, targets, ignore, top_k, logprob, entropy, lse, top_v,
                        top_i);
   });
 }
@@ -706,7 +787,7 @@ cudaError_t launch_token_logprobs_backward(const LogitsView& x, long long rows,
   return with_type(x.dtype, [&](auto t) {
     using T = decltype(t);
     const int shares = shares_of<T>(x.V);
-    return launch_rows(token_logprobs_backward_kernel<T>, rows * shares, 1, st, x, targets, ignore,
+    return launch_rows(token_logprobs_backward_kernel<T>, kGThreadsL, rows * shares, 1, st, x, targets, ignore,
                        lse, entropy, g_lp, g_en, static_cast<T*>(dx), shares);
   });
 }
@@ -716,7 +797,7 @@ cudaError_t launch_logits_kl_forward(const LogitsView& s, const LogitsView& t, l
                                      float* lse_t, float* row_kl, float* loss, cudaStream_t st) {
   const int n = cluster_of(rows, s.V);
   const cudaError_t e = with_type(s.dtype, [&](auto x) {
-    return launch_rows(logits_kl_forward_kernel<decltype(x)>, rows, n, st, s, t, mask, mdt, inv_tau,
+    return launch_rows(logits_kl_forward_kernel<decltype(x)>, kLThreads, rows, n, st, s, t, mask, mdt, inv_tau,
                        lse_s, lse_t, row_kl);
   });
   return e != cudaSuccess ? e : launch_reduce_partials(row_kl, (int)rows, loss, st);
@@ -729,7 +810,7 @@ cudaError_t launch_logits_kl_backward(const LogitsView& s, const LogitsView& t, 
   return with_type(s.dtype, [&](auto x) {
     using T = decltype(x);
     const int shares = shares_of<T>(s.V);
-    return launch_rows(logits_kl_backward_kernel<T>, rows * shares, 1, st, s, t, mask, mdt, inv_tau,
+    return launch_rows(logits_kl_backward_kernel<T>, kGThreadsL, rows * shares, 1, st, s, t, mask, mdt, inv_tau,
                        lse_s, lse_t, dloss, static_cast<T*>(ds), shares);
   });
 }
