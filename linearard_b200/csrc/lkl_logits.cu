@@ -272,24 +272,32 @@ struct TopList {
     const uint64_t prev = __shfl_up_sync(kAll, key, 1);
     if (x > key) key = lane > 0 && x > prev ? prev : x;
   }
+  // Joins another such list: the better of each pair with the other reversed is a
+  // bitonic sequence of the 32 best (Batcher), which five exchanges sort.
+  __device__ __forceinline__ void merge(uint64_t other, int lane) {
+    const uint64_t o = __shfl_sync(kAll, other, 31 - lane);
+    key = o > key ? o : key;
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) exchange(j, (lane & j) == 0);
+  }
+  // Sorts 32 elements, one a lane.
+  __device__ __forceinline__ void sort(int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1)
+        exchange(j, ((lane & j) == 0) == ((lane & k) == 0 || k == 32));
+  }
+  __device__ __forceinline__ void exchange(int j, bool larger) {
+    const uint64_t o = __shfl_xor_sync(kAll, key, j);
+    key = (o > key) == larger ? o : key;
+  }
   // Value that an element has to reach to be among the best k (-inf: any does).
   __device__ __forceinline__ float threshold(int k) const {
     const uint64_t last = __shfl_sync(kAll, key, k - 1);
     return last ? top_value(last) : -CUDART_INF_F;
   }
 };
-
-// k-th largest of the lanes' values (NaN counts as -inf).
-__device__ __forceinline__ float kth_of_lanes(float v, int k, int lane) {
-  int rank = 0;
-  if (isnan(v)) v = -CUDART_INF_F;
-#pragma unroll
-  for (int o = 0; o < 32; ++o) {
-    const float w = __shfl_sync(kAll, v, o);
-    rank += w > v || (w == v && o < lane);
-  }
-  return __shfl_sync(kAll, v, __ffs(__ballot_sync(kAll, rank == k - 1)) - 1);
-}
 
 // ---------------------------------------------------------------- token forward
 // Adds the pair x (two values as one register pair) to sums relative to m2.
@@ -313,6 +321,7 @@ __device__ __forceinline__ void token_pair(uint64_t x, uint64_t m2, uint64_t c2,
 struct TopShared {
   float kth[kLWarps], part[kLWarps];
   float lane[kLWarps][32];
+  uint64_t lists[kLWarps][32];
 };
 
 // Sums over this block's share of the row.  GUARD: -inf logits add exactly 0 to
@@ -385,10 +394,40 @@ __device__ __forceinline__ TokenStat token_pass(const T* row, long long V, int t
     }
     need = fmaxf(need, least);
     const bool in = mine < v1;
-    if (fresh) need = fmaxf(need, kth_of_lanes(in ? bm : -CUDART_INF_F, top_k, lane));
-    fresh = false;
-    uint32_t lanes = __ballot_sync(kAll, in && !(bm < need));
-    if (!lanes) continue;
+    // what this lane still has to offer, and what it has offered already
+    float offer = in ? bm : -CUDART_INF_F;
+    bool any = in;
+    uint64_t own = 0;
+    if (fresh) {
+      // the list starts with every lane's best element; the lane's next best decides
+      // whether the rest is looked at
+      fresh = false;
+      float next = -CUDART_INF_F;
+      int arg = -1;
+      offer = -CUDART_INF_F;
+      any = false;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float x = Elem<T>::get(raw[e / N], e % N);
+        if (!(full || mine + (e / N) * kLThreads < v1) || isnan(x)) continue;
+        if (arg < 0 || x > offer) {
+          any = arg >= 0;
+          next = offer;
+          offer = x;
+          arg = e;
+        } else {
+          any = true;
+          next = fmaxf(next, x);
+        }
+      }
+      if (arg >= 0)
+        own = top_key(offer, (uint32_t)(cut.lead + (mine + (arg / N) * kLThreads) * N + arg % N));
+      top.key = own;
+      top.sort(lane);
+      offer = next;
+      need = fmaxf(need, top.threshold(top_k));
+    }
+    uint32_t lanes = __ballot_sync(kAll, any && !(offer < need));
     // the elements of one lane after the other, one a lane
     while (lanes) {
       const int from = __ffs(lanes) - 1;
@@ -402,13 +441,14 @@ __device__ __forceinline__ TokenStat token_pass(const T* row, long long V, int t
       const float x = ts.lane[warp][lane];
       uint32_t hit = __ballot_sync(kAll, lane < E && at < v1 && x >= need);
       const uint64_t key = top_key(x, (uint32_t)(cut.lead + at * N + lane % N));
+      hit &= __ballot_sync(kAll, key != __shfl_sync(kAll, own, from));
       while (hit) {
         const int h = __ffs(hit) - 1;
         hit &= hit - 1;
         top.insert(__shfl_sync(kAll, key, h), lane);
       }
       need = fmaxf(need, top.threshold(top_k));
-      lanes &= __ballot_sync(kAll, !(bm < need));
+      lanes &= __ballot_sync(kAll, !(offer < need));
       __syncwarp();
     }
     const float a_k = top.threshold(top_k), a_part = top.threshold(share_k);
@@ -440,7 +480,107 @@ __device__ __forceinline__ TokenStat token_pass(const T* row, long long V, int t
   return s;
 }
 
-template <typename T, bool TOP>
+// Joins the warps' lists in warp 0.
+__device__ __forceinline__ void join_lists(TopList& top, TopShared& ts) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ts.lists[warp][lane] = top.key;
+  __syncthreads();
+  if (warp == 0)
+    for (int w = 1; w < kLWarps; ++w) top.merge(ts.lists[w][lane], lane);
+}
+
+// The best elements of this block's share, in warp 0 (one a lane, sorted).
+//
+// mine: the largest logit that this thread saw in the pass over the row.  The k-th
+// largest of the threads' maxima is reached by k elements at least and, unless many
+// logits are equal, by few more (22 expected for k = 20 of any row length).  So a
+// second look at the share, which is in L2 by now, compares each 16 bytes' maximum with
+// it and collects what reaches it.  Rows with more such elements than `cand` holds
+// (equal logits) take the pass that keeps a sorted list a warp.
+constexpr int kTopCand = 256;
+struct TopShared2 {
+  float mine[kLThreads];
+  float bound;
+  int count;
+  uint64_t cand[kTopCand];
+};
+
+template <typename T>
+__device__ __forceinline__ TopList top_pass(const T* row, long long V, int top_k, float mine,
+                                            TopShared& ts, TopShared2& tc) {
+  constexpr int N = Elem<T>::N, U = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (isnan(mine)) mine = -CUDART_INF_F;
+  tc.mine[threadIdx.x] = mine;
+  if (threadIdx.x == 0) tc.count = 0;
+  __syncthreads();
+  int rank_of = 0;
+  const float4* all = reinterpret_cast<const float4*>(tc.mine);
+#pragma unroll 8
+  for (int k = 0; k < kLThreads / 4; ++k) {
+    const float4 o = all[k];
+    const int at = 4 * k;
+    rank_of += (o.x > mine || (o.x == mine && at < (int)threadIdx.x));
+    rank_of += (o.y > mine || (o.y == mine && at + 1 < (int)threadIdx.x));
+    rank_of += (o.z > mine || (o.z == mine && at + 2 < (int)threadIdx.x));
+    rank_of += (o.w > mine || (o.w == mine && at + 3 < (int)threadIdx.x));
+  }
+  if (rank_of == top_k - 1) tc.bound = mine;
+  __syncthreads();
+  const float bound = tc.bound;
+  const RowCut<T> cut(row, V);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), n_blocks = (int)cluster.num_blocks();
+  const int v0 = (int)((long long)cut.nv * rank / n_blocks);
+  const int v1 = (int)((long long)cut.nv * (rank + 1) / n_blocks);
+  const uint4* vec = reinterpret_cast<const uint4*>(row + cut.lead);
+  auto take = [&](float x, long long idx) {
+    if (!(x >= bound)) return;
+    const int at = atomicAdd(&tc.count, 1);
+    if (at < kTopCand) tc.cand[at] = top_key(x, (uint32_t)idx);
+  };
+  auto look = [&](const uint4& raw, int at) {
+    if (Elem<T>::top(raw) < bound) return;
+#pragma unroll
+    for (int e = 0; e < N; ++e) take(Elem<T>::get(raw, e), cut.lead + (long long)at * N + e);
+  };
+  int v = v0 + threadIdx.x;
+  for (; v + (U - 1) * kLThreads < v1; v += U * kLThreads) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = __ldg(vec + v + u * kLThreads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) look(raw[u], v + u * kLThreads);
+  }
+  for (; v < v1; v += kLThreads) look(__ldg(vec + v), v);
+  if (rank == 0) {
+    const long long c = cut.end_elem(threadIdx.x, V);
+    if (c >= 0) take(Elem<T>::one(row + c), c);
+  }
+  __syncthreads();
+  const int count = tc.count;
+  TopList top{0};
+  if (count <= kTopCand) {
+    if (warp == 0)
+      for (int at = 0; at < count; at += 32) {   // in any order: the keys are distinct
+        TopList part{at + lane < count ? tc.cand[at + lane] : 0};
+        part.sort(lane);
+        if (at == 0) top = part;
+        else top.merge(part.key, lane);
+      }
+    return top;
+  }
+  if (lane == 0) ts.kth[warp] = ts.part[warp] = -CUDART_INF_F;
+  __syncthreads();
+  token_pass<T, false, true>(row, V, top_k, top, ts);
+  join_lists(top, ts);
+  return top;
+}
+
+// Alternatives are found in the one pass (kTopList) or by a second look (kTopLook).
+enum TopMode { kTopNone, kTopList, kTopLook };
+
+template <typename T, int MODE>
 __global__ void __launch_bounds__(kLThreads)
 token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets, int64_t ignore,
                       int top_k, float* __restrict__ logprob, float* __restrict__ entropy,
@@ -448,22 +588,22 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
                       int64_t* __restrict__ top_i) {
   __shared__ Joint joint;
   __shared__ TopShared ts;
-  __shared__ uint64_t lists[TOP ? kLWarps : 1][32];
+  __shared__ TopShared2 tc;
   cg::cluster_group cluster = cg::this_cluster();
   const int n = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const long long row = blockIdx.x / n;
   const T* x = row_ptr<T>(view, row);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  TopList top{0};
-  if (TOP) {
+  TopList none{0}, top{0};
+  if (MODE == kTopList) {
     if (lane == 0) ts.kth[warp] = ts.part[warp] = -CUDART_INF_F;
     __syncthreads();
   }
-  TokenStat s = join_all(token_pass<T, false, TOP>(x, view.V, top_k, top, ts), joint, kLog2e);
-  if (isnan(s.sum[1]) && s.sum[0] > 0.f) {   // the same in every thread of the cluster
-    TopList none{0};
+  TokenStat s = token_pass<T, false, MODE == kTopList>(x, view.V, top_k, top, ts);
+  const float mine = s.m[0];
+  s = join_all(s, joint, kLog2e);
+  if (isnan(s.sum[1]) && s.sum[0] > 0.f)   // the same in every thread of the cluster
     s = join_all(token_pass<T, true, false>(x, view.V, 0, none, ts), joint, kLog2e);
-  }
   const bool empty = s.m[0] == -CUDART_INF_F;
   const float log_l = empty ? CUDART_NAN_F : logf(s.sum[0]);
   if (rank == 0 && threadIdx.x == 0) {
@@ -475,21 +615,15 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
     entropy[row] = log_l - s.sum[1] / s.sum[0];
     lse_out[row] = s.m[0] + log_l;
   }
-  if (TOP) {
-    lists[warp][lane] = top.key;
-    if (n > 1) cluster.sync();
-    else __syncthreads();
+  if (MODE != kTopNone) {
+    if (MODE == kTopLook) top = top_pass<T>(x, view.V, top_k, mine, ts, tc);
+    else join_lists(top, ts);
+    if (n > 1) {
+      if (warp == 0) ts.lists[0][lane] = top.key;
+      cluster.sync();
+    }
     if (rank == 0 && warp == 0) {
-      for (int w = 1; w < n * kLWarps; ++w) {
-        const uint64_t* from = n > 1 ? cluster.map_shared_rank(&lists[w % kLWarps][0], w / kLWarps)
-                                     : &lists[w][0];
-        const uint64_t mine = lane < top_k ? from[lane] : 0;
-        for (int k = 0; k < top_k; ++k) {   // sorted: the first that does not fit ends the list
-          const uint64_t key = __shfl_sync(kAll, mine, k);
-          if (key <= __shfl_sync(kAll, top.key, top_k - 1)) break;
-          top.insert(key, lane);
-        }
-      }
+      for (int r = 1; r < n; ++r) top.merge(cluster.map_shared_rank(&ts.lists[0][0], r)[lane], lane);
       if (lane < top_k) {
         const long long idx = (uint32_t)~(uint32_t)top.key;
         top_v[row * top_k + lane] =
@@ -735,6 +869,11 @@ int cluster_of(long long rows, long long V) {
   return n;
 }
 
+// A second look needs the shares of all resident blocks (ten an SM) to stay in L2: up
+// to 104 KB a block it is faster (2004 x 50257 bf16, top 20: 77 us, list 102), above
+// it is not (4096 x 32000 fp32: 169 us, list 144; 2048 x 128256 bf16: 180, 177).
+constexpr long long kTopLookBytes = 104 << 10;
+
 template <typename K, typename... A>
 cudaError_t launch_rows(K kernel, int threads, long long rows, int cluster, cudaStream_t st,
                         A... args) {
@@ -770,12 +909,15 @@ int shares_of(long long V) {
 cudaError_t launch_token_logprobs(const LogitsView& x, long long rows, const int64_t* targets,
                                   int64_t ignore, int top_k, float* logprob, float* entropy,
                                   float* lse, float* top_v, int64_t* top_i, cudaStream_t st) {
-  const int n = cluster_of(rows, x.V);
   return with_type(x.dtype, [&](auto t) {
     using T = decltype(t);
-    return launch_rows(top_k ? token_logprobs_kernel<T, true> : token_logprobs_kernel<T, false>,
-                       kLThreads, rows, n, st, x, targets, ignore, top_k, logprob, entropy, lse, top_v,
-                       top_i);
+    const int n = cluster_of(rows, x.V);
+    const bool look = x.V * (long long)sizeof(T) / n <= kTopLookBytes;
+    return launch_rows(!top_k ? token_logprobs_kernel<T, kTopNone>
+                       : look ? token_logprobs_kernel<T, kTopLook>
+                              : token_logprobs_kernel<T, kTopList>,
+                       kLThreads, rows, n, st, x, targets, ignore, top_k, logprob, entropy, lse,
+                       top_v, top_i);
   });
 }
 
