@@ -20,6 +20,12 @@ What differs from the reference driver, in mechanism only:
   no dropout (peft's defaults for these fields, ``train.py:271-273``);
 * the model is ``LlamaModel`` without the LM head: the logits-KL term is off
   by default in the reference (``lam_l = 0``), so logits are not computed.
+  ``--lam-l`` > 0 adds it (``train.py:413-423``): a frozen head that both
+  models share, and ``lam_l`` times the mean KL of the tokens' distributions
+  (``logits_kl_align``).  ``--token-metrics`` reports the student's next-token
+  loss, entropy and accuracy on the sequence (``token_logprobs``);
+* ``--attention own`` runs the models' attention on ``linearard_b200.attention``
+  (forward and recomputing backward) instead of SDPA.
 
     python -m linearard_b200.distill [--layers 32] [--seq 16384] [--steps 3]
     torchrun --nproc-per-node 8 --master-addr 127.0.0.1 -m linearard_b200.distill
@@ -37,7 +43,9 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
+from .attention import attn
 from .attention_KL import attn_kl_align_grouped
+from .logits import logits_kl_align, token_logprobs
 
 _ACTIVE = None   # the Capture the registered attention function records into
 
@@ -61,18 +69,39 @@ class Capture:
         self.q[layer], self.k[layer], self.v[layer] = q, k, v
 
 
-def register_capture_attention(name="lkl_capture"):
+def register_capture_attention(name=None, attention="sdpa"):
     """Register an attention implementation that records q, k, v (after
-    RoPE, as the reference hook sees them) and then runs SDPA."""
+    RoPE, as the reference hook sees them) and then runs SDPA, or this package's
+    attention (``attention="own"``: fp16 or bf16 on CUDA; a [B, T] padding mask
+    removes tokens as queries and as keys)."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
+    from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    assert attention in ("sdpa", "own"), "attention must be sdpa or own"
+    name = name or ("lkl_capture" if attention == "sdpa" else "lkl_capture_own")
 
     def capture_attention(module, query, key, value, attention_mask, **kwargs):
         if _ACTIVE is not None:
             _ACTIVE.record(module.layer_idx, query, key, value)
-        return sdpa_attention_forward(module, query, key, value, attention_mask, **kwargs)
+        if attention == "sdpa":
+            return sdpa_attention_forward(module, query, key, value, attention_mask, **kwargs)
+        assert not kwargs.get("dropout"), "the attention has no dropout"
+        assert attention_mask is None or attention_mask.ndim == 2, \
+            "the attention takes [B, T] padding masks"
+        causal = kwargs.get("is_causal")
+        causal = getattr(module, "is_causal", True) if causal is None else causal
+        if attention_mask is not None:
+            attention_mask = attention_mask.contiguous()
+        out = attn(query, key, value, attention_mask, causal, kwargs.get("scaling"))
+        return out.transpose(1, 2), None
+
+    def padding_mask(*args, attention_mask=None, **kwargs):
+        return attention_mask            # [B, T]: the operator takes it as it is
 
     ALL_ATTENTION_FUNCTIONS.register(name, capture_attention)
+    if attention == "own":
+        ALL_MASK_ATTENTION_FUNCTIONS.register(name, padding_mask)
     return name
 
 
@@ -120,7 +149,7 @@ def build_models(args, device, seed=0):
     """Teacher (native RoPE, frozen) and student (same weights, linear RoPE x
     factor, LoRA on q/k/v), random init in bf16 on `device`."""
     from transformers import LlamaModel
-    attn = register_capture_attention()
+    impl = register_capture_attention(attention=getattr(args, "attention", "sdpa"))
     base_rope = {"rope_type": "default", "rope_theta": args.rope_theta}
     student_rope = {"rope_type": "linear", "factor": args.rope_factor,
                     "rope_theta": args.rope_theta}
@@ -131,10 +160,10 @@ def build_models(args, device, seed=0):
         with torch.device(device):
             teacher = LlamaModel(llama_config(args.layers, args.hidden, args.heads,
                                               args.intermediate, args.vocab, args.seq,
-                                              base_rope, attn))
+                                              base_rope, impl))
             student = LlamaModel(llama_config(args.layers, args.hidden, args.heads,
                                               args.intermediate, args.vocab, args.seq,
-                                              student_rope, attn))
+                                              student_rope, impl))
     finally:
         torch.set_default_dtype(old)
     student.load_state_dict(teacher.state_dict())
@@ -164,6 +193,38 @@ def relation_loss(cap_s: Capture, cap_t: Capture, layers, attn_mask=None, sm_sca
     return kl.sum() / denom / max(1, len(layers))
 
 
+def build_head(args, device, seed=0):
+    """The frozen LM head that both models share, random init in bf16."""
+    g = torch.Generator(device=device).manual_seed(seed)
+    head = nn.Linear(args.hidden, args.vocab, bias=False, device=device, dtype=torch.bfloat16)
+    head.weight.data.normal_(0.0, 0.02, generator=g)
+    return head.requires_grad_(False)
+
+
+def logits_loss(logits_s, logits_t, attn_mask=None, temperature=1.0):
+    """Mean over the valid tokens of KL(teacher || student) of their next-token
+    distributions (the term that ``lam_l`` weighs, train.py:413-423)."""
+    kl = logits_kl_align(logits_s, logits_t, attn_mask=attn_mask, temperature=temperature)
+    if attn_mask is None:
+        return kl / max(1, logits_s.shape[:-1].numel())
+    return kl / attn_mask.sum().clamp_min(1)
+
+
+def token_metrics(logits, input_ids, attn_mask=None):
+    """The student's next-token loss, entropy and accuracy: position t answers
+    token t + 1; positions whose next token is padding do not count."""
+    targets = input_ids[:, 1:]
+    if attn_mask is not None:
+        targets = targets.masked_fill(attn_mask[:, 1:] == 0, -100)
+    with torch.no_grad():
+        r = token_logprobs(logits[:, :-1], targets, top_k=1)
+        on = targets != -100
+        n = on.sum().clamp_min(1)
+        return {"nll": -r.logprob.sum() / n,
+                "entropy": r.entropy.masked_fill(~on, 0.0).sum() / n,
+                "accuracy": ((r.top_indices[..., 0] == targets) & on).sum() / n}
+
+
 def parse(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--layers", type=int, default=32)
@@ -177,6 +238,10 @@ def parse(argv=None):
     ap.add_argument("--lora-r", type=int, default=16)
     ap.add_argument("--lora-alpha", type=float, default=32.0)
     ap.add_argument("--lr", type=float, default=1e-4)
+    ap.add_argument("--attention", choices=("sdpa", "own"), default="sdpa")
+    ap.add_argument("--lam-l", type=float, default=0.0)
+    ap.add_argument("--temperature", type=float, default=1.0)
+    ap.add_argument("--token-metrics", action="store_true")
     ap.add_argument("--steps", type=int, default=3)
     ap.add_argument("--warmup", type=int, default=1)
     return ap.parse_args(argv)
@@ -197,6 +262,9 @@ def main(argv=None):
     opt = torch.optim.AdamW(lora, lr=args.lr)
     layers = list(range(args.layers))
     g = torch.Generator(device=dev).manual_seed(1000 + rank)
+    with_logits = args.lam_l > 0 or args.token_metrics
+    head = build_head(args, dev) if with_logits else None
+    tokens = {}
 
     def step(marks=None):
         def mark():
@@ -206,12 +274,21 @@ def main(argv=None):
         ids = torch.randint(0, args.vocab, (1, args.seq), device=dev, generator=g)
         mark()
         with torch.no_grad(), Capture() as cap_t:
-            teacher(input_ids=ids, use_cache=False)
+            out_t = teacher(input_ids=ids, use_cache=False)
         mark()
         with Capture() as cap_s:
-            model(input_ids=ids, use_cache=False)
+            out_s = model(input_ids=ids, use_cache=False)
         mark()
         loss = relation_loss(cap_s, cap_t, layers)
+        if with_logits:
+            logits_s = head(out_s.last_hidden_state)
+            if args.lam_l > 0:
+                with torch.no_grad():
+                    logits_t = head(out_t.last_hidden_state)
+                loss = loss + args.lam_l * logits_loss(logits_s, logits_t,
+                                                       temperature=args.temperature)
+            if args.token_metrics:
+                tokens.update(token_metrics(logits_s.detach(), ids))
         mark()
         loss.backward()                      # DDP all-reduces the LoRA gradients
         mark()
@@ -254,8 +331,10 @@ def main(argv=None):
             "ms_per_step": ms_step, "steps": args.steps, "warmup": args.warmup,
             "config": {"layers": args.layers, "hidden": args.hidden, "heads": args.heads,
                        "seq_len": args.seq, "batch_per_gpu": 1, "rope_factor": args.rope_factor,
-                       "lora_r": args.lora_r, "parallelism": f"ddp{world}"},
+                       "lora_r": args.lora_r, "parallelism": f"ddp{world}",
+                       "attention": args.attention, "lam_l": args.lam_l},
             "loss": float(loss.item()),
+            **({"tokens_rank0": {k: float(v) for k, v in tokens.items()}} if tokens else {}),
             "phase_ms_rank0": phases,
             "peak_mem_gb": torch.cuda.max_memory_allocated(dev) / 2**30,
         }), flush=True)
