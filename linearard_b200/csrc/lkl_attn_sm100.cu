@@ -511,9 +511,7 @@ cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const u
 // P and dS overwrite the first half of what they come from).
 //
 // Sixteen row warps, 32 queries of 128 each (eight warps with 64 queries left the
-// exponentials of a tile at 1800 cycles for want of independent work; ring slots are
-// released by the row warps, since a commit costs the MMA thread some 250 cycles).
-// P is handed over in two parts, so that half of dV's GEMM runs under its second part.
+// exponentials of a tile at 1800 cycles for want of independent work).  P is handed over in two parts, so that half of dV's GEMM runs under its second part.
 constexpr int kFbRowWarps = 16;
 constexpr int kFbThreads = 640;
 constexpr int kFbProducer = 16, kFbMma = 17, kFbCleaner = 18, kFbStats = 19;
@@ -641,7 +639,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   FbMisc* misc = reinterpret_cast<FbMisc*>(smem + L::OFF_MISC);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int* err = &g_device_error;
   volatile int* abort = &misc->abort;
   constexpr uint32_t kColDp = 128, kColDv = 256, kColDk = 256 + D;
@@ -665,7 +663,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
     for (int s = 0; s < L::NS; ++s) {
       mbar_init(&misc->full[s], 1);
       mbar_init(&misc->ready[s], 1);
-      mbar_init(&misc->empty[s], kFbRowWarps);
+      mbar_init(&misc->empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&misc->lse_full[s], 1);
@@ -694,7 +692,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = misc->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, misc->tmem_base, 0);
 
   if (warp >= kFbRowWarps) {
     reg_dec<kFbOtherRegs>();
@@ -742,7 +740,10 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         }
       }
     } else if (warp == kFbMma) {
-      if (lane == 0 && walk0.on()) {
+      // the whole warp runs the loop, so that descriptors stay in uniform registers; one
+      // lane issues
+      if (walk0.on()) {
+        const uint32_t leader = elect_one();
         const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
         const uint32_t id_g = idesc_f16(kBM, D, BF16, BF16, 0, 1);
         const uint64_t k_desc = kmajor_desc(smem_u32(smem + L::OFF_K), 0);
@@ -755,7 +756,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         uint32_t phase = 0;
         auto take = [&] {        // waits for the next load; its position, or -1
           const int at = slot;
-          const bool got = mbar_wait(&loaded[slot], phase, abort, err);
+          const bool got = mbar_wait_warp(&loaded[slot], phase, abort, err);
           if (++slot == L::NS) {
             slot = 0;
             phase ^= 1;
@@ -769,17 +770,17 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint64_t off = (uint64_t)((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
-            umma_f16_ss(tmem + col, ad + off, bd + off, id_s, kk > 0);
+            umma_f16_ss_by(leader, tmem + col, ad + off, bd + off, id_s, kk > 0);
           }
-          umma_commit(bar);
+          umma_commit_by(leader, bar);
         };
         // One 16-query step of acc += A^T-from-TMEM x ring tile; the 32 queries of
         // warpgroup w have their 16-bit values from column 32 w on
         auto grad = [&](int at, uint32_t acc, uint32_t col, int kk, bool start) {
-          umma_f16_ts(tmem + acc, tmem + col + (kk >> 1) * 32 + (kk & 1) * 8,
+          umma_f16_ts_by(leader, tmem + acc, tmem + col + (kk >> 1) * 32 + (kk & 1) * 8,
                       mn_desc + at * kTile + (uint64_t)(kk * 16 * 128 >> 4), id_g, start ? 0u : 1u);
         };
-        bool ok = mbar_wait(&misc->kv_full, 0, abort, err);
+        bool ok = mbar_wait_warp(&misc->kv_full, 0, abort, err);
         int q_at = ok ? take() : -1, do_at = -1;
         if ((ok = q_at >= 0)) {
           scores(k_desc, q_at, 0, &misc->s_full);
@@ -793,22 +794,24 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
           w.next();
           const bool more = w.on();
           for (int part = 0; part < 2; ++part) {
-            if (!(ok = mbar_wait(&misc->p_full[part], par, abort, err))) break;
+            if (!(ok = mbar_wait_warp(&misc->p_full[part], par, abort, err))) break;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               grad(do_at, kColDv, 0, 2 * k + part, first && part == 0 && k == 0);
           }
           if (!ok) break;
+          umma_commit_by(leader, &misc->empty[do_at]);
           int q_next = 0;
           if (more) {
             if (!(ok = (q_next = take()) >= 0)) break;
             scores(k_desc, q_next, 0, &misc->s_full);
           }
-          if (!(ok = mbar_wait(&misc->ds_full, par, abort, err))) break;
+          if (!(ok = mbar_wait_warp(&misc->ds_full, par, abort, err))) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 8; ++k) grad(q_at, kColDk, kColDp, k, first && k == 0);
+          umma_commit_by(leader, &misc->empty[q_at]);
           if (!more) break;
           q_at = q_next;
           if (!(ok = (do_at = take()) >= 0)) break;
@@ -816,7 +819,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
           par ^= 1;
           first = false;
         }
-        if (ok) umma_commit(&misc->acc_full);
+        if (ok) umma_commit_by(leader, &misc->acc_full);
       }
     } else if (warp == kFbCleaner) {
       if (MASKED) {
@@ -851,7 +854,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
     const bool key_ok = key < p.T && ((keys.w[warp & 3] >> lane) & 1u);
     uint4* const buf = reinterpret_cast<uint4*>(dsbuf) + (size_t)(wg * 4) * kBM + r;
     const float* const dl = reinterpret_cast<const float*>(smem + L::OFF_DELTA) + wg * 32;
-    int it = 0, ring = 0;   // ring: position of the previous query tile's Q, dO behind it
+    int it = 0;
     bool ok = true;
     for (FbWalk<MASKED> w = walk0; w.on(); w.next(), ++it) {
       const float* nl =
@@ -863,8 +866,6 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         break;
       }
       tc_fence_after();
-      // S(i) was issued behind dV(i - 1), which read dO(i - 1) last
-      if (it > 0 && lane == 0) mbar_arrive(&misc->empty[(ring + 1) % L::NS]);
       float pr[32];
       tmem_ld32(lane_addr, pr);
       tmem_wait_ld_dep(pr);
@@ -905,11 +906,6 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         break;
       }
       tc_fence_after();
-      // dP(i) was issued behind dK(i - 1), which read Q(i - 1) last
-      if (it > 0) {
-        if (lane == 0) mbar_arrive(&misc->empty[ring]);
-        ring = (ring + 2) % L::NS;
-      }
       uint32_t ds[16];
       {
         float x[32];

@@ -851,12 +851,12 @@ logits_kl_backward_kernel(const LogitsView sv, const LogitsView tv, const void* 
     map_row<T>(out, out, sv.V, share, Nothing{}, [](int, int, long long) { return 0.f; });
     return;
   }
-  const float g = (dloss ? *dloss : 1.f) * inv_tau, c = inv_tau * kLog2e;
-  const float zs = lse_s[row] * kLog2e, zt = lse_t[row] * kLog2e;
+  // the log probability first: a likely token's exponent is small and keeps its bits
+  const float g = (dloss ? *dloss : 1.f) * inv_tau, zs = lse_s[row], zt = lse_t[row];
   map_row<T>(s, out, sv.V, share, LoadPair<T>{s, t, same_offset(s, t)},
              [&](const Pair& v, int e, long long) {
-               return g * (ex2(fmaf(Elem<T>::get(v.s, e), c, -zs)) -
-                           ex2(fmaf(Elem<T>::get(v.t, e), c, -zt)));
+               return g * (ex2(fmaf(Elem<T>::get(v.s, e), inv_tau, -zs) * kLog2e) -
+                           ex2(fmaf(Elem<T>::get(v.t, e), inv_tau, -zt) * kLog2e));
              });
 }
 
