@@ -152,7 +152,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   FaMisc* misc = reinterpret_cast<FaMisc*>(smem + L::OFF_MISC);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int* err = &g_device_error;
   volatile int* abort = &misc->abort;
 
@@ -201,7 +201,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = misc->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, misc->tmem_base, 0);
   constexpr uint32_t kColO = 256;
 
   if (warp >= 8) {
@@ -232,7 +232,8 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
       // apart, so that one's softmax runs under the other's GEMMs.  (A thread a tile lets
       // them fall into step: 679 us instead of 541.)  The pipe waits for this thread, so
       // the loop keeps ring positions and descriptors in registers.
-      if (lane == 0 && kt0 >= 0) {
+      if (kt0 >= 0) {
+        const uint32_t leader = elect_one();
         const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
         const uint32_t id_o = idesc_f16(kBM, D, BF16, BF16, 0, 1);
         const uint64_t q_desc = kmajor_desc(smem_u32(smem + L::OFF_Q), 0);
@@ -253,26 +254,26 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint64_t off = (uint64_t)((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
-            umma_f16_ss(tmem + t * 128, qd + off, kd + off, id_s, kk > 0);
+            umma_f16_ss_by(leader, tmem + t * 128, qd + off, kd + off, id_s, kk > 0);
           }
-          umma_commit(&misc->s_full[t]);
+          umma_commit_by(leader, &misc->s_full[t]);
         };
         // O_t += P_t V, in the order in which P arrives
         auto sum = [&](int t, uint64_t vd, uint32_t parity, bool first) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (!mbar_wait(&misc->p_full[t][half], parity, abort, err)) return false;
+            if (!mbar_wait_warp(&misc->p_full[t][half], parity, abort, err)) return false;
             tc_fence_after();
 #pragma unroll
             for (int kk = half * 6; kk < 6 + half * 2; ++kk)
-              umma_f16_ts(tmem + kColO + t * D, tmem + t * 128 + kk * 8,
+              umma_f16_ts_by(leader, tmem + kColO + t * D, tmem + t * 128 + kk * 8,
                           vd + (uint64_t)(kk * 16 * 128 >> 4), id_o,
                           (!first || kk > 0) ? 1u : 0u);
           }
           return true;
         };
-        bool ok = mbar_wait(&misc->q_full, 0, abort, err) &&
-                  mbar_wait(&misc->k_full[0], 0, abort, err);
+        bool ok = mbar_wait_warp(&misc->q_full, 0, abort, err) &&
+                  mbar_wait_warp(&misc->k_full[0], 0, abort, err);
         uint32_t par[2] = {0, 0};
         bool on[2] = {false, false}, fresh[2] = {true, true};
         if (ok) {
@@ -286,8 +287,8 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
         while (ok) {
           kt = live_tile<MASKED>(bits, words, b, kt - 1);
           const bool more = kt >= 0;
-          if (!(ok = mbar_wait(&v_loaded[v_slot], v_phase, abort, err) &&
-                     (!more || mbar_wait(&misc->k_full[k_slot], k_phase, abort, err))))
+          if (!(ok = mbar_wait_warp(&v_loaded[v_slot], v_phase, abort, err) &&
+                     (!more || mbar_wait_warp(&misc->k_full[k_slot], k_phase, abort, err))))
             break;
           tc_fence_after();
           const uint64_t vd = v_desc + v_slot * kTile, kd = k_desc + k_slot * kTile;
@@ -297,7 +298,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
               ok = sum(t, vd, par[t], fresh[t]);
               par[t] ^= 1;
               fresh[t] = false;
-              if (ok && !more) umma_commit(&misc->o_full[t]);
+              if (ok && !more) umma_commit_by(leader, &misc->o_full[t]);
             }
             if (ok && more && kt < n_ct[t]) {
               score(t, kd);
@@ -1027,7 +1028,7 @@ attn_sm100_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const AttnProblem
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   FqMisc* misc = reinterpret_cast<FqMisc*>(smem + L::OFF_MISC);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   int* err = &g_device_error;
   volatile int* abort = &misc->abort;
   const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5, G = p.Hq / p.Hkv;
@@ -1069,7 +1070,7 @@ attn_sm100_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const AttnProblem
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = misc->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, misc->tmem_base, 0);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1094,35 +1095,38 @@ attn_sm100_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const AttnProblem
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t id = idesc_f16(kBM, D, BF16, BF16, 1, 1);
-      uint64_t* loaded = MASKED ? misc->ready : misc->full;
-      int n = 0, it = 0;
-      bool ok = true;
-      for (int rd = 0, w = work_at(0); ok && w < n_work; w = work_at(++rd)) {
-        const FqWork k = fq_work(p, c, n_t, w);
-        int kt = first_kt(k);
-        if (kt < 0) continue;
-        const int ab = it & 1;
-        if (it >= 2 && !mbar_wait(&misc->acc_empty[ab], ((it >> 1) - 1) & 1, abort, err)) break;
+    const uint32_t leader = elect_one();
+    const uint32_t id = idesc_f16(kBM, D, BF16, BF16, 1, 1);
+    const uint64_t a_desc = desc_interleave(smem_u32(smem), 128, kBM * 16);
+    const uint64_t b_desc = mnmajor_desc(smem_u32(smem) + L::DS_BYTES, 0);
+    uint64_t* loaded = MASKED ? misc->ready : misc->full;
+    int slot = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int rd = 0, w = work_at(0); ok && w < n_work; w = work_at(++rd)) {
+      const FqWork k = fq_work(p, c, n_t, w);
+      int kt = first_kt(k);
+      if (kt < 0) continue;
+      const int ab = it & 1;
+      if (it >= 2 && !mbar_wait_warp(&misc->acc_empty[ab], ((it >> 1) - 1) & 1, abort, err)) break;
+      tc_fence_after();
+      for (uint32_t more = 0; kt >= 0; kt = next_kt(k, kt), more = 1) {
+        if (!(ok = mbar_wait_warp(&loaded[slot], phase, abort, err))) break;
         tc_fence_after();
-        for (uint32_t more = 0; kt >= 0; kt = next_kt(k, kt), ++n, more = 1) {
-          const int s = n % L::NS;
-          if (!mbar_wait(&loaded[s], (n / L::NS) & 1, abort, err)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t at = smem_u32(smem + s * L::STAGE), bt = at + L::DS_BYTES;
+        const uint64_t off = (uint64_t)slot * (L::STAGE >> 4);   // descriptors count 16 bytes
 #pragma unroll
-          for (int kk = 0; kk < kBN / 16; ++kk)
-            umma_f16_ss(tmem + ab * 128, desc_interleave(at + kk * 2 * 128, 128, kBM * 16),
-                        mnmajor_desc(bt, kk), id, (more || kk > 0) ? 1u : 0u);
-          umma_commit(&misc->empty[s]);
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          umma_f16_ss_by(leader, tmem + ab * 128, a_desc + off + (uint64_t)(kk * 2 * 128 >> 4),
+                         b_desc + off + (uint64_t)(kk * 16 * 128 >> 4), id,
+                         (more || kk > 0) ? 1u : 0u);
+        umma_commit_by(leader, &misc->empty[slot]);
+        if (++slot == L::NS) {
+          slot = 0;
+          phase ^= 1;
         }
-        if (ok) umma_commit(&misc->acc_full[ab]);
-        ++it;
       }
+      if (ok) umma_commit_by(leader, &misc->acc_full[ab]);
+      ++it;
     }
   } else if (warp == 2) {
     if (MASKED) {
