@@ -345,7 +345,8 @@ size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_ma
  * 128 rows) and, on the tensor cores, the 16-bit dS tiles that the key-stationary
  * launch hands to the dq launch: all of them up to 8 GiB, beyond that the
  * backward runs in chunks of kv heads or, where one kv head's query heads need
- * more, of key tiles.  Less also works, in more chunks, down to the dS tiles of
+ * more, of key tiles; and, where one kv head's key tiles are few and long, fp32
+ * sums of dk and dv for up to four thread blocks each.  Less also works, in more chunks, down to the dS tiles of
  * one key tile ((Hq / Hkv) * ceil(T / 128) tiles of 32 KB) and one kv head's dq in fp32; below that
  * LKL_ERR_WORKSPACE. */
 size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);

@@ -42,6 +42,7 @@ bool attn_sm100_backward_supports(const AttnProblem& p, const AttnTensors& t);
 // summed over launches in attn_sm100_acc_bytes of fp32).
 size_t attn_stats_bytes(const AttnProblem& p);
 size_t attn_sm100_ds_bytes(const AttnProblem& p);
+size_t attn_sm100_sums_bytes(const AttnProblem& p);   // behind the dS tiles, optional
 size_t attn_sm100_ds_min_bytes(const AttnProblem& p);
 size_t attn_sm100_group_bytes(const AttnProblem& p);
 size_t attn_sm100_acc_bytes(const AttnProblem& p);

@@ -527,6 +527,7 @@ struct FbChunk {
   int g0, g1, j0, j1;
   int split;
   int band;            // kv groups per band of work items
+  int parts;           // CTAs that share a key tile (its query tiles in turn)
   long long tph;       // dS tiles per query head
 };
 
@@ -595,30 +596,27 @@ struct FbMisc {
 };
 static_assert(sizeof(FbMisc) <= 512, "misc region too small");
 
-// Next query tile at or above i with a token in it, or n_t.
-template <bool MASKED>
-__device__ __forceinline__ int live_tile_up(const uint32_t* bits, int words, int b, int i,
-                                            int n_t) {
-  if (MASKED)
-    while (i < n_t && !tile_bits<true>(bits, words, b, i).any()) ++i;
-  return i;
-}
-
-// The (query head, query tile) pairs of a dkv CTA, in the order every role takes them.
+// The (query head, query tile) pairs of a dkv CTA, in the order every role takes
+// them: of each head the tiles first_, first_ + step, ... that have a token.
 template <bool MASKED>
 struct FbWalk {
   const uint32_t* bits;
-  int words, b, n_t, first, h, h_end, i;
+  int words, b, n_t, step, first, h, h_end, i;
   __device__ __forceinline__ FbWalk(const uint32_t* bits_, int words_, int b_, int n_t_, int first_,
-                                    int h0, int G)
-      : bits(bits_), words(words_), b(b_), n_t(n_t_), h(h0), h_end(h0 + G) {
-    first = live_tile_up<MASKED>(bits, words, b, first_, n_t);
+                                    int step_, int h0, int G)
+      : bits(bits_), words(words_), b(b_), n_t(n_t_), step(step_), h(h0), h_end(h0 + G) {
+    first = live(first_);
     i = first;
     if (first >= n_t) h = h_end;
   }
+  __device__ __forceinline__ int live(int t) const {
+    if (MASKED)
+      while (t < n_t && !tile_bits<true>(bits, words, b, t).any()) t += step;
+    return t;
+  }
   __device__ __forceinline__ bool on() const { return h < h_end; }
   __device__ __forceinline__ void next() {
-    i = live_tile_up<MASKED>(bits, words, b, i + 1, n_t);
+    i = live(i + step);
     if (i >= n_t) {
       i = first;
       ++h;
@@ -635,7 +633,8 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_dk,
                       const __grid_constant__ CUtensorMap tm_dv, const AttnProblem p,
                       const FbChunk c, const uint32_t* __restrict__ bits,
-                      const float* __restrict__ stats, uint16_t* __restrict__ dsbuf) {
+                      const float* __restrict__ stats, uint16_t* __restrict__ dsbuf,
+                      float* __restrict__ sums) {
   using L = FbLayout<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
@@ -647,9 +646,10 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
 
   const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5, G = p.Hq / p.Hkv;
   // bands of kv groups, key tiles ascending (the longest first when causal)
+  const int part = (int)(blockIdx.x % c.parts);
   int lg, j;
   {
-    const int n_j = c.j1 - c.j0, n_g = c.g1 - c.g0, blk = blockIdx.x;
+    const int n_j = c.j1 - c.j0, n_g = c.g1 - c.g0, blk = (int)(blockIdx.x / c.parts);
     const int k = blk / (c.band * n_j), r = blk % (c.band * n_j);
     const int size = min(c.band, n_g - k * c.band);
     lg = k * c.band + r % size;
@@ -657,7 +657,8 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
   }
   const int grp = c.g0 + lg, b = grp / p.Hkv, g = grp % p.Hkv;
   const TileBits keys = tile_bits<MASKED>(bits, words, b, j);
-  const FbWalk<MASKED> walk0(bits, words, b, n_t, p.causal ? j : 0, g * G, keys.any() ? G : 0);
+  const FbWalk<MASKED> walk0(bits, words, b, n_t, (p.causal ? j : 0) + part, c.parts, g * G,
+                             keys.any() ? G : 0);
 
   if (threadIdx.x == 0) {
     mbar_init(&misc->kv_full, 1);
@@ -953,11 +954,24 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
       uint8_t* const tile = smem + (which ? L::OFF_K : L::OFF_V);
       const float scale = which ? p.sc : 1.f;
       const bool live = key_ok && it > 0;
+      // several CTAs a key tile: this one's fp32 sums, [part][dv, dk][group][T][D]
+      float* const sum_row =
+          sums + ((((size_t)part * 2 + which) * (c.g1 - c.g0) + lg) * p.T + key) * p.D;
 #pragma unroll
       for (int c2 = 0; c2 < D / 2; c2 += 32) {
         float v[32];
         tmem_ld32(row_addr + (which ? kColDk : kColDv) + col0 + c2, v);
         tmem_wait_ld_dep(v);
+        if (c.parts > 1) {
+          if (key >= p.T) continue;
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            if (col0 + c2 + k >= p.D) break;
+            *reinterpret_cast<float4*>(sum_row + col0 + c2 + k) =
+                live ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0, 0, 0, 0);
+          }
+          continue;
+        }
         uint32_t u[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2)
@@ -965,7 +979,7 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         stage_row32(tile, r, col0 + c2, u);
       }
       named_bar(1 + which, 256);
-      if ((wg & 1) == 0)
+      if ((wg & 1) == 0 && c.parts == 1)
         store_rows_tma<D>(which ? &tm_dk : &tm_dv, tile, warp & 3, lane, j * kBN, p.T, g, b);
     }
   }
@@ -975,6 +989,36 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
   if (warp == kFbMma) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// dk and dv of key rows [j0, j1) * 128 of a chunk: the parts' sums in their order, rounded.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+attn_sm100_sum_parts_kernel(const AttnProblem p, const AttnTensors a, const FbChunk c,
+                            const float* __restrict__ sums) {
+  const int n8 = p.D / 8, r0 = c.j0 * kBN, rows = min(p.T, c.j1 * kBN) - r0, n_g = c.g1 - c.g0;
+  const long long total = 2ll * n_g * rows * n8;
+  for (long long x = blockIdx.x * 256ll + threadIdx.x; x < total; x += gridDim.x * 256ll) {
+    const int col = (int)(x % n8) * 8;
+    const long long y = x / n8;
+    const int key = r0 + (int)(y % rows), lg = (int)(y / rows) % n_g, which = (int)(y / rows / n_g);
+    float v[8] = {};
+    for (int part = 0; part < c.parts; ++part) {
+      const float4* from = reinterpret_cast<const float4*>(
+          sums + ((((size_t)part * 2 + which) * n_g + lg) * p.T + key) * p.D + col);
+      const float4 lo = from[0], hi = from[1];
+      v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+      v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+    }
+    const float sc = which ? p.sc : 1.f;
+    const int grp = c.g0 + lg, b = grp / p.Hkv, g = grp % p.Hkv;
+    const TensorStrides& st = which ? a.sdk : a.sdv;
+    uint16_t* row = static_cast<uint16_t*>(which ? a.dk : a.dv) + (size_t)b * st.b +
+                    (size_t)g * st.h + (size_t)key * st.t + col;
+    *reinterpret_cast<uint4*>(row) =
+        make_uint4(pack2t<BF16>(v[0] * sc, v[1] * sc), pack2t<BF16>(v[2] * sc, v[3] * sc),
+                   pack2t<BF16>(v[4] * sc, v[5] * sc), pack2t<BF16>(v[6] * sc, v[7] * sc));
   }
 }
 
@@ -1244,12 +1288,35 @@ FbPlan fb_plan(const AttnProblem& p, long long cap_tiles) {
   return FbPlan{1, (int)std::min<long long>(n_t, keys), true};
 }
 
+// CTAs a key tile.  Few and long work items leave the GPU waiting for the longest (2 kv
+// heads of 4 query heads, 15001 tokens: 236 items, 472 query tiles in the longest, 379
+// a SM on average): below three items a SM up to four CTAs share one, and their fp32
+// sums of dk and dv are joined by a small launch (890 -> 815 + 17 us there; with 512
+// items, 32 / 8 heads x 8192, it only costs 35 us).  Each keeps 16 query tiles on average.
+constexpr int kFbSms = 148;
+int fb_parts(const AttnProblem& p, const FbPlan& plan) {
+  const long long n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv;
+  const long long items = (long long)plan.per * plan.keys;
+  const long long tiles = G * (p.causal ? (n_t + 1) / 2 : n_t);
+  const long long want = (3 * kFbSms + items - 1) / items;
+  return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(want, 4), tiles / 16));
+}
+size_t fb_sums_bytes(const AttnProblem& p, const FbPlan& plan) {
+  const int parts = fb_parts(p, plan);
+  return parts > 1 ? (size_t)parts * 2 * plan.per * p.T * p.D * 4 : 0;
+}
+
 template <int D, bool BF16, bool MASKED>
 cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
                               float* stats, uint16_t* dsbuf, size_t ds_bytes, float* acc32,
                               cudaStream_t st) {
-  const FbPlan plan = fb_plan(p, (long long)(ds_bytes / (kDTileElems * 2)));
+  // [dS tiles][fp32 sums of dv and dk, where the scratch has room for them]
+  const size_t tiles = std::min(ds_bytes, attn_sm100_ds_bytes(p));
+  const FbPlan plan = fb_plan(p, (long long)(tiles / (kDTileElems * 2)));
   if (plan.keys <= 0) return cudaErrorInvalidValue;
+  const size_t sums_at = (tiles + 255) & ~size_t(255), sums_bytes = fb_sums_bytes(p, plan);
+  const int parts = sums_bytes && ds_bytes >= sums_at + sums_bytes ? fb_parts(p, plan) : 1;
+  float* sums = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(dsbuf) + sums_at);
   CUtensorMap mq, mk, mv, mdo, mdk, mdv;
   if (!attn_map(&mq, t.q, p, p.Hq, t.sq) || !attn_map(&mk, t.k, p, p.Hkv, t.sk) ||
       !attn_map(&mv, t.v, p, p.Hkv, t.sv) || !attn_map(&mdo, t.dout, p, p.Hq, t.sdo) ||
@@ -1276,13 +1343,20 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
       c.j0 = j0;
       c.j1 = std::min(n_t, j0 + plan.keys);
       c.split = plan.split;
+      c.parts = parts;
       c.band = (int)std::max<long long>(
           1, std::min<long long>(c.g1 - g0, (64ll << 20) / std::max<long long>(group_bytes, 1)));
       const int i0 = p.causal ? j0 : 0;
       c.tph = plan.split ? (long long)(n_t - i0) * (c.j1 - j0) : fb_tiles_per_head(p);
-      kkv<<<(c.g1 - g0) * (c.j1 - j0), kFbThreads, FbLayout<D>::BYTES, st>>>(
-          mq, mk, mv, mdo, mdk, mdv, p, c, bits, stats, dsbuf);
+      kkv<<<(c.g1 - c.g0) * (c.j1 - c.j0) * parts, kFbThreads, FbLayout<D>::BYTES, st>>>(
+          mq, mk, mv, mdo, mdk, mdv, p, c, bits, stats, dsbuf, sums);
       if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      if (parts > 1) {
+        const long long n = 2ll * (c.g1 - c.g0) * (std::min(p.T, c.j1 * kBN) - j0 * kBN) * (p.D / 8);
+        attn_sm100_sum_parts_kernel<BF16><<<(int)std::min<long long>((n + 255) / 256, 4 * kFbSms),
+                                            256, 0, st>>>(p, t, c, sums);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      }
       const int work = (c.g1 - g0) * G * (n_t - i0);
       kq<<<std::min(work, num_sms), kFqThreads, FqLayout<D>::BYTES, st>>>(mk, p, t, c, bits, dsbuf,
                                                                           acc32);
@@ -1320,6 +1394,10 @@ size_t attn_sm100_ds_bytes(const AttnProblem& p) {
   const long long all = fb_tiles_per_head(p) * p.B * p.Hq * kDTileElems * 2;
   const long long min = (long long)attn_sm100_ds_min_bytes(p);
   return (size_t)std::min(all, std::max(kDBufCapBytes, min));
+}
+
+size_t attn_sm100_sums_bytes(const AttnProblem& p) {
+  return fb_sums_bytes(p, fb_plan(p, (long long)(attn_sm100_ds_bytes(p) / (kDTileElems * 2))));
 }
 
 size_t attn_sm100_ds_min_bytes(const AttnProblem& p) {

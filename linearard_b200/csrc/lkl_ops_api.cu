@@ -127,7 +127,7 @@ size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_m
   if (a.D > 128) return n;
   const size_t ds = lkl::attn_sm100_ds_bytes(a);
   if (ds < lkl::attn_sm100_group_bytes(a)) n += round256(lkl::attn_sm100_acc_bytes(a));
-  return n + round256(ds);
+  return n + round256(ds) + round256(lkl::attn_sm100_sums_bytes(a));
 }
 
 int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_strides* strides,
@@ -197,7 +197,7 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   if (tc)
     return launch_status(lkl::launch_attn_sm100_backward(
         a, t, bits, reinterpret_cast<float*>(base + at.stats), base + at.ds,
-        std::min(at.ds_bytes, lkl::attn_sm100_ds_bytes(a)),
+        at.ds_bytes,
         reinterpret_cast<float*>(base + at.acc), st));
   float2* rows = reinterpret_cast<float2*>(base + at.stats);
   if ((s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;

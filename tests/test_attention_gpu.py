@@ -315,3 +315,17 @@ def test_nothing_to_do():
         assert out.shape == q.shape
         out.sum().backward()
         assert q.grad.shape == q.shape
+
+
+@pytest.mark.parametrize("Hq,Hkv,causal,mask", [(2, 1, True, False), (1, 1, False, True),
+                                                (4, 2, True, True)])
+def test_long_key_tiles_are_shared(Hq, Hkv, causal, mask):
+    """Few key tiles with many query tiles each: several blocks share one and their
+    sums are joined.  The same bounds, and the same bits every time."""
+    T = 4300
+    q, k, v, g = make(1, Hq, Hkv, T, 64, "bf16")
+    m = right_pad(1, T, [4111]) if mask else None
+    check(q, k, v, g, m, causal)
+    out, lse = attn_forward(q, k, v, m, causal)
+    a, b = (attn_backward(g, q, k, v, out, lse, m, causal) for _ in range(2))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
