@@ -78,7 +78,10 @@ def _readable(t):
 def _like(t):
     """An uninitialised tensor of t's shape and type, in its order of heads and tokens."""
     B, H, T, D = t.shape
-    if t.stride(1) < t.stride(2):
+    s = t.stride()
+    if s == (H * T * D, T * D, D, 1) or s == (T * H * D, D, H * D, 1):
+        return torch.empty_like(t)      # dense: keeps the strides
+    if s[1] < s[2]:
         return torch.empty((B, T, H, D), device=t.device, dtype=t.dtype).transpose(1, 2)
     return torch.empty((B, H, T, D), device=t.device, dtype=t.dtype)
 
@@ -92,38 +95,41 @@ def _workspace(n, device):
 
 
 def _forward(q, k, v, mask, prob):
-    """out and lse of checked arguments; mask on the device or None."""
+    """(out, lse, plan) of checked arguments; mask on the device or None.  plan: the
+    strides of q, k, v and out for the backward, None where one had to be copied."""
     L, dev = _lib.lib(), q.device
     with on_device(dev):
-        (q, sq), (k, sk), (v, sv) = _readable(q), _readable(k), _readable(v)
-        out = _like(q)
+        (rq, sq), (rk, sk), (rv, sv) = _readable(q), _readable(k), _readable(v)
+        out = _like(rq)
         lse = torch.empty((prob.B, prob.Hq, prob.T), device=dev, dtype=torch.float32)
         ref = ctypes.byref(prob)
-        n, ws, at = 0, None, None
+        n, ws, at, m = 0, None, None, None
         if mask is not None:
-            n = L.lkl_attn_forward_workspace_size(ref, 1)
+            n, m = L.lkl_attn_forward_workspace_size(ref, 1), mask.data_ptr()
             ws, at = _workspace(n, dev)
-        st = L.lkl_attn_forward(q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                (ctypes.c_int64 * 12)(*sq, *sk, *sv, *_strides(out)),
-                                None if mask is None else mask.data_ptr(), ref, out.data_ptr(),
+        strides = (*sq, *sk, *sv, *_strides(out))
+        st = L.lkl_attn_forward(rq.data_ptr(), rk.data_ptr(), rv.data_ptr(),
+                                (ctypes.c_int64 * 12)(*strides), m, ref, out.data_ptr(),
                                 lse.data_ptr(), at, n, raw_stream(dev))
     _lib.check(st, "lkl_attn_forward")
-    return out, lse
+    return out, lse, strides if rq is q and rk is k and rv is v else None
 
 
-def _backward(dout, q, k, v, out, lse, mask, prob):
+def _backward(dout, q, k, v, out, lse, mask, prob, plan=None):
     L, dev = _lib.lib(), q.device
     with on_device(dev):
         dq, dk, dv = _like(q), _like(k), _like(v)
-        (q, sq), (k, sk), (v, sv), (out, so), (dout, sd) = (_readable(t)
-                                                            for t in (q, k, v, out, dout))
+        if plan is None:
+            (q, sq), (k, sk), (v, sv), (out, so) = (_readable(t) for t in (q, k, v, out))
+            plan = (*sq, *sk, *sv, *so)
+        dout, sd = _readable(dout)
         ref = ctypes.byref(prob)
         n = L.lkl_attn_backward_workspace_size(ref, 0 if mask is None else 1)
         ws, at = _workspace(n, dev)
         st = L.lkl_attn_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            dout.data_ptr(), (ctypes.c_int64 * 24)(*sq, *sk, *sv, *so, *sd, *_strides(dq),
-                                                   *_strides(dk), *_strides(dv)),
+            dout.data_ptr(), (ctypes.c_int64 * 24)(*plan, *sd, *_strides(dq), *_strides(dk),
+                                                   *_strides(dv)),
             None if mask is None else mask.data_ptr(), ref, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), at, n, raw_stream(dev))
     _lib.check(st, "lkl_attn_backward")
@@ -135,7 +141,7 @@ def attn_forward(q, k, v, attn_mask=None, causal=True, sm_scale=None):
     Rows that the mask removes have out 0 and lse 0."""
     _check(q, k, v)
     mask, mdt = prepare_mask(attn_mask, q.shape[0], q.shape[2], q.device)
-    return _forward(q, k, v, mask, _problem(q, k, causal, mdt, sm_scale))
+    return _forward(q, k, v, mask, _problem(q, k, causal, mdt, sm_scale))[:2]
 
 
 def attn_backward(dout, q, k, v, out, lse, attn_mask=None, causal=True, sm_scale=None):
@@ -155,7 +161,7 @@ def attn_backward(dout, q, k, v, out, lse, attn_mask=None, causal=True, sm_scale
 class AttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, prob):
-        out, lse = _forward(q, k, v, mask, prob)
+        out, lse, ctx.plan = _forward(q, k, v, mask, prob)
         ctx.save_for_backward(q, k, v, out, lse, mask)
         ctx.prob = prob
         return out
@@ -163,7 +169,7 @@ class AttnFn(torch.autograd.Function):
     @once_when_recorded
     def backward(ctx, dout):
         q, k, v, out, lse, mask = ctx.saved_tensors
-        dq, dk, dv = _backward(dout, q, k, v, out, lse, mask, ctx.prob)
+        dq, dk, dv = _backward(dout, q, k, v, out, lse, mask, ctx.prob, ctx.plan)
         return dq, dk, dv, None, None
 
 
