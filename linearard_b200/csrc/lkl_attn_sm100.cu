@@ -170,7 +170,11 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
   }
   const int kt0 = live_tile<MASKED>(bits, words, b, max(n_ct[0], n_ct[1]) - 1);
 
-  if (threadIdx.x == 0) {
+  // The producer sets the barriers up and starts the first loads before the block meets.
+  if (warp == kFaProducer && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
     mbar_init(&misc->q_full, 1);
     const int users = 4 * ((n_ct[0] > 0) + (n_ct[1] > 0));   // softmax warps
     for (int s = 0; s < 4; ++s) {
@@ -188,15 +192,23 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
     }
     misc->abort = 0;
     fence_barrier_init();
+    fence_proxy_async_smem();
+    if (kt0 >= 0) {
+      mbar_arrive_expect_tx(&misc->q_full, ((n_ct[0] > 0) + (n_ct[1] > 0)) * L::TILE);
+      mbar_arrive_expect_tx(&misc->k_full[0], L::TILE);
+      mbar_arrive_expect_tx(&misc->v_full[0], L::TILE);
+      issue_tile_loads(smem + L::OFF_K, &tm_k, &misc->k_full[0], D, kt0 * kBN, g, b);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (n_ct[t] > 0)
+          issue_tile_loads(smem + L::OFF_Q + t * L::TILE, &tm_q, &misc->q_full, D,
+                           (wk.m * 2 + t) * kBM, h, b);
+      issue_tile_loads(smem + L::OFF_V, &tm_v, &misc->v_full[0], D, kt0 * kBN, g, b);
+    }
   }
   if (warp == kFaMma) {
     tmem_alloc(&misc->tmem_base, kTmemCols);
     tmem_relinquish();
-  }
-  if (warp == kFaProducer && lane == 0) {
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
   }
   tc_fence_before();
   __syncthreads();
@@ -208,14 +220,9 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
     reg_dec<kFaOtherRegs>();
     if (warp == kFaProducer) {
       if (lane == 0 && kt0 >= 0) {
-        mbar_arrive_expect_tx(&misc->q_full, ((n_ct[0] > 0) + (n_ct[1] > 0)) * L::TILE);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (n_ct[t] > 0)
-            issue_tile_loads(smem + L::OFF_Q + t * L::TILE, &tm_q, &misc->q_full, D,
-                             (wk.m * 2 + t) * kBM, h, b);
-        int n = 0;
-        for (int kt = kt0; kt >= 0; kt = live_tile<MASKED>(bits, words, b, kt - 1), ++n) {
+        int n = 1;   // the first tiles are on their way
+        for (int kt = live_tile<MASKED>(bits, words, b, kt0 - 1); kt >= 0;
+             kt = live_tile<MASKED>(bits, words, b, kt - 1), ++n) {
           const int sk = n % L::NK, sv = n % L::NV;
           if (n >= L::NK && !mbar_wait(&misc->k_empty[sk], (n / L::NK - 1) & 1, abort, err)) break;
           mbar_arrive_expect_tx(&misc->k_full[sk], L::TILE);
@@ -660,7 +667,12 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
   const FbWalk<MASKED> walk0(bits, words, b, n_t, (p.causal ? j : 0) + part, c.parts, g * G,
                              keys.any() ? G : 0);
 
-  if (threadIdx.x == 0) {
+  // The producer sets the barriers up and starts the first loads before the block meets.
+  if (warp == kFbProducer && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_do);
     mbar_init(&misc->kv_full, 1);
     for (int s = 0; s < L::NS; ++s) {
       mbar_init(&misc->full[s], 1);
@@ -680,16 +692,22 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
     mbar_init(&misc->acc_full, 1);
     misc->abort = 0;
     fence_barrier_init();
+    fence_proxy_async_smem();
+    if (walk0.on()) {
+      mbar_arrive_expect_tx(&misc->kv_full, 2 * L::TILE);
+      issue_tile_loads(smem + L::OFF_K, &tm_k, &misc->kv_full, D, j * kBN, g, b);
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        mbar_arrive_expect_tx(&misc->full[o], L::TILE);
+        issue_tile_loads(smem + L::OFF_RING + o * L::TILE, o ? &tm_do : &tm_q, &misc->full[o], D,
+                         walk0.i * kBM, walk0.h, b);
+        if (o == 0) issue_tile_loads(smem + L::OFF_V, &tm_v, &misc->kv_full, D, j * kBN, g, b);
+      }
+    }
   }
   if (warp == kFbMma) {
     tmem_alloc(&misc->tmem_base, kTmemCols);
     tmem_relinquish();
-  }
-  if (warp == kFbProducer && lane == 0) {
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-    tma_prefetch_desc(&tm_do);
   }
   tc_fence_before();
   __syncthreads();
@@ -700,12 +718,10 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
     reg_dec<kFbOtherRegs>();
     if (warp == kFbProducer) {
       if (lane == 0 && walk0.on()) {
-        mbar_arrive_expect_tx(&misc->kv_full, 2 * L::TILE);
-        issue_tile_loads(smem + L::OFF_K, &tm_k, &misc->kv_full, D, j * kBN, g, b);
-        issue_tile_loads(smem + L::OFF_V, &tm_v, &misc->kv_full, D, j * kBN, g, b);
-        int n = 0;   // Q(0), dO(0), Q(1), dO(1), ...
+        int n = 2;   // Q(0), dO(0), which are on their way, Q(1), dO(1), ...
         bool ok = true;
-        for (FbWalk<MASKED> w = walk0; ok && w.on(); w.next())
+        FbWalk<MASKED> w = walk0;
+        for (w.next(); ok && w.on(); w.next())
           for (int o = 0; o < 2; ++o, ++n) {
             const int s = n % L::NS;
             if (n >= L::NS && !mbar_wait(&misc->empty[s], (n / L::NS - 1) & 1, abort, err)) {
