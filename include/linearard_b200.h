@@ -63,7 +63,9 @@ enum lkl_status {
   LKL_ERR_LAUNCH = 7,           /* a kernel launch or driver call failed             */
   LKL_ERR_NO_DEVICE = 8,        /* current device is not sm_100 / no CUDA device     */
   LKL_ERR_DEVICE_TIMEOUT = 9,   /* a device-side bounded wait expired (see below)    */
-  LKL_ERR_BAD_ALIAS = 10,       /* dq == dk requires qs == ks and Hkv_s == Hq        */
+  LKL_ERR_BAD_ALIAS = 10,       /* dq == dk requires qs == ks and Hkv_s == Hq; an
+                                   output of the attention or logits calls that is
+                                   one of their inputs                               */
   LKL_ERR_TOO_LARGE = 11,       /* a size exceeds what the entry point supports      */
   LKL_ERR_UNSUPPORTED = 12      /* strided inputs on a shape the tensor-core path
                                    does not cover (ABI version 3)                     */
@@ -322,7 +324,8 @@ int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, cons
  * every pointer is 16-byte aligned and every stride a positive multiple of 8
  * elements; everything else runs on CUDA-core kernels.  lkl_last_path() tells which.
  * Sums and softmax statistics are fp32; P and dS are rounded to the tensors'
- * type before their products on the tensor cores.  Results are reproducible
+ * type before their products on the tensor cores (in fp16 a dS beyond 65504
+ * overflows: scale the loss so that dout . v stays below).  Results are reproducible
  * bit for bit: every output row has one writer.
  * May be captured into CUDA graphs. */
 typedef struct lkl_attn_problem {
@@ -387,7 +390,7 @@ int32_t lkl_token_logprobs(const void* logits, const lkl_logits* l, const int64_
                            int64_t ignore_index, int32_t top_k, float* logprob, float* entropy,
                            float* lse, float* top_logprobs, int64_t* top_indices, void* stream);
 
-/* d_logits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy), g =
+/* May not write over the logits.  d_logits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy), g =
  * d_logprob (0 for an ignored target, NaN for one outside [0, V)), h =
  * d_entropy; NULL means 0.  d_logits: contiguous [B, T, V] of the logits' type. */
 int32_t lkl_token_logprobs_backward(const void* logits, const lkl_logits* l,

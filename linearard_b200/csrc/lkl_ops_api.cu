@@ -32,24 +32,23 @@ AttnProblem to_attn(const lkl_attn_problem* p) {
 inline size_t attn_bits_bytes(const lkl_attn_problem* p) {
   return round256((size_t)p->B * (size_t)((p->T + 31) / 32) * sizeof(uint32_t));
 }
-// Backward scratch: [mask bits][row statistics][fp32 dq sums][dS tiles]; the
+// Backward scratch: [mask bits][row statistics][fp32 dq sums][dS tiles ...]; the
 // sums only where the tiles of one kv group do not fit at once.
+size_t attn_stats_end(const lkl_attn_problem* p, bool has_mask) {
+  return (has_mask ? attn_bits_bytes(p) : 0) + round256(lkl::attn_stats_bytes(to_attn(p)));
+}
 struct AttnScratch {
-  size_t stats, acc, ds, ds_bytes;   // offsets, and the bytes left for dS
+  size_t acc, ds, ds_bytes;   // offsets, and the bytes left from ds on
 };
 AttnScratch attn_scratch(const lkl_attn_problem* p, bool has_mask, size_t ws_bytes) {
   const AttnProblem a = to_attn(p);
+  const size_t group = lkl::attn_sm100_group_bytes(a);
   AttnScratch s;
-  s.stats = has_mask ? attn_bits_bytes(p) : 0;
-  s.acc = s.ds = s.stats + round256(lkl::attn_stats_bytes(a));
-  if (ws_bytes < s.ds + lkl::attn_sm100_group_bytes(a))
+  s.acc = s.ds = attn_stats_end(p, has_mask);
+  if (ws_bytes < s.ds + group || lkl::attn_sm100_ds_bytes(a) < group)
     s.ds += round256(lkl::attn_sm100_acc_bytes(a));
   s.ds_bytes = ws_bytes > s.ds ? ws_bytes - s.ds : 0;
   return s;
-}
-// What the CUDA-core backward needs; the tensor cores' add dS tiles.
-size_t attn_backward_base(const lkl_attn_problem* p, bool has_mask) {
-  return attn_scratch(p, has_mask, SIZE_MAX).ds;
 }
 
 // Strides of tensor `which` (`strides` or the contiguous ones).
@@ -123,11 +122,10 @@ size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_ma
 size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask) {
   if (check_attn(p) != LKL_OK || p->B == 0 || p->T == 0) return 0;
   const AttnProblem a = to_attn(p);
-  size_t n = attn_backward_base(p, has_mask != 0);
+  const size_t n = attn_stats_end(p, has_mask != 0);
   if (a.D > 128) return n;
-  const size_t ds = lkl::attn_sm100_ds_bytes(a);
-  if (ds < lkl::attn_sm100_group_bytes(a)) n += round256(lkl::attn_sm100_acc_bytes(a));
-  return n + round256(ds) + round256(lkl::attn_sm100_sums_bytes(a));
+  return attn_scratch(p, has_mask != 0, SIZE_MAX).ds + round256(lkl::attn_sm100_ds_bytes(a)) +
+         round256(lkl::attn_sm100_sums_bytes(a));
 }
 
 int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_strides* strides,
@@ -139,6 +137,7 @@ int32_t lkl_attn_forward(const void* q, const void* k, const void* v, const lkl_
   if (!q || !k || !v || !out || !lse) return LKL_ERR_NULL_POINTER;
   if (!aligned(q, 2) || !aligned(k, 2) || !aligned(v, 2) || !aligned(out, 2) || !aligned(lse, 4))
     return LKL_ERR_MISALIGNED;
+  if (out == q || out == k || out == v) return LKL_ERR_BAD_ALIAS;
   if ((s = check_mask(mask, p->mask_dtype)) || (s = check_attn_strides(strides, 4))) return s;
   if ((s = check_workspace(lkl_attn_forward_workspace_size(p, mask != nullptr), ws, ws_bytes)))
     return s;
@@ -170,9 +169,11 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   for (const void* x : all)
     if (!aligned(x, 2)) return LKL_ERR_MISALIGNED;
   if (!aligned(lse, 4)) return LKL_ERR_MISALIGNED;
-  if (dq == dk || dq == dv || dk == dv) return LKL_ERR_BAD_ALIAS;
+  for (int g = 5; g < 8; ++g)   // a gradient is neither an input nor another gradient
+    for (int x = 0; x < g; ++x)
+      if (all[g] == all[x]) return LKL_ERR_BAD_ALIAS;
   if ((s = check_mask(mask, p->mask_dtype)) || (s = check_attn_strides(strides, 8))) return s;
-  if ((s = check_workspace(attn_backward_base(p, mask != nullptr), ws, ws_bytes))) return s;
+  if ((s = check_workspace(attn_stats_end(p, mask != nullptr), ws, ws_bytes))) return s;
   AttnTensors t{};
   t.q = q, t.k = k, t.v = v, t.out = const_cast<void*>(out), t.lse = const_cast<float*>(lse);
   t.dout = dout, t.dq = dq, t.dk = dk, t.dv = dv;
@@ -193,13 +194,14 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
   uint32_t* bits;
   if ((s = attn_bits(p, mask, ws, &bits, st))) return s;
   uint8_t* const base = static_cast<uint8_t*>(ws);
+  float* const stats = reinterpret_cast<float*>(base + (mask ? attn_bits_bytes(p) : 0));
   t_last_path = tc ? 1 : 0;
   if (tc)
     return launch_status(lkl::launch_attn_sm100_backward(
-        a, t, bits, reinterpret_cast<float*>(base + at.stats), base + at.ds,
+        a, t, bits, stats, base + at.ds,
         at.ds_bytes,
         reinterpret_cast<float*>(base + at.acc), st));
-  float2* rows = reinterpret_cast<float2*>(base + at.stats);
+  float2* rows = reinterpret_cast<float2*>(stats);
   if ((s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;
   return launch_status(lkl::launch_attn_generic_backward(a, t, bits, rows, st));
 }
@@ -231,6 +233,7 @@ int32_t lkl_token_logprobs_backward(const void* logits, const lkl_logits* l,
   if (s) return s;
   if (l->B * l->T == 0) return LKL_OK;
   if (!targets || !lse || !entropy || !d_logits) return LKL_ERR_NULL_POINTER;
+  if (d_logits == logits) return LKL_ERR_BAD_ALIAS;
   if (!aligned(targets, 8) || !aligned(lse, 4) || !aligned(entropy, 4) ||
       !aligned(d_logprob, 4) || !aligned(d_entropy, 4) ||
       !aligned(d_logits, logits_elem(l->dtype)))
@@ -275,6 +278,7 @@ int32_t lkl_logits_kl_backward(const void* s_logits, const lkl_logits* s, const 
   if (e) return e;
   if (s->B * s->T == 0) return LKL_OK;
   if (!lse_s || !lse_t || !ds) return LKL_ERR_NULL_POINTER;
+  if (ds == s_logits || ds == t_logits) return LKL_ERR_BAD_ALIAS;
   if (!aligned(lse_s, 4) || !aligned(lse_t, 4) || !aligned(dloss, 4) ||
       !aligned(ds, logits_elem(s->dtype)))
     return LKL_ERR_MISALIGNED;

@@ -329,3 +329,53 @@ def test_long_key_tiles_are_shared(Hq, Hkv, causal, mask):
     out, lse = attn_forward(q, k, v, m, causal)
     a, b = (attn_backward(g, q, k, v, out, lse, m, causal) for _ in range(2))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_captured_through_autograd():
+    """Forward and torch.autograd.grad inside one capture, after a warm-up on the
+    capture's stream whose graph is gone (autograd ties the leaves of a living graph
+    to the stream that it was built on)."""
+    q, k, v, g = (t.detach() for t in make(1, 2, 2, 260, 64, "bf16"))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        torch.autograd.grad(attn(*leaves), leaves, g)
+        with torch.cuda.graph(graph, stream=s):
+            out = attn(*leaves)
+            grads = torch.autograd.grad(out, leaves, g)
+    graph.replay()
+    torch.cuda.synchronize()
+    o, z = attn_forward(q, k, v)
+    assert torch.equal(out, o)
+    for a, b in zip(grads, attn_backward(g, q, k, v, o, z)):
+        assert torch.equal(a, b)
+
+
+def test_no_second_derivative():
+    q, k, v, g = make(1, 2, 2, 40, 64, "bf16")
+    q = q.detach().requires_grad_(True)
+    (d,) = torch.autograd.grad(attn(q, k, v), q, g, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), q)
+
+
+def test_refusals():
+    q, k, v, g = make(2, 4, 2, 40, 64, "bf16", "bhtd")
+    for bad in ((q.float(), k, v), (q, k, v.half()), (q[..., :60], k[..., :60], v[..., :60]),
+                (q[:, :3], k, v), (q, k[:, :, :30], v[:, :, :30]), (q, k, v[:, :1]),
+                (q.transpose(2, 3), k, v), (q[0], k[0], v[0])):
+        with pytest.raises(AssertionError):
+            attn(*bad)
+    for mask in (torch.ones(2, 41, device="cuda", dtype=torch.int64), torch.ones(2, 40, device="cuda"),
+                 torch.ones(2, 1, 40, 40, device="cuda", dtype=torch.bool), [1, 2]):
+        with pytest.raises(AssertionError):
+            attn(q, k, v, mask)
+    for sc in (0.0, -1.0, float("nan"), float("inf"), "1"):
+        with pytest.raises(AssertionError):
+            attn(q, k, v, sm_scale=sc)
+    out, lse = attn_forward(q, k, v)
+    for bad in ((g.float(), out, lse), (g, out[:, :2], lse), (g, out, lse.half()), (g, out, lse[:, :2])):
+        with pytest.raises(AssertionError):
+            attn_backward(bad[0], q, k, v, *bad[1:])

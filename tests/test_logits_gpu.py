@@ -298,3 +298,42 @@ def test_nothing_to_do():
     assert loss.item() == 0
     loss.backward()
     assert x.grad.shape == x.shape
+
+
+def test_no_second_derivative():
+    x, y = logits(3, 50, dtype="fp32").requires_grad_(True), logits(3, 50, dtype="fp32", seed=1)
+    for f in (lambda: token_logprobs(x, torch.zeros(3, dtype=torch.int64, device="cuda")).logprob.sum(),
+              lambda: logits_kl_align(x, y)):
+        (d,) = torch.autograd.grad(f(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(d.sum(), x)
+
+
+def test_refusals():
+    x = logits(2, 5, 100)
+    ids = torch.zeros(2, 5, dtype=torch.int64, device="cuda")
+    for a, b, kw in ((x.double(), ids, {}), (x, ids.int(), {}), (x, ids[:, :4], {}), (x, ids.cpu(), {}),
+                     (x.transpose(1, 2), ids, {}), (x[None], ids[None], {}), (x, ids, dict(top_k=33)),
+                     (x, ids, dict(top_k=-1)), (x[..., :3], ids, dict(top_k=4)),
+                     (x, ids, dict(top_k=1.5)), (x, ids, dict(ignore_index=None))):
+        with pytest.raises(AssertionError):
+            token_logprobs(a, b, **kw)
+    m = torch.ones(2, 5, device="cuda", dtype=torch.bool)
+    for a, b, kw in ((x, x.float(), {}), (x, x[:, :4], {}), (x, x.cpu(), {}),
+                     (x, x, dict(temperature=0.0)), (x, x, dict(temperature=float("nan"))),
+                     (x, x, dict(temperature="1")), (x, x, dict(attn_mask=m[:, :4])),
+                     (x, x, dict(attn_mask=m.float())), (x.transpose(1, 2), x.transpose(1, 2), {})):
+        with pytest.raises(AssertionError):
+            logits_kl_align(a, b, **kw)
+
+
+def test_gradients_of_what_is_seen_twice():
+    """The same row for the whole batch, and one tensor as student and teacher."""
+    row = logits(1, 4, 300, dtype="fp32").requires_grad_(True)
+    ids = torch.arange(8, device="cuda").view(2, 4)
+    (d,) = torch.autograd.grad(token_logprobs(row.expand(2, -1, -1), ids).logprob.sum(), row)
+    many = row.detach().expand(2, -1, -1).contiguous()
+    ref = TokenRef(many, ids, g=torch.ones(2, 4, device="cuda"))
+    assert_within(d, ref.d.sum(0, keepdim=True), ref.d_tol.sum(0, keepdim=True), "d_row")
+    (d,) = torch.autograd.grad(logits_kl_align(row, row), row)
+    assert (d == 0).all()

@@ -9,7 +9,7 @@ from linearard_b200 import _lib
 from linearard_b200.attention import attn, attn_forward
 from linearard_b200.logits import logits_kl_align, token_logprobs
 
-FAKE, FAKE2, FAKE3 = (ctypes.c_void_p(0x10000 * i) for i in (1, 2, 3))
+FAKE, FAKE2, FAKE3, FAKE4 = (ctypes.c_void_p(0x10000 * i) for i in (1, 2, 3, 4))
 
 
 def prob(**kw):
@@ -51,7 +51,7 @@ def test_attention_refuses_bad_problems(kw, code):
     p = prob(**kw)
     assert fwd(p) == code
     assert _lib.lib().lkl_attn_backward(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, None, None,
-                                        ctypes.byref(p), FAKE, FAKE2, FAKE3, FAKE, 1 << 40,
+                                        ctypes.byref(p), FAKE4, FAKE2, FAKE3, FAKE, 1 << 40,
                                         None) == code
     assert _lib.lib().lkl_attn_forward_workspace_size(ctypes.byref(p), 1) == 0
     assert _lib.lib().lkl_attn_backward_workspace_size(ctypes.byref(p), 1) == 0
@@ -78,10 +78,13 @@ def test_attention_refuses_bad_pointers_strides_and_scratch():
 
     def bwd(dk=FAKE2, ws=FAKE, n=256, strides=None):
         return L.lkl_attn_backward(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, strides, None,
-                                   ctypes.byref(p), FAKE, dk, FAKE3, ws, n, None)
+                                   ctypes.byref(p), FAKE4, dk, FAKE3, ws, n, None)
     assert bwd() == 6
     assert bwd(dk=None) == 1
-    assert bwd(dk=FAKE, n=1 << 40) == 10
+    for other in (FAKE, FAKE3, FAKE4):      # an input, dv, dq
+        assert bwd(dk=other, n=1 << 40) == 10
+    assert L.lkl_attn_forward(FAKE, FAKE3, FAKE4, None, None, ctypes.byref(p), FAKE3, FAKE, None, 0,
+                              None) == 10
     s = [good] * 8
     s[6] = _lib.LKLStrides(b=300 * 512, h=0, t=512)
     assert bwd(n=1 << 40, strides=(_lib.LKLStrides * 8)(*s)) == 2
@@ -95,12 +98,12 @@ def test_logits_refuse_bad_rows(kw, code):
     L, r, ok = _lib.lib(), rows(**kw), rows()
     b, o = ctypes.byref(r), ctypes.byref(ok)
     assert L.lkl_token_logprobs(FAKE, b, FAKE, -100, 0, FAKE, FAKE, FAKE, None, None, None) == code
-    assert L.lkl_token_logprobs_backward(FAKE, b, FAKE, -100, FAKE, FAKE, FAKE, FAKE, FAKE,
+    assert L.lkl_token_logprobs_backward(FAKE, b, FAKE, -100, FAKE, FAKE, FAKE, FAKE, FAKE2,
                                          None) == code
     for x, y in ((b, o), (o, b)):
         assert L.lkl_logits_kl_forward(FAKE, x, FAKE, y, None, 0, 1.0, FAKE, FAKE, FAKE, FAKE,
                                        1 << 20, None) == code
-        assert L.lkl_logits_kl_backward(FAKE, x, FAKE, y, None, 0, 1.0, FAKE, FAKE, None, FAKE,
+        assert L.lkl_logits_kl_backward(FAKE, x, FAKE, y, None, 0, 1.0, FAKE, FAKE, None, FAKE2,
                                         None) == code
 
 
@@ -126,3 +129,20 @@ def test_logits_refuse_bad_arguments():
         assert kl(tau=tau) == 2
     assert kl(mask=FAKE, mdt=5) == 4 and kl(loss=None) == 1
     assert kl(n=L.lkl_logits_kl_workspace_size(b) - 1) == 6 and kl(ws=None) == 6
+    # a gradient does not overwrite the logits
+    assert L.lkl_token_logprobs_backward(FAKE, b, FAKE, -100, FAKE, FAKE, FAKE, FAKE, FAKE,
+                                         None) == 10
+    for x, y in ((FAKE, FAKE2), (FAKE2, FAKE)):
+        assert L.lkl_logits_kl_backward(x, b, y, b, None, 0, 1.0, FAKE, FAKE, None, FAKE, None) == 10
+
+
+def test_backward_scratch_of_a_group_beyond_8_gib():
+    """One kv head whose dS tiles exceed 8 GiB runs in chunks of key tiles: the
+    scratch asked for is 8 GiB of tiles and the fp32 dq of its query heads."""
+    L, p = _lib.lib(), prob(B=1, Hq=8, Hkv=1, T=40000)
+    n_t = (40000 + 127) // 128
+    need = L.lkl_attn_backward_workspace_size(ctypes.byref(p), 0)
+    stats, acc = 8 * n_t * 1024, 8 * 40000 * 128 * 4
+    assert 8 * n_t * (n_t + 1) // 2 * 32768 > 8 << 30
+    assert need >= stats + acc + (8 << 30)
+    assert need < stats + acc + (8 << 30) + (1 << 30)
