@@ -308,7 +308,8 @@ int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, cons
  *   S_ij = sm_scale q_i . k_j,  lse_i = log sum_j e^S_ij,
  *   P_ij = e^(S_ij - lse_i),    out_i = sum_j P_ij v_j.
  * The backward keeps no n x n map: it recomputes P from q, k and lse;
- *   delta_i = dout_i . out_i,  dS_ij = P_ij (dout_i . v_j - delta_i),
+ *   delta_i = dout_i . out_i (= sum_j P_ij dout_i . v_j, which is what
+ *   sequences of up to 128 tokens take),  dS_ij = P_ij (dout_i . v_j - delta_i),
  *   dq_i = sm_scale sum_j dS_ij k_j,  dk_j = sm_scale sum_i dS_ij q_i,
  *   dv_j = sum_i P_ij dout_i   (dk, dv: over the query heads of the kv head).
  * The mask is the [B, T] padding mask of the calls above: a token that it
@@ -319,10 +320,12 @@ int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, cons
  * All tensors are 16-bit of one type except lse (fp32 [B, Hq, T], contiguous).
  * `strides` gives the element strides (b, h, t) of every 16-bit tensor in the
  * order of its index below, each with a d stride of 1; NULL: all contiguous
- * [B, H, T, D].  Input strides may be any non-negative number (0 where a tensor is
- * broadcast), output strides are positive.  Head dims 8, 16, 32, 64 and 128 run on the tensor cores when
- * every pointer is 16-byte aligned and every stride a positive multiple of 8
- * elements; everything else runs on CUDA-core kernels.  lkl_last_path() tells which.
+ * [B, H, T, D].  Input strides may be any non-negative number (0 where a
+ * tensor is broadcast), output strides are positive.  Head dims 8, 16, 32, 64
+ * and 128 run on the tensor cores when every pointer is 16-byte aligned and
+ * every stride a positive multiple of 8 elements; everything else runs on
+ * CUDA-core kernels.  lkl_last_path() tells which.  An output may not start
+ * where an input does.
  * Sums and softmax statistics are fp32; P and dS are rounded to the tensors'
  * type before their products on the tensor cores (in fp16 a dS beyond 65504
  * overflows: scale the loss so that dout . v stays below).  Results are reproducible
@@ -345,12 +348,13 @@ enum lkl_attn_tensor {
 size_t lkl_attn_forward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);
 
 /* Bytes of scratch of the backward: the packed mask, 1 KB per (batch, head,
- * 128 rows) and, on the tensor cores, the 16-bit dS tiles that the key-stationary
- * launch hands to the dq launch: all of them up to 8 GiB, beyond that the
- * backward runs in chunks of kv heads or, where one kv head's query heads need
- * more, of key tiles; and, where one kv head's key tiles are few and long, fp32
- * sums of dk and dv for up to four thread blocks each.  Less also works, in more chunks, down to the dS tiles of
- * one key tile ((Hq / Hkv) * ceil(T / 128) tiles of 32 KB) and one kv head's dq in fp32; below that
+ * 128 rows) and, on the tensor cores, the 16-bit dS tiles that the
+ * key-stationary launch hands to the dq launch: all of them up to 8 GiB, beyond
+ * that the backward runs in chunks of kv heads or, where one kv head's query
+ * heads need more, of key tiles; and, where the key tiles are few and long,
+ * fp32 sums of dk and dv for up to four thread blocks each.  Less also works,
+ * in more chunks, down to the dS tiles of one key tile ((Hq / Hkv) *
+ * ceil(T / 128) tiles of 32 KB) and one kv head's dq in fp32; below that
  * LKL_ERR_WORKSPACE. */
 size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_mask);
 
@@ -390,9 +394,10 @@ int32_t lkl_token_logprobs(const void* logits, const lkl_logits* l, const int64_
                            int64_t ignore_index, int32_t top_k, float* logprob, float* entropy,
                            float* lse, float* top_logprobs, int64_t* top_indices, void* stream);
 
-/* May not write over the logits.  d_logits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy), g =
+/* d_logits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy), g =
  * d_logprob (0 for an ignored target, NaN for one outside [0, V)), h =
- * d_entropy; NULL means 0.  d_logits: contiguous [B, T, V] of the logits' type. */
+ * d_entropy; NULL means 0.  d_logits: contiguous [B, T, V] of the logits' type,
+ * not the logits themselves (LKL_ERR_BAD_ALIAS). */
 int32_t lkl_token_logprobs_backward(const void* logits, const lkl_logits* l,
                                     const int64_t* targets, int64_t ignore_index,
                                     const float* lse, const float* entropy,

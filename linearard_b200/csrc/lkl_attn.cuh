@@ -27,6 +27,13 @@ cudaError_t launch_attn_generic_forward(const AttnProblem& p, const AttnTensors&
 // rows[b, h, i] = (-lse log2(e), delta_i); (-inf, 0) for a row the mask removes.
 cudaError_t launch_attn_delta(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
                               float2* rows, cudaStream_t st);
+// The same from the probabilities instead of the rounded out, for sequences up to
+// kExactDeltaTokens: into `rows`, or where that is null into the tensor-core launch's
+// `stats`.
+constexpr int kExactDeltaTokens = 128;
+cudaError_t launch_attn_exact_delta(const AttnProblem& p, const AttnTensors& t,
+                                    const uint32_t* bits, float2* rows, float* stats,
+                                    cudaStream_t st);
 cudaError_t launch_attn_generic_backward(const AttnProblem& p, const AttnTensors& t,
                                          const uint32_t* bits, const float2* rows,
                                          cudaStream_t st);

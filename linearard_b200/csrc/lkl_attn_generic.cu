@@ -145,6 +145,57 @@ __global__ void attn_delta_kernel(const AttnProblem p, const AttnTensors a,
   }
 }
 
+// delta_i = sum_j P_ij (dout_i . v_j), which equals dout_i . out_i but for out's
+// rounding and that of P behind it.  dS_ij = P_ij (dP_ij - delta_i) is a small
+// difference where one key has most of a row, as in short sequences: with the rounded
+// out, dk of two tokens was off by 17% (bf16), and 1% at eight.  Sequences up to
+// kExactDeltaTokens pay for the second look at S and dP (one key tile of 128 at most);
+// beyond that rows of many keys carry the gradient and both ways end at 0.4%.
+template <int D>
+__global__ void __launch_bounds__(kAThreads)
+attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
+                        const uint32_t* __restrict__ bits, float2* __restrict__ rows,
+                        float* __restrict__ stats, int n_rt) {
+  extern __shared__ float smem[];
+  float* sQ = smem;
+  float* sG = sQ + kABM * (D + 1);
+  float* sK = sG + kABM * (D + 1);
+  float* sV = sK + kABM * (D + 1);
+  const int n_t = (p.T + kABM - 1) / kABM, words = (p.T + 31) >> 5;
+  const int bh = blockIdx.x / n_rt, mt = blockIdx.x % n_rt;   // n_rt: row tiles written
+  const int b = bh / p.Hq, h = bh % p.Hq, g = h / (p.Hq / p.Hkv);
+  const int r = threadIdx.x >> 3, sub = threadIdx.x & 7, i = mt * kABM + r;
+  const bool row = i < p.T && token_valid(bits, words, b, i);
+  const float z = row ? -a.lse[(size_t)bh * p.T + i] * kLog2e : -CUDART_INF_F;
+  attn_load_tile<D>(sQ, a.q, a.sq, b, h, mt * kABM, p.T, p.dtype, bits);
+  attn_load_tile<D>(sG, a.dout, a.sdo, b, h, mt * kABM, p.T, p.dtype, bits);
+  float delta = 0.f;
+  const int n_j = mt >= n_t ? 0 : p.causal ? mt + 1 : n_t;
+  for (int j = 0; j < n_j; ++j) {
+    __syncthreads();
+    attn_load_tile<D>(sK, a.k, a.sk, b, g, j * kABM, p.T, p.dtype, bits);
+    attn_load_tile<D>(sV, a.v, a.sv, b, g, j * kABM, p.T, p.dtype, bits);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int cl = sub + 8 * k, c = j * kABM + cl;
+      if (row && c < p.T && (!p.causal || c <= i) && token_valid(bits, words, b, c)) {
+        const float s = attn_dot<D>(sQ + r * (D + 1), sK + cl * (D + 1)) * p.sc * kLog2e;
+        delta = fmaf(exp2f(s + z), attn_dot<D>(sG + r * (D + 1), sV + cl * (D + 1)), delta);
+      }
+    }
+  }
+  delta = sum8(delta);
+  if (sub != 0) return;
+  if (rows) {
+    if (i < p.T) rows[(size_t)bh * p.T + i] = make_float2(z, delta);
+  } else {   // [head][128 rows][2][128]; rows past T up to the tile's end included
+    float* at = stats + (size_t)bh * ((p.T + 127) / 128) * 256 + (i >> 7) * 256 + (i & 127);
+    at[0] = z;
+    at[128] = delta;
+  }
+}
+
 // dq_i = sc sum_j P_ij (dout_i . v_j - delta_i) k_j; query rows are stationary.
 template <int D>
 __global__ void __launch_bounds__(kAThreads)
@@ -276,6 +327,15 @@ cudaError_t attn_generic_fwd(const AttnProblem& p, const AttnTensors& t, const u
 }
 
 template <int D>
+cudaError_t attn_exact_delta(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
+                             float2* rows, float* stats, cudaStream_t st) {
+  // the tensor-core launch reads whole tiles of 128 rows
+  const int n_rt = stats ? (p.T + 127) / 128 * 4 : (p.T + kABM - 1) / kABM;
+  return attn_launch(attn_exact_delta_kernel<D>, (long long)p.B * p.Hq * n_rt,
+                     4 * kABM * (D + 1) * 4, st, p, t, bits, rows, stats, n_rt);
+}
+
+template <int D>
 cudaError_t attn_generic_bwd(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
                              const float2* rows, cudaStream_t st) {
   const int n_t = (p.T + kABM - 1) / kABM;
@@ -297,6 +357,19 @@ cudaError_t launch_attn_generic_forward(const AttnProblem& p, const AttnTensors&
     case 64: return attn_generic_fwd<64>(p, t, bits, st);
     case 128: return attn_generic_fwd<128>(p, t, bits, st);
     default: return attn_generic_fwd<256>(p, t, bits, st);
+  }
+}
+
+cudaError_t launch_attn_exact_delta(const AttnProblem& p, const AttnTensors& t,
+                                    const uint32_t* bits, float2* rows, float* stats,
+                                    cudaStream_t st) {
+  switch (p.D) {
+    case 8: return attn_exact_delta<8>(p, t, bits, rows, stats, st);
+    case 16: return attn_exact_delta<16>(p, t, bits, rows, stats, st);
+    case 32: return attn_exact_delta<32>(p, t, bits, rows, stats, st);
+    case 64: return attn_exact_delta<64>(p, t, bits, rows, stats, st);
+    case 128: return attn_exact_delta<128>(p, t, bits, rows, stats, st);
+    default: return attn_exact_delta<256>(p, t, bits, rows, stats, st);
   }
 }
 

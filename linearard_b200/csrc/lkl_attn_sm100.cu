@@ -4,13 +4,21 @@
 // 128-key tiles from the diagonal down.  Per tile and key tile, two GEMMs
 // (S = Q K^T, O += P V) and one exponential per score.  At head dim 128 the
 // 16,384 exponentials of a tile take 1024 cycles of the SM's MUFU pipe and its
-// two GEMMs about 1024 cycles of the tensor pipe, so neither may wait: while
-// one tile's warpgroup computes P, the other tile's GEMMs run.
+// 16 MMA steps 1024 cycles of the tensor pipe at its peak, about 1370 as they run (S reads
+// 8 KB of shared memory a step, all that an SM delivers in 64 cycles), so neither may
+// wait: while one tile's warpgroup computes P, the other tile's GEMMs run.
+//
+// Measured at 32 / 8 heads x 8192 tokens, D 128, bf16, causal: 453 us, 1213 TFLOP/s, 73%
+// of the measured burst peak; two tiles x 128 keys take some 3300 cycles: softmax 1900,
+// own GEMMs 1370 behind it.  Tried and slower there: P through shared memory, so
+// that S is free early (384 KB of shared memory a period: 610 against 541 us then);
+// 64-key units with two score buffers a tile (766); an MMA thread a tile (679);
+// the maximum beside the exponentials of the tile before (540 against 530).
 //
 // Warps 0-3 / 4-7: softmax of tile 0 / 1, one row a thread, so a row's maximum
 // and sum need no exchange.  Warp 8: TMA producer.  Warp 9: MMA issuer and TMEM
 // owner.  Warp 10: with a padding mask, clears the rows of removed tokens in the
-// loaded tiles (P is 0 there, but 0 x NaN is not).
+// loaded V tiles (P is 0 there, but 0 x NaN is not).
 //
 // TMEM: S0, S1 (128 columns each; P, 16-bit, overwrites the first 64 of its S),
 // then O0, O1.  tcgen05.mma of one thread run in order, so S_t(j+1), issued
@@ -235,10 +243,12 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
         }
       }
     } else if (warp == kFaMma) {
-      // One thread issues both tiles' GEMMs, in turns: that keeps the tiles half a period
-      // apart, so that one's softmax runs under the other's GEMMs.  (A thread a tile lets
-      // them fall into step: 679 us instead of 541.)  The pipe waits for this thread, so
-      // the loop keeps ring positions and descriptors in registers.
+      // One warp issues both tiles' GEMMs, in turns: that keeps the tiles half a period
+      // apart, so that one's softmax runs under the other's GEMMs.  The tensor pipe waits
+      // for this warp, so it runs the loop as one: ring positions and descriptors are
+      // then the same in every lane and stay in the uniform registers that the MMA
+      // instructions read.  With the loop under `lane == 0` each MMA took 75 to 95 cycles to
+      // issue instead of 25 (8192 tokens: 500 us instead of 453).
       if (kt0 >= 0) {
         const uint32_t leader = elect_one();
         const uint32_t id_s = idesc_f16(kBM, kBN, BF16, BF16, 0, 0);
@@ -362,7 +372,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
       }
       tc_fence_after();
       // S(n) is complete, and with it all that was issued before: K(n) and V(n - 1) are
-      // free.  (Commits of their own in the MMA thread cost it 250 cycles each.)
+      // free, without commits of their own.
       if (lane == 0) {
         mbar_arrive(&misc->k_empty[(n + skip) % L::NK]);
         if (n > 0) mbar_arrive(&misc->v_empty[(n + skip - 1) % L::NV]);
@@ -512,14 +522,19 @@ cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const u
 // 16,384 exponentials.  Reducing dq in L2 instead would move 64 KB of fp32 a
 // pair, in an order that changes from run to run.
 //
-// Bound of the dkv launch: four GEMMs of 512 cycles a tile pair against 1024
-// cycles of exponentials.  The issue order dV(i), S(i+1), dK(i), dP(i+1) keeps the
-// tensor pipe busy: dS(i) is computed under dV(i) and S(i+1), P(i+1) under dK(i)
-// and dP(i+1).  All 512 TMEM columns are in use (S, dP, dV, dK at head dim 128;
-// P and dS overwrite the first half of what they come from).
+// Bound of the dkv launch: the tensor pipe, 32 MMA steps a tile pair (2048 cycles at the
+// peak, some 3000 as they run) against 1024 cycles of exponentials.  Measured at
+// 32 / 8 heads x 8192 tokens, D 128, causal: a pair every 3100 cycles, and as long without
+// any exponential, TMEM access or TMA load; 4211 when one lane issued and eight row
+// warps had 64 queries each.  The issue order dV(i), S(i+1), dK(i), dP(i+1) keeps the
+// pipe busy: dS(i) is computed under dV(i) and S(i+1), P(i+1) under dK(i) and dP(i+1).
+// All 512 TMEM columns are in use (S, dP, dV, dK at head dim 128; P and dS overwrite
+// part of what they come from).  The dq launch reads dS at the copy rate (286 us for
+// 1.84 GB at 8 heads x 15001).
 //
 // Sixteen row warps, 32 queries of 128 each (eight warps with 64 queries left the
-// exponentials of a tile at 1800 cycles for want of independent work).  P is handed over in two parts, so that half of dV's GEMM runs under its second part.
+// exponentials of a tile at 1800 cycles for want of independent work).  P is handed
+// over in two parts, so that half of dV's GEMM runs under its second part.
 constexpr int kFbRowWarps = 16;
 constexpr int kFbThreads = 640;
 constexpr int kFbProducer = 16, kFbMma = 17, kFbCleaner = 18, kFbStats = 19;
@@ -729,8 +744,8 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
               break;
             }
             mbar_arrive_expect_tx(&misc->full[s], L::TILE);
-            issue_tile_loads(smem + L::OFF_RING + s * L::TILE, o ? &tm_do : &tm_q, &misc->full[s], D,
-                             w.i * kBM, w.h, b);
+            issue_tile_loads(smem + L::OFF_RING + s * L::TILE, o ? &tm_do : &tm_q,
+                             &misc->full[s], D, w.i * kBM, w.h, b);
           }
       }
     } else if (warp == kFbStats) {
@@ -1348,8 +1363,13 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
       (e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
     return e;
   const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
-  attn_sm100_delta_kernel<<<p.B * p.Hq * n_t, 256, 0, st>>>(p, t, bits, stats);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (p.T <= kExactDeltaTokens) {
+    e = launch_attn_exact_delta(p, t, bits, nullptr, stats, st);
+  } else {
+    attn_sm100_delta_kernel<<<p.B * p.Hq * n_t, 256, 0, st>>>(p, t, bits, stats);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return e;
   const long long group_bytes = 4ll * G * p.T * p.D;   // queries and dO
   for (int g0 = 0; g0 < groups; g0 += plan.per)
     for (int j0 = 0; j0 < n_t; j0 += plan.keys) {
@@ -1368,7 +1388,8 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
           mq, mk, mv, mdo, mdk, mdv, p, c, bits, stats, dsbuf, sums);
       if ((e = cudaGetLastError()) != cudaSuccess) return e;
       if (parts > 1) {
-        const long long n = 2ll * (c.g1 - c.g0) * (std::min(p.T, c.j1 * kBN) - j0 * kBN) * (p.D / 8);
+        const int rows = std::min(p.T, c.j1 * kBN) - j0 * kBN;
+        const long long n = 2ll * (c.g1 - c.g0) * rows * (p.D / 8);
         attn_sm100_sum_parts_kernel<BF16><<<(int)std::min<long long>((n + 255) / 256, 4 * kFbSms),
                                             256, 0, st>>>(p, t, c, sums);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;

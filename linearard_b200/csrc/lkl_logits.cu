@@ -7,9 +7,16 @@
 // running maximum m and sums relative to it,
 //   l = sum e^(x - m),  a = sum e^(x - m) (x - m)     (token: entropy = log l - a / l)
 //   A = sum e^(t - m_t) (t - s)                       (KL = A / l_t - (lse_t - lse_s)),
-// over batches of four 16-byte loads, and join threads, warps and blocks in a
-// fixed order.  Differences from m are taken before they are scaled: the
-// exponent of a likely token keeps all its bits, whatever the logits' offset.
+// over batches of 16-byte loads, and join threads, warps and blocks in a fixed
+// order: the maxima first, so that each thread rescales once.  Differences from m are
+// taken before they are scaled: the exponent of a likely token keeps all its bits,
+// whatever the logits' offset.
+//
+// Measured (of 6561 GB/s, the copy rate): KL backward 6.5 TB/s; KL forward 5.4 TB/s at
+// 16384 x 32000 bf16, token forward 5.3, backward 5.5 TB/s.  Blocks of 128 threads
+// let ten rows of an SM overlap their ends (256 threads and pairwise joins: 4.0 and
+// 3.8 TB/s); packed fp32 pairs and 16-bit maxima keep an element at about five
+// instructions, which with the exponential is what is left between 5.4 and 6.5 TB/s.
 //
 // A row belongs to a cluster of 1, 2, 4 or 8 blocks that join their sums
 // through distributed shared memory, so that few rows still fill the GPU and
@@ -498,8 +505,8 @@ __device__ __forceinline__ void join_lists(TopList& top, TopShared& ts) {
 // it and collects what reaches it.  Rows with more such elements than `cand` holds
 // (equal logits) take the pass that keeps a sorted list a warp.
 constexpr int kTopCand = 256;
-struct TopShared2 {
-  float mine[kLThreads];
+struct TopLook {
+  alignas(16) float mine[kLThreads];   // read four at a time
   float bound;
   int count;
   uint64_t cand[kTopCand];
@@ -507,7 +514,7 @@ struct TopShared2 {
 
 template <typename T>
 __device__ __forceinline__ TopList top_pass(const T* row, long long V, int top_k, float mine,
-                                            TopShared& ts, TopShared2& tc) {
+                                            TopShared& ts, TopLook& tc) {
   constexpr int N = Elem<T>::N, U = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (isnan(mine)) mine = -CUDART_INF_F;
@@ -588,7 +595,7 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
                       int64_t* __restrict__ top_i) {
   __shared__ Joint joint;
   __shared__ TopShared ts;
-  __shared__ TopShared2 tc;
+  __shared__ TopLook tc;
   cg::cluster_group cluster = cg::this_cluster();
   const int n = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const long long row = blockIdx.x / n;
@@ -623,7 +630,8 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
       cluster.sync();
     }
     if (rank == 0 && warp == 0) {
-      for (int r = 1; r < n; ++r) top.merge(cluster.map_shared_rank(&ts.lists[0][0], r)[lane], lane);
+      for (int r = 1; r < n; ++r)
+        top.merge(cluster.map_shared_rank(&ts.lists[0][0], r)[lane], lane);
       if (lane < top_k) {
         const long long idx = (uint32_t)~(uint32_t)top.key;
         top_v[row * top_k + lane] =
@@ -656,7 +664,8 @@ __device__ __forceinline__ KLStat kl_pass(const T* s, const T* t, long long V, f
       to[1] = max_nan(to[1], Elem<T>::top(y[u]));
     }
     if (!(to[0] == st.m[0] && to[1] == st.m[1])) st.move(to, c);
-    const float ms = to[0] == -CUDART_INF_F ? 0.f : to[0], mt = to[1] == -CUDART_INF_F ? 0.f : to[1];
+    const float ms = to[0] == -CUDART_INF_F ? 0.f : to[0];
+    const float mt = to[1] == -CUDART_INF_F ? 0.f : to[1];
     const uint64_t ms2 = f2pack(ms, ms), mt2 = f2pack(mt, mt);
     uint64_t ls = 0, lt = 0, a = 0;
 #pragma unroll
@@ -929,8 +938,8 @@ cudaError_t launch_token_logprobs_backward(const LogitsView& x, long long rows,
   return with_type(x.dtype, [&](auto t) {
     using T = decltype(t);
     const int shares = shares_of<T>(x.V);
-    return launch_rows(token_logprobs_backward_kernel<T>, kGThreadsL, rows * shares, 1, st, x, targets, ignore,
-                       lse, entropy, g_lp, g_en, static_cast<T*>(dx), shares);
+    return launch_rows(token_logprobs_backward_kernel<T>, kGThreadsL, rows * shares, 1, st, x,
+                       targets, ignore, lse, entropy, g_lp, g_en, static_cast<T*>(dx), shares);
   });
 }
 
@@ -939,8 +948,8 @@ cudaError_t launch_logits_kl_forward(const LogitsView& s, const LogitsView& t, l
                                      float* lse_t, float* row_kl, float* loss, cudaStream_t st) {
   const int n = cluster_of(rows, s.V);
   const cudaError_t e = with_type(s.dtype, [&](auto x) {
-    return launch_rows(logits_kl_forward_kernel<decltype(x)>, kLThreads, rows, n, st, s, t, mask, mdt, inv_tau,
-                       lse_s, lse_t, row_kl);
+    return launch_rows(logits_kl_forward_kernel<decltype(x)>, kLThreads, rows, n, st, s, t, mask,
+                       mdt, inv_tau, lse_s, lse_t, row_kl);
   });
   return e != cudaSuccess ? e : launch_reduce_partials(row_kl, (int)rows, loss, st);
 }
@@ -952,8 +961,8 @@ cudaError_t launch_logits_kl_backward(const LogitsView& s, const LogitsView& t, 
   return with_type(s.dtype, [&](auto x) {
     using T = decltype(x);
     const int shares = shares_of<T>(s.V);
-    return launch_rows(logits_kl_backward_kernel<T>, kGThreadsL, rows * shares, 1, st, s, t, mask, mdt, inv_tau,
-                       lse_s, lse_t, dloss, static_cast<T*>(ds), shares);
+    return launch_rows(logits_kl_backward_kernel<T>, kGThreadsL, rows * shares, 1, st, s, t, mask,
+                       mdt, inv_tau, lse_s, lse_t, dloss, static_cast<T*>(ds), shares);
   });
 }
 

@@ -379,3 +379,32 @@ def test_refusals():
     for bad in ((g.float(), out, lse), (g, out[:, :2], lse), (g, out, lse.half()), (g, out, lse[:, :2])):
         with pytest.raises(AssertionError):
             attn_backward(bad[0], q, k, v, *bad[1:])
+
+
+@pytest.mark.parametrize("D", [16, 128, 256])
+@pytest.mark.parametrize("T", [2, 3, 5, 8, 33, 128])
+def test_short_sequences_keep_small_gradients(T, D):
+    """Where one key has most of a row, dS is a small difference of dout . v and
+    delta: short sequences take delta from the probabilities, so that what is left are
+    the roundings of dS and of the results, u each and relative to their size."""
+    q, k, v, g = make(2, 4, 4, T, D, "bf16", seed=T, scale=2.2)
+    ref = AttnRef(q, k, v, None, True, None, g)
+    out, lse = attn_forward(q, k, v)
+    dq, dk, _ = attn_backward(g, q, k, v, out, lse)
+    u = 2.0 ** -8
+    kk, qq, gg, vv = (t.double() for t in (k, q, g, v))
+    S = (qq @ kk.transpose(-1, -2)) * D ** -0.5
+    keep = torch.ones(T, T, dtype=torch.bool, device="cuda").tril()
+    P = S.masked_fill(~keep, -torch.inf).softmax(-1)
+    dP = gg @ vv.transpose(-1, -2)
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+    # fp32: the sums behind S, dP and delta, on terms of size P |dout||v|
+    c = (2 * D + 64) * 2.0 ** -24
+    mag = gg.abs() @ vv.abs().transpose(-1, -2)
+    size = (qq.abs() @ kk.abs().transpose(-1, -2)) * D ** -0.5
+    top = torch.where(keep, size, 0.0).amax(-1, keepdim=True)
+    tol = torch.where(keep, u * dS.abs() + P * (mag + (P * mag).sum(-1, keepdim=True))
+                      * (c * (2 + 2 * top) + 2.0 ** -18), 0.0) + 2.0 ** -126
+    assert_within(dq, ref.dq, D ** -0.5 * tol @ kk.abs() * (1 + u) + u * ref.dq.abs() + 1e-30, "dq")
+    assert_within(dk, ref.dk, D ** -0.5 * tol.transpose(-1, -2) @ qq.abs() * (1 + u)
+                  + u * ref.dk.abs() + 1e-30, "dk")
