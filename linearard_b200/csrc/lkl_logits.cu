@@ -12,11 +12,10 @@
 // taken before they are scaled: the exponent of a likely token keeps all its bits,
 // whatever the logits' offset.
 //
-// Measured (of 6561 GB/s, the copy rate): KL backward 6.5 TB/s; KL forward 5.4 TB/s at
-// 16384 x 32000 bf16, token forward 5.3, backward 5.5 TB/s.  Blocks of 128 threads
-// let ten rows of an SM overlap their ends (256 threads and pairwise joins: 4.0 and
-// 3.8 TB/s); packed fp32 pairs and 16-bit maxima keep an element at about five
-// instructions, which with the exponential is what is left between 5.4 and 6.5 TB/s.
+// Measured at 16384 x 32000 bf16 (of 6561 GB/s, the copy rate): KL backward 6.5 TB/s, forward
+// 6.1; token forward 5.9, backward 5.5 TB/s.  Blocks of 128 threads let ten rows of an SM
+// overlap their ends, and 128 bytes in flight a thread fill HBM (64 bytes: 5.4 and 5.3;
+// 256 threads and pairwise joins: 4.0 and 3.8; 64 threads: 3.8 and 3.7).
 //
 // A row belongs to a cluster of 1, 2, 4 or 8 blocks that join their sums
 // through distributed shared memory, so that few rows still fill the GPU and
@@ -337,10 +336,12 @@ struct TopShared {
 // TOP: an element can be among the best k only if it reaches the k-th best of any
 // warp, and also the least of the warps' (k / warps)-th best.  Few elements do after
 // the first batch; a batch's maximum, known for the sums, rules most batches out.
-template <typename T, bool GUARD, bool TOP>
+// U: 16-byte loads in flight a thread.
+template <typename T, bool GUARD, bool TOP, int U>
 __device__ __forceinline__ TokenStat token_pass(const T* row, long long V, int top_k, TopList& top,
                                                 TopShared& ts) {
-  constexpr int N = Elem<T>::N, U = 4, E = U * N;
+  constexpr int N = Elem<T>::N, E = U * N;
+  static_assert(!TOP || E <= 32, "a lane's elements fit a warp");
   const RowCut<T> cut(row, V);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), n_blocks = (int)cluster.num_blocks();
@@ -579,7 +580,7 @@ __device__ __forceinline__ TopList top_pass(const T* row, long long V, int top_k
   }
   if (lane == 0) ts.kth[warp] = ts.part[warp] = -CUDART_INF_F;
   __syncthreads();
-  token_pass<T, false, true>(row, V, top_k, top, ts);
+  token_pass<T, false, true, 4>(row, V, top_k, top, ts);
   join_lists(top, ts);
   return top;
 }
@@ -606,11 +607,13 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
     if (lane == 0) ts.kth[warp] = ts.part[warp] = -CUDART_INF_F;
     __syncthreads();
   }
-  TokenStat s = token_pass<T, false, MODE == kTopList>(x, view.V, top_k, top, ts);
+  // alone, 8 loads: 196 -> 177 us at 16384 x 32000 bf16; with alternatives, 4: 347, 8: 400
+  constexpr int U = MODE == kTopNone ? 8 : 4;
+  TokenStat s = token_pass<T, false, MODE == kTopList, U>(x, view.V, top_k, top, ts);
   const float mine = s.m[0];
   s = join_all(s, joint, kLog2e);
   if (isnan(s.sum[1]) && s.sum[0] > 0.f)   // the same in every thread of the cluster
-    s = join_all(token_pass<T, true, false>(x, view.V, 0, none, ts), joint, kLog2e);
+    s = join_all(token_pass<T, true, false, U>(x, view.V, 0, none, ts), joint, kLog2e);
   const bool empty = s.m[0] == -CUDART_INF_F;
   const float log_l = empty ? CUDART_NAN_F : logf(s.sum[0]);
   if (rank == 0 && threadIdx.x == 0) {
@@ -647,7 +650,7 @@ token_logprobs_kernel(const LogitsView view, const int64_t* __restrict__ targets
 template <typename T, bool GUARD>
 __device__ __forceinline__ KLStat kl_pass(const T* s, const T* t, long long V, float c) {
   constexpr int N = Elem<T>::N;
-  constexpr int U = 2;   // loads in flight a thread and stream
+  constexpr int U = 4;   // loads in flight a thread and stream
   const RowCut<T> cut(s, V);
   const bool vec = same_offset(s, t);
   cg::cluster_group cluster = cg::this_cluster();
