@@ -13,7 +13,10 @@
 // own GEMMs 1370 behind it.  Tried and slower there: P through shared memory, so
 // that S is free early (384 KB of shared memory a period: 610 against 541 us then);
 // 64-key units with two score buffers a tile (766); an MMA thread a tile (679);
-// the maximum beside the exponentials of the tile before (540 against 530).
+// the maximum beside the exponentials (540 against 530).  Head dims up to 64 leave 128 TMEM
+// columns free; P (and the backward's P and dS) in columns of their own, so that the next
+// scores need not wait, gained nothing there (16 heads x 8192, D 64: forward 212
+// either way, backward 585 against 630 us).
 //
 // Warps 0-3 / 4-7: softmax of tile 0 / 1, one row a thread, so a row's maximum
 // and sum need no exchange.  Warp 8: TMA producer.  Warp 9: MMA issuer and TMEM
