@@ -308,8 +308,8 @@ int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, cons
  *   S_ij = sm_scale q_i . k_j,  lse_i = log sum_j e^S_ij,
  *   P_ij = e^(S_ij - lse_i),    out_i = sum_j P_ij v_j.
  * The backward keeps no n x n map: it recomputes P from q, k and lse;
- *   delta_i = dout_i . out_i (= sum_j P_ij dout_i . v_j, which is what
- *   sequences of up to 128 tokens take),  dS_ij = P_ij (dout_i . v_j - delta_i),
+ *   delta_i = dout_i . out_i (= sum_j P_ij dout_i . v_j, which is what rows that
+ *   see at most 256 keys take),  dS_ij = P_ij (dout_i . v_j - delta_i),
  *   dq_i = sm_scale sum_j dS_ij k_j,  dk_j = sm_scale sum_i dS_ij q_i,
  *   dv_j = sum_i P_ij dout_i   (dk, dv: over the query heads of the kv head).
  * The mask is the [B, T] padding mask of the calls above: a token that it

@@ -27,13 +27,17 @@ cudaError_t launch_attn_generic_forward(const AttnProblem& p, const AttnTensors&
 // rows[b, h, i] = (-lse log2(e), delta_i); (-inf, 0) for a row the mask removes.
 cudaError_t launch_attn_delta(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
                               float2* rows, cudaStream_t st);
-// The same from the probabilities instead of the rounded out, for sequences up to
-// kExactDeltaTokens: into `rows`, or where that is null into the tensor-core launch's
-// `stats`.
-constexpr int kExactDeltaTokens = 128;
+// delta_i = sum_j P_ij (dout_i . v_j) equals dout_i . out_i but for out's rounding and that
+// of P behind it.  dS_ij = P_ij (dP_ij - delta_i) is a small difference where one key has
+// most of a row, as in rows of few keys: with the rounded out, dk of two tokens was off by
+// 17% (bf16), and 1% at eight.  Rows that see at most this many keys (in a causal sequence
+// of any length, its first) therefore take the sum; beyond it rows of many keys carry the
+// gradient and the two ways differ by less than the roundings of dS and of the result
+// (dq of 4096 tokens: 0.0025 of its size against 0.0024).
+constexpr int kExactDeltaKeys = 256;
+// The same into rows[] by that sum, for the rows below kExactDeltaKeys.
 cudaError_t launch_attn_exact_delta(const AttnProblem& p, const AttnTensors& t,
-                                    const uint32_t* bits, float2* rows, float* stats,
-                                    cudaStream_t st);
+                                    const uint32_t* bits, float2* rows, cudaStream_t st);
 cudaError_t launch_attn_generic_backward(const AttnProblem& p, const AttnTensors& t,
                                          const uint32_t* bits, const float2* rows,
                                          cudaStream_t st);

@@ -145,24 +145,19 @@ __global__ void attn_delta_kernel(const AttnProblem p, const AttnTensors a,
   }
 }
 
-// delta_i = sum_j P_ij (dout_i . v_j), which equals dout_i . out_i but for out's
-// rounding and that of P behind it.  dS_ij = P_ij (dP_ij - delta_i) is a small
-// difference where one key has most of a row, as in short sequences: with the rounded
-// out, dk of two tokens was off by 17% (bf16), and 1% at eight.  Sequences up to
-// kExactDeltaTokens pay for the second look at S and dP (one key tile of 128 at most);
-// beyond that rows of many keys carry the gradient and both ways end at 0.4%.
+// delta_i = sum_j P_ij (dout_i . v_j) for rows that see few keys; a block takes 32.
 template <int D>
 __global__ void __launch_bounds__(kAThreads)
 attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
                         const uint32_t* __restrict__ bits, float2* __restrict__ rows,
-                        float* __restrict__ stats, int n_rt) {
+                        int n_rt) {
   extern __shared__ float smem[];
   float* sQ = smem;
   float* sG = sQ + kABM * (D + 1);
   float* sK = sG + kABM * (D + 1);
   float* sV = sK + kABM * (D + 1);
   const int n_t = (p.T + kABM - 1) / kABM, words = (p.T + 31) >> 5;
-  const int bh = blockIdx.x / n_rt, mt = blockIdx.x % n_rt;   // n_rt: row tiles written
+  const int bh = blockIdx.x / n_rt, mt = blockIdx.x % n_rt;   // n_rt: row tiles to take
   const int b = bh / p.Hq, h = bh % p.Hq, g = h / (p.Hq / p.Hkv);
   const int r = threadIdx.x >> 3, sub = threadIdx.x & 7, i = mt * kABM + r;
   const bool row = i < p.T && token_valid(bits, words, b, i);
@@ -170,7 +165,7 @@ attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
   attn_load_tile<D>(sQ, a.q, a.sq, b, h, mt * kABM, p.T, p.dtype, bits);
   attn_load_tile<D>(sG, a.dout, a.sdo, b, h, mt * kABM, p.T, p.dtype, bits);
   float delta = 0.f;
-  const int n_j = mt >= n_t ? 0 : p.causal ? mt + 1 : n_t;
+  const int n_j = p.causal ? mt + 1 : n_t;
   for (int j = 0; j < n_j; ++j) {
     __syncthreads();
     attn_load_tile<D>(sK, a.k, a.sk, b, g, j * kABM, p.T, p.dtype, bits);
@@ -186,14 +181,7 @@ attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
     }
   }
   delta = sum8(delta);
-  if (sub != 0) return;
-  if (rows) {
-    if (i < p.T) rows[(size_t)bh * p.T + i] = make_float2(z, delta);
-  } else {   // [head][128 rows][2][128]; rows past T up to the tile's end included
-    float* at = stats + (size_t)bh * ((p.T + 127) / 128) * 256 + (i >> 7) * 256 + (i & 127);
-    at[0] = z;
-    at[128] = delta;
-  }
+  if (sub == 0 && i < p.T) rows[(size_t)bh * p.T + i] = make_float2(z, delta);
 }
 
 // dq_i = sc sum_j P_ij (dout_i . v_j - delta_i) k_j; query rows are stationary.
@@ -328,11 +316,10 @@ cudaError_t attn_generic_fwd(const AttnProblem& p, const AttnTensors& t, const u
 
 template <int D>
 cudaError_t attn_exact_delta(const AttnProblem& p, const AttnTensors& t, const uint32_t* bits,
-                             float2* rows, float* stats, cudaStream_t st) {
-  // the tensor-core launch reads whole tiles of 128 rows
-  const int n_rt = stats ? (p.T + 127) / 128 * 4 : (p.T + kABM - 1) / kABM;
+                             float2* rows, cudaStream_t st) {
+  const int n = p.T < kExactDeltaKeys ? p.T : kExactDeltaKeys, n_rt = (n + kABM - 1) / kABM;
   return attn_launch(attn_exact_delta_kernel<D>, (long long)p.B * p.Hq * n_rt,
-                     4 * kABM * (D + 1) * 4, st, p, t, bits, rows, stats, n_rt);
+                     4 * kABM * (D + 1) * 4, st, p, t, bits, rows, n_rt);
 }
 
 template <int D>
@@ -361,15 +348,14 @@ cudaError_t launch_attn_generic_forward(const AttnProblem& p, const AttnTensors&
 }
 
 cudaError_t launch_attn_exact_delta(const AttnProblem& p, const AttnTensors& t,
-                                    const uint32_t* bits, float2* rows, float* stats,
-                                    cudaStream_t st) {
+                                    const uint32_t* bits, float2* rows, cudaStream_t st) {
   switch (p.D) {
-    case 8: return attn_exact_delta<8>(p, t, bits, rows, stats, st);
-    case 16: return attn_exact_delta<16>(p, t, bits, rows, stats, st);
-    case 32: return attn_exact_delta<32>(p, t, bits, rows, stats, st);
-    case 64: return attn_exact_delta<64>(p, t, bits, rows, stats, st);
-    case 128: return attn_exact_delta<128>(p, t, bits, rows, stats, st);
-    default: return attn_exact_delta<256>(p, t, bits, rows, stats, st);
+    case 8: return attn_exact_delta<8>(p, t, bits, rows, st);
+    case 16: return attn_exact_delta<16>(p, t, bits, rows, st);
+    case 32: return attn_exact_delta<32>(p, t, bits, rows, st);
+    case 64: return attn_exact_delta<64>(p, t, bits, rows, st);
+    case 128: return attn_exact_delta<128>(p, t, bits, rows, st);
+    default: return attn_exact_delta<256>(p, t, bits, rows, st);
   }
 }
 

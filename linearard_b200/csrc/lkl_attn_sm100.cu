@@ -27,6 +27,11 @@
 // then O0, O1.  tcgen05.mma of one thread run in order, so S_t(j+1), issued
 // after O_t += P_t(j) V(j), may overwrite P_t(j), and its commit also says that
 // O_t is complete up to j.
+//
+// Roundings: scores, statistics and every sum are fp32 (products of 16-bit inputs are
+// exact in it).  P is rounded to the inputs' type because the second GEMM takes 16-bit
+// operands; the row sum adds the unrounded P.  That error and the output's own rounding
+// are alike in size: 0.0022 of the output in bf16, 0.0016 with the latter alone.
 #include <math_constants.h>
 
 #include "lkl_attn.cuh"
@@ -535,6 +540,12 @@ cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const u
 // part of what they come from).  The dq launch reads dS at the copy rate (286 us for
 // 1.84 GB at 8 heads x 15001).
 //
+// Roundings: P and dS are rounded to the inputs' type, the only one that the GEMMs take,
+// and dS is handed over as rounded, which halves the dq launch's bytes.  The gradients
+// carry that error beside their result's own: 0.0024 of their size in bf16 instead of
+// 0.0017, 0.0003 instead of 0.0002 in fp16.  dS as a sum of two 16-bit values would
+// take that back for a third more MMA steps and twice the hand-over.
+//
 // Sixteen row warps, 32 queries of 128 each (eight warps with 64 queries left the
 // exponentials of a tile at 1800 cycles for want of independent work).  P is handed
 // over in two parts, so that half of dV's GEMM runs under its second part.
@@ -564,36 +575,173 @@ __host__ __device__ __forceinline__ long long fb_tile(const FbChunk& c, int caus
 
 // Query rows' statistics as the dkv launch reads them: per (head, query tile)
 // 128 exponent offsets -lse log2(e) (-inf for a row without gradient), then
-// 128 delta_i = dout_i . out_i.
+// 128 delta_i.
 constexpr int kFbStatBytes = 2 * kBM * 4;
 
-// A block takes one tile of 128 rows; D / 8 neighbouring lanes share a row.
+// c += A B for 16 rows x 16 x 8 columns, fp32 sums of 16-bit products.
+template <bool BF16>
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The 16-bit values 32 c + 8 (lane % 4) .. + 7 of a row of p.D, zeros past its end, for
+// c < NC.  A contraction may take its terms in any order, as long as both operands take
+// the same: words 0 and 1 are one step of 16, words 2 and 3 the next.
+template <int NC>
+__device__ __forceinline__ void load_fragment_row(uint4 (&x)[NC], const void* base, size_t at,
+                                                  bool on, int D) {
+  const int e = (threadIdx.x & 3) * 8;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    x[c] = on && 32 * c + e < D
+               ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at + 32 * c + e)
+               : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// delta_i = sum_j P_ij (dout_i . v_j) for 16 rows from `first` on, straight from global
+// memory: a head's few keys come from L1 and L2, and 256 x 256 x D products a head are too
+// few for staging tiles and TMEM to pay.  The eight warps take 8 keys each in turn, at
+// most four times, and are joined in their order.  Bound by the latency of those
+// steps: 11.8 us for the 256 rows of 32 heads, D 128.
+template <int D, bool BF16>
+__device__ __forceinline__ void exact_delta_rows(const AttnProblem& p, const AttnTensors& a,
+                                                 const uint32_t* bits, int b, int h, int first,
+                                                 float* dst) {
+  constexpr int NC = D / 32;
+  __shared__ float part[8][16];
+  const int words = (p.T + 31) >> 5, lane = threadIdx.x & 31, quad = lane >> 2;
+  const int warp = threadIdx.x >> 5, i0 = first + quad, i1 = i0 + 8;
+  const bool on0 = i0 < p.T && token_valid(bits, words, b, i0);
+  const bool on1 = i1 < p.T && token_valid(bits, words, b, i1);
+  const float* lse = a.lse + ((size_t)b * p.Hq + h) * p.T;
+  const float z0 = on0 ? -lse[i0] * kLog2e : -CUDART_INF_F;
+  const float z1 = on1 ? -lse[i1] * kLog2e : -CUDART_INF_F;
+  const size_t q = (size_t)b * a.sq.b + (size_t)h * a.sq.h;
+  const size_t g = (size_t)b * a.sdo.b + (size_t)h * a.sdo.h;
+  uint4 q0[NC], q1[NC], g0[NC], g1[NC];
+  load_fragment_row(q0, a.q, q + (size_t)i0 * a.sq.t, on0, p.D);
+  load_fragment_row(q1, a.q, q + (size_t)i1 * a.sq.t, on1, p.D);
+  load_fragment_row(g0, a.dout, g + (size_t)i0 * a.sdo.t, on0, p.D);
+  load_fragment_row(g1, a.dout, g + (size_t)i1 * a.sdo.t, on1, p.D);
+  const int kv = h / (p.Hq / p.Hkv);
+  const size_t kb = (size_t)b * a.sk.b + (size_t)kv * a.sk.h;
+  const size_t vb = (size_t)b * a.sv.b + (size_t)kv * a.sv.h;
+  const int keys = first >= p.T ? 0 : p.causal ? min(p.T, first + 16) : p.T;
+  const float sl = p.sc * kLog2e;
+  float d0 = 0.f, d1 = 0.f;
+  for (int j = warp * 8; j < keys; j += 64) {
+    const int row = j + quad;
+    uint4 k[NC], v[NC];
+    load_fragment_row(k, a.k, kb + (size_t)row * a.sk.t, row < p.T, p.D);
+    load_fragment_row(v, a.v, vb + (size_t)row * a.sv.t, row < p.T, p.D);
+    float s[4] = {}, x[4] = {};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      mma_16x8x16<BF16>(s, q0[c].x, q1[c].x, q0[c].y, q1[c].y, k[c].x, k[c].y);
+      mma_16x8x16<BF16>(s, q0[c].z, q1[c].z, q0[c].w, q1[c].w, k[c].z, k[c].w);
+      mma_16x8x16<BF16>(x, g0[c].x, g1[c].x, g0[c].y, g1[c].y, v[c].x, v[c].y);
+      mma_16x8x16<BF16>(x, g0[c].z, g1[c].z, g0[c].w, g1[c].w, v[c].z, v[c].w);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = j + 2 * (lane & 3) + e;
+      if (col < p.T && token_valid(bits, words, b, col)) {
+        if (on0 && (!p.causal || col <= i0)) d0 = fmaf(exp2f(fmaf(s[e], sl, z0)), x[e], d0);
+        if (on1 && (!p.causal || col <= i1)) d1 = fmaf(exp2f(fmaf(s[e + 2], sl, z1)), x[e + 2], d1);
+      }
+    }
+  }
+  for (int o = 1; o < 4; o <<= 1) {
+    d0 += __shfl_xor_sync(0xffffffffu, d0, o);
+    d1 += __shfl_xor_sync(0xffffffffu, d1, o);
+  }
+  if ((lane & 3) == 0) {
+    part[warp][quad] = d0;
+    part[warp][quad + 8] = d1;
+    if (warp == 0) {
+      dst[quad] = z0;
+      dst[quad + 8] = z1;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float d = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) d += part[w][threadIdx.x];
+    dst[kBM + threadIdx.x] = d;
+  }
+}
+
+// Query tiles that see at most kExactDeltaKeys keys, the first of a head
+__host__ __device__ __forceinline__ int exact_delta_tiles(const AttnProblem& p) {
+  const int n_t = (p.T + kBM - 1) / kBM;
+  return p.T <= kExactDeltaKeys ? n_t : p.causal ? kExactDeltaKeys / kBM : 0;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256, 2)
+attn_sm100_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
+                              const uint32_t* __restrict__ bits, float* __restrict__ stats) {
+  const int n_t = (p.T + kBM - 1) / kBM, units = exact_delta_tiles(p) * (kBM / 16);
+  const int bh = blockIdx.x / units, first = blockIdx.x % units * 16;
+  exact_delta_rows<D, BF16>(p, a, bits, bh / p.Hq, bh % p.Hq, first,
+                            stats + ((size_t)bh * n_t + first / kBM) * 2 * kBM + first % kBM);
+}
+
+// The other tiles, one a block: delta_i = dout_i . out_i, D / 8 neighbouring lanes a row.
+// Bound by HBM: 64 MB of 32 heads x 4096, D 128 in 14.1 us (4.7 TB/s; 17.5 with one row's
+// loads at a time).  A launch of its own, since the 126 registers of the above leave too
+// few warps to read with: both in one launch took 34 us there.
 __global__ void __launch_bounds__(256)
 attn_sm100_delta_kernel(const AttnProblem p, const AttnTensors a,
                         const uint32_t* __restrict__ bits, float* __restrict__ stats) {
-  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5;
-  const int bh = blockIdx.x / n_t, qt = blockIdx.x % n_t, b = bh / p.Hq, h = bh % p.Hq;
-  const int lanes = p.D / 8, sub = threadIdx.x % lanes;
-  float* dst = stats + (size_t)blockIdx.x * 2 * kBM;
-  for (int r = threadIdx.x / lanes; r < kBM; r += 256 / lanes) {
-    const int i = qt * kBM + r;
-    const bool on = i < p.T && token_valid(bits, words, b, i);
-    float s = 0.f;
-    if (on) {
-      const uint4 x = *reinterpret_cast<const uint4*>(
-          static_cast<const uint16_t*>(a.out) + (size_t)b * a.so.b + (size_t)h * a.so.h +
-          (size_t)i * a.so.t + sub * 8);
-      const uint4 y = *reinterpret_cast<const uint4*>(
-          static_cast<const uint16_t*>(a.dout) + (size_t)b * a.sdo.b + (size_t)h * a.sdo.h +
-          (size_t)i * a.sdo.t + sub * 8);
+  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5, few = exact_delta_tiles(p);
+  const int bh = blockIdx.x / (n_t - few), qt = few + blockIdx.x % (n_t - few);
+  const int b = bh / p.Hq, h = bh % p.Hq, lanes = p.D / 8, sub = threadIdx.x % lanes;
+  float* dst = stats + ((size_t)bh * n_t + qt) * 2 * kBM;
+  const uint16_t* out = static_cast<const uint16_t*>(a.out) + (size_t)b * a.so.b +
+                        (size_t)h * a.so.h + sub * 8;
+  const uint16_t* dout = static_cast<const uint16_t*>(a.dout) + (size_t)b * a.sdo.b +
+                         (size_t)h * a.sdo.h + sub * 8;
+  // four rows at a time, all loads before the first use
+  for (int r0 = threadIdx.x / lanes; r0 < kBM; r0 += 4 * (256 / lanes)) {
+    uint4 x[4], y[4];
+    float z[4];
+    bool on[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + k * (256 / lanes), i = qt * kBM + r;
+      on[k] = r < kBM && i < p.T && token_valid(bits, words, b, i);
+      x[k] = y[k] = make_uint4(0u, 0u, 0u, 0u);
+      z[k] = CUDART_INF_F;
+      if (on[k]) {
+        x[k] = *reinterpret_cast<const uint4*>(out + (size_t)i * a.so.t);
+        y[k] = *reinterpret_cast<const uint4*>(dout + (size_t)i * a.sdo.t);
+        if (sub == 0) z[k] = a.lse[(size_t)bh * p.T + i];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + k * (256 / lanes);
+      float s = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        s = fmaf(load_elem(&x, e, p.dtype), load_elem(&y, e, p.dtype), s);
-    }
-    for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (sub == 0) {
-      dst[r] = on ? -a.lse[(size_t)bh * p.T + i] * kLog2e : -CUDART_INF_F;
-      dst[kBM + r] = s;
+        s = fmaf(load_elem(&x[k], e, p.dtype), load_elem(&y[k], e, p.dtype), s);
+      for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (sub == 0 && r < kBM) {
+        dst[r] = -z[k] * kLog2e;
+        dst[kBM + r] = s;
+      }
     }
   }
 }
@@ -1366,13 +1514,13 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
       (e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
     return e;
   const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
-  if (p.T <= kExactDeltaTokens) {
-    e = launch_attn_exact_delta(p, t, bits, nullptr, stats, st);
-  } else {
-    attn_sm100_delta_kernel<<<p.B * p.Hq * n_t, 256, 0, st>>>(p, t, bits, stats);
-    e = cudaGetLastError();
-  }
-  if (e != cudaSuccess) return e;
+  const int few = exact_delta_tiles(p), heads = p.B * p.Hq;
+  if (few > 0)
+    attn_sm100_exact_delta_kernel<D, BF16>
+        <<<heads * few * (kBM / 16), 256, 0, st>>>(p, t, bits, stats);
+  if (n_t > few)
+    attn_sm100_delta_kernel<<<heads * (n_t - few), 256, 0, st>>>(p, t, bits, stats);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const long long group_bytes = 4ll * G * p.T * p.D;   // queries and dO
   for (int g0 = 0; g0 < groups; g0 += plan.per)
     for (int j0 = 0; j0 < n_t; j0 += plan.keys) {

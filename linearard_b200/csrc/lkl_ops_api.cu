@@ -202,9 +202,9 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
         at.ds_bytes,
         reinterpret_cast<float*>(base + at.acc), st));
   float2* rows = reinterpret_cast<float2*>(stats);
-  if ((s = launch_status(a.T <= lkl::kExactDeltaTokens
-                             ? lkl::launch_attn_exact_delta(a, t, bits, rows, nullptr, st)
-                             : lkl::launch_attn_delta(a, t, bits, rows, st))))
+  const bool few = a.T <= lkl::kExactDeltaKeys;
+  if (!few && (s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;
+  if ((few || a.causal) && (s = launch_status(lkl::launch_attn_exact_delta(a, t, bits, rows, st))))
     return s;
   return launch_status(lkl::launch_attn_generic_backward(a, t, bits, rows, st));
 }

@@ -408,3 +408,34 @@ def test_short_sequences_keep_small_gradients(T, D):
     assert_within(dq, ref.dq, D ** -0.5 * tol @ kk.abs() * (1 + u) + u * ref.dq.abs() + 1e-30, "dq")
     assert_within(dk, ref.dk, D ** -0.5 * tol.transpose(-1, -2) @ qq.abs() * (1 + u)
                   + u * ref.dk.abs() + 1e-30, "dk")
+
+
+@pytest.mark.parametrize("causal, T, D", [
+    (True, 129, 16), (True, 256, 128), (True, 300, 64), (True, 300, 256), (True, 1000, 128),
+    (False, 200, 32), (False, 256, 128),
+])
+def test_rows_of_few_keys_keep_small_gradients(causal, T, D):
+    """Rows that see at most 256 keys take delta from the probabilities in a sequence of any
+    length, so that their dq holds no more than the roundings of dS and of the result."""
+    n, H, Hkv = min(T, 256), 4, 2
+    q, k, v, g = make(2, H, Hkv, T, D, "bf16", seed=T, scale=2.2)
+    out, lse = attn_forward(q, k, v, causal=causal)
+    dq, _, _ = attn_backward(g, q, k, v, out, lse, causal=causal)
+    qq, gg = q[:, :, :n].double(), g[:, :, :n].double()
+    kk, vv = (t[:, :, :n].double().repeat_interleave(H // Hkv, 1) for t in (k, v))
+    S = (qq @ kk.transpose(-1, -2)) * D ** -0.5
+    keep = torch.ones(n, n, dtype=torch.bool, device="cuda")
+    keep = keep.tril() if causal else keep
+    P = S.masked_fill(~keep, -torch.inf).softmax(-1)
+    dP = gg @ vv.transpose(-1, -2)
+    dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+    # fp32 as above; a sum over up to 256 keys instead of 128 behind dq and delta
+    u, c = 2.0 ** -8, (2 * D + 512) * 2.0 ** -24
+    mag = gg.abs() @ vv.abs().transpose(-1, -2)
+    size = (qq.abs() @ kk.abs().transpose(-1, -2)) * D ** -0.5
+    top = torch.where(keep, size, 0.0).amax(-1, keepdim=True)
+    tol = torch.where(keep, u * dS.abs() + P * (mag + (P * mag).sum(-1, keepdim=True))
+                      * (c * (2 + 2 * top) + 2.0 ** -18), 0.0) + 2.0 ** -126
+    exact = D ** -0.5 * dS @ kk
+    assert_within(dq[:, :, :n], exact, D ** -0.5 * tol @ kk.abs() * (1 + u) + u * exact.abs()
+                  + 1e-30, "dq")
