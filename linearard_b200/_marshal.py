@@ -6,7 +6,7 @@ import contextlib
 
 import torch
 
-__all__ = ["on_device", "raw_stream", "once_when_recorded"]
+__all__ = ["on_device", "raw_stream", "once_when_recorded", "same_as_saved"]
 
 _HERE = contextlib.nullcontext()
 
@@ -31,3 +31,12 @@ def once_when_recorded(backward):
     def run(ctx, *grads):
         return (once if torch.is_grad_enabled() else backward)(ctx, *grads)
     return staticmethod(run)
+
+
+def same_as_saved(t, shape, dtype, device):
+    """Checks a tensor that autograd kept for the backward.  A saved-tensor hook
+    (``torch.autograd.graph.save_on_cpu``, activation offload) may give it back with
+    other strides, never with another shape, type or device."""
+    assert t.shape == shape and t.dtype is dtype and t.device == device, \
+        "a saved tensor came back with another shape, dtype or device"
+    return t

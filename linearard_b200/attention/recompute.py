@@ -22,8 +22,8 @@ import ctypes
 import torch
 
 from .. import _lib
-from .._marshal import on_device, once_when_recorded, raw_stream
-from ..attention_KL._common import (_DT, SUPPORTED_HEAD_DIMS, TC_HEAD_DIMS, check_lse,
+from .._marshal import on_device, once_when_recorded, raw_stream, same_as_saved
+from ..attention_KL._common import (_DT, _MASK_DT, SUPPORTED_HEAD_DIMS, TC_HEAD_DIMS, check_lse,
                                     prepare_mask, scale_of)
 
 __all__ = ["attn", "attn_forward", "attn_backward", "AttnFn"]
@@ -95,8 +95,7 @@ def _workspace(n, device):
 
 
 def _forward(q, k, v, mask, prob):
-    """(out, lse, plan) of checked arguments; mask on the device or None.  plan: the
-    strides of q, k, v and out for the backward, None where one had to be copied."""
+    """(out, lse) of checked arguments; mask on the device or None."""
     L, dev = _lib.lib(), q.device
     with on_device(dev):
         (rq, sq), (rk, sk), (rv, sv) = _readable(q), _readable(k), _readable(v)
@@ -107,29 +106,26 @@ def _forward(q, k, v, mask, prob):
         if mask is not None:
             n, m = L.lkl_attn_forward_workspace_size(ref, 1), mask.data_ptr()
             ws, at = _workspace(n, dev)
-        strides = (*sq, *sk, *sv, *_strides(out))
         st = L.lkl_attn_forward(rq.data_ptr(), rk.data_ptr(), rv.data_ptr(),
-                                (ctypes.c_int64 * 12)(*strides), m, ref, out.data_ptr(),
-                                lse.data_ptr(), at, n, raw_stream(dev))
+                                (ctypes.c_int64 * 12)(*sq, *sk, *sv, *_strides(out)), m, ref,
+                                out.data_ptr(), lse.data_ptr(), at, n, raw_stream(dev))
     _lib.check(st, "lkl_attn_forward")
-    return out, lse, strides if rq is q and rk is k and rv is v else None
+    return out, lse
 
 
-def _backward(dout, q, k, v, out, lse, mask, prob, plan=None):
+def _backward(dout, q, k, v, out, lse, mask, prob):
     L, dev = _lib.lib(), q.device
     with on_device(dev):
         dq, dk, dv = _like(q), _like(k), _like(v)
-        if plan is None:
-            (q, sq), (k, sk), (v, sv), (out, so) = (_readable(t) for t in (q, k, v, out))
-            plan = (*sq, *sk, *sv, *so)
+        (q, sq), (k, sk), (v, sv), (out, so) = (_readable(t) for t in (q, k, v, out))
         dout, sd = _readable(dout)
         ref = ctypes.byref(prob)
         n = L.lkl_attn_backward_workspace_size(ref, 0 if mask is None else 1)
         ws, at = _workspace(n, dev)
         st = L.lkl_attn_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            dout.data_ptr(), (ctypes.c_int64 * 24)(*plan, *sd, *_strides(dq), *_strides(dk),
-                                                   *_strides(dv)),
+            dout.data_ptr(), (ctypes.c_int64 * 24)(*sq, *sk, *sv, *so, *sd, *_strides(dq),
+                                                   *_strides(dk), *_strides(dv)),
             None if mask is None else mask.data_ptr(), ref, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), at, n, raw_stream(dev))
     _lib.check(st, "lkl_attn_backward")
@@ -141,7 +137,7 @@ def attn_forward(q, k, v, attn_mask=None, causal=True, sm_scale=None):
     Rows that the mask removes have out 0 and lse 0."""
     _check(q, k, v)
     mask, mdt = prepare_mask(attn_mask, q.shape[0], q.shape[2], q.device)
-    return _forward(q, k, v, mask, _problem(q, k, causal, mdt, sm_scale))[:2]
+    return _forward(q, k, v, mask, _problem(q, k, causal, mdt, sm_scale))
 
 
 def attn_backward(dout, q, k, v, out, lse, attn_mask=None, causal=True, sm_scale=None):
@@ -161,7 +157,7 @@ def attn_backward(dout, q, k, v, out, lse, attn_mask=None, causal=True, sm_scale
 class AttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, prob):
-        out, lse, ctx.plan = _forward(q, k, v, mask, prob)
+        out, lse = _forward(q, k, v, mask, prob)
         ctx.save_for_backward(q, k, v, out, lse, mask)
         ctx.prob = prob
         return out
@@ -169,7 +165,15 @@ class AttnFn(torch.autograd.Function):
     @once_when_recorded
     def backward(ctx, dout):
         q, k, v, out, lse, mask = ctx.saved_tensors
-        dq, dk, dv = _backward(dout, q, k, v, out, lse, mask, ctx.prob, ctx.plan)
+        p, dt, dev = ctx.prob, dout.dtype, dout.device
+        # strides are read from what came back: a hook may have changed them
+        for t, H in ((q, p.Hq), (k, p.Hkv), (v, p.Hkv), (out, p.Hq)):
+            same_as_saved(t, (p.B, H, p.T, p.D), dt, dev)
+        lse = same_as_saved(lse, (p.B, p.Hq, p.T), torch.float32, dev).contiguous()
+        if mask is not None:
+            assert _MASK_DT.get(mask.dtype) == p.mask_dtype, "a saved mask came back as another type"
+            mask = same_as_saved(mask, (p.B, p.T), mask.dtype, dev).contiguous()
+        dq, dk, dv = _backward(dout, q, k, v, out, lse, mask, p)
         return dq, dk, dv, None, None
 
 
