@@ -4,6 +4,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from .._marshal import same_as_saved
 
 _DT = {torch.float16: _lib.LKL_F16, torch.bfloat16: _lib.LKL_BF16, torch.float32: _lib.LKL_F32}
 
@@ -22,3 +23,12 @@ def rows_of(x) -> _lib.LKLLogits:
     if x.ndim == 2:
         return _lib.LKLLogits(1, x.shape[0], x.shape[1], 0, x.stride(0), _DT[x.dtype])
     return _lib.LKLLogits(*x.shape, *x.stride()[:2], _DT[x.dtype])
+
+
+def saved_rows(x, shape, dtype, device):
+    """(tensor, its rows) of logits that autograd kept for a backward: the strides are
+    those that it came back with."""
+    same_as_saved(x, shape, dtype, device)
+    if x.stride(-1) != 1 and x.shape[-1] != 1:
+        x = x.contiguous()
+    return x, rows_of(x)

@@ -15,9 +15,9 @@ import ctypes
 import torch
 
 from .. import _lib
-from .._marshal import on_device, once_when_recorded, raw_stream
-from ..attention_KL._common import prepare_mask
-from ._common import check_logits, rows_of
+from .._marshal import on_device, once_when_recorded, raw_stream, same_as_saved
+from ..attention_KL._common import _MASK_DT, prepare_mask
+from ._common import check_logits, rows_of, saved_rows
 
 __all__ = ["logits_kl_align", "logits_kl_forward", "logits_kl_backward", "LogitsKLAlignFn"]
 
@@ -106,14 +106,24 @@ class LogitsKLAlignFn(torch.autograd.Function):
     def forward(ctx, s_logits, t_logits, mask, mdt, temperature, rows):
         loss, lse_s, lse_t = _forward(s_logits, t_logits, mask, mdt, temperature, rows)
         ctx.save_for_backward(s_logits, t_logits, lse_s, lse_t, mask)
-        ctx.mdt, ctx.temperature, ctx.rows = mdt, temperature, rows
+        ctx.mdt, ctx.temperature = mdt, temperature
+        ctx.shape, ctx.dtype, ctx.device = s_logits.shape, s_logits.dtype, s_logits.device
         return loss
 
     @once_when_recorded
     def backward(ctx, dloss):
         s_logits, t_logits, lse_s, lse_t, mask = ctx.saved_tensors
-        ds = _backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.mdt, ctx.temperature, ctx.rows,
-                       dloss.to(torch.float32))
+        shape, dt, dev = ctx.shape, ctx.dtype, ctx.device
+        lse_s, lse_t = (same_as_saved(t, shape[:-1], torch.float32, dev).contiguous()
+                        for t in (lse_s, lse_t))
+        if mask is not None:
+            assert _MASK_DT.get(mask.dtype) == ctx.mdt, "a saved mask came back as another type"
+            rows = shape[:-1] if len(shape) == 3 else (1, shape[0])
+            mask = same_as_saved(mask, rows, mask.dtype, dev).contiguous()
+        (s_logits, s_rows), (t_logits, t_rows) = (saved_rows(x, shape, dt, dev)
+                                                  for x in (s_logits, t_logits))
+        ds = _backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.mdt, ctx.temperature,
+                       (s_rows, t_rows), dloss.to(torch.float32))
         return ds, None, None, None, None, None      # the teacher gets no gradient
 
 

@@ -14,8 +14,8 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
-from .._marshal import on_device, once_when_recorded, raw_stream
-from ._common import check_logits, rows_of
+from .._marshal import on_device, once_when_recorded, raw_stream, same_as_saved
+from ._common import check_logits, rows_of, saved_rows
 
 __all__ = ["token_logprobs", "TokenLogprobs", "TokenLogprobsFn", "MAX_TOP_K"]
 
@@ -54,7 +54,8 @@ class TokenLogprobsFn(torch.autograd.Function):
         logprob, entropy, lse, top_v, top_i = _forward(logits, rows, targets, top_k, ignore_index)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, targets, lse, entropy)
-        ctx.rows, ctx.ignore_index = rows, ignore_index
+        ctx.shape, ctx.dtype, ctx.device = logits.shape, logits.dtype, logits.device
+        ctx.ignore_index = ignore_index
         if top_k:
             ctx.mark_non_differentiable(top_v, top_i)
         return logprob, entropy, top_v, top_i
@@ -64,13 +65,17 @@ class TokenLogprobsFn(torch.autograd.Function):
         if d_logprob is None and d_entropy is None:
             return None, None, None, None, None
         logits, targets, lse, entropy = ctx.saved_tensors
-        dev = logits.device
+        dev, shape = ctx.device, ctx.shape[:-1]
+        targets = same_as_saved(targets, shape, torch.int64, dev)
+        lse, entropy = (same_as_saved(t, shape, torch.float32, dev) for t in (lse, entropy))
         with on_device(dev):
+            logits, rows = saved_rows(logits, ctx.shape, ctx.dtype, dev)
+            targets, lse, entropy = (t.contiguous() for t in (targets, lse, entropy))
             g, h = (None if d is None else d.to(torch.float32).contiguous()
                     for d in (d_logprob, d_entropy))
-            dx = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+            dx = torch.empty(ctx.shape, device=dev, dtype=ctx.dtype)
             st = _lib.lib().lkl_token_logprobs_backward(
-                logits.data_ptr(), ctypes.byref(ctx.rows), targets.data_ptr(), ctx.ignore_index,
+                logits.data_ptr(), ctypes.byref(rows), targets.data_ptr(), ctx.ignore_index,
                 lse.data_ptr(), entropy.data_ptr(), None if g is None else g.data_ptr(),
                 None if h is None else h.data_ptr(), dx.data_ptr(), raw_stream(dev))
         _lib.check(st, "lkl_token_logprobs_backward")

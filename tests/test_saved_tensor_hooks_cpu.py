@@ -8,6 +8,7 @@ import torch
 
 from linearard_b200 import _lib
 from linearard_b200.attention import recompute
+from linearard_b200.logits import _common, kl, token
 
 
 class Recorder:
@@ -28,7 +29,7 @@ def recorder(monkeypatch):
     import contextlib
     r = Recorder()
     monkeypatch.setattr(_lib, "lib", lambda: r)
-    for m in (recompute,):
+    for m in (recompute, kl, token):
         monkeypatch.setattr(m, "on_device", lambda device: contextlib.nullcontext())
         monkeypatch.setattr(m, "raw_stream", lambda device: 0)
     return r
@@ -108,3 +109,79 @@ def test_attention_backward_refuses_other_types_from_a_hook(recorder):
         with pytest.raises(AssertionError, match="saved"):
             torch.autograd.grad(out.sum(), q)
         assert "lkl_attn_backward" not in recorder.calls
+
+
+def rows_end(r):
+    """One past the last element that a row descriptor reaches."""
+    return (r.B - 1) * r.sb + (r.T - 1) * r.st + r.V
+
+
+def check_rows(args, at, given, shape):
+    """The kernel's row descriptor is that of the tensor it is given."""
+    r = args[at + 1]._obj
+    mine = [t for t in given if t.data_ptr() == args[at] and tuple(t.shape) == shape]
+    assert (r.B, r.T, r.V) == shape
+    if mine and mine[0].stride(-1) == 1:
+        t = mine[0]
+        assert (r.sb, r.st) == t.stride()[:2]
+        assert rows_end(r) * t.element_size() <= (t.untyped_storage().nbytes()
+                                                  - t.storage_offset() * t.element_size())
+    else:                        # copied: rows have to be dense
+        assert not any(t.data_ptr() == args[at] for t in given)
+        assert (r.sb, r.st) == (shape[1] * shape[2], shape[2])
+
+
+@pytest.mark.parametrize("unpack", UNPACK)
+@pytest.mark.parametrize("cut", ["shift", "vocab", "whole"])
+def test_token_backward_reads_what_the_hook_gave_back(recorder, unpack, cut):
+    x = torch.randn(2, 6, 7)
+    x = {"shift": x[:, :-1], "vocab": x[..., 1:5], "whole": x}[cut].requires_grad_(True)
+    ids = torch.zeros(x.shape[:2], dtype=torch.int64)
+    hooks, given = held(UNPACK[unpack])
+    with hooks:
+        outs = token.TokenLogprobsFn.apply(x, _common.rows_of(x), ids, 0, -100)
+    (d,) = torch.autograd.grad(outs[0].sum(), x)
+    args = recorder.calls["lkl_token_logprobs_backward"]
+    check_rows(args, 0, given, tuple(x.shape))
+    assert d.shape == x.shape
+    if unpack != "strange":
+        for k in (2, 4, 5):          # targets, lse, entropy
+            assert any(t.data_ptr() == args[k] and t.is_contiguous() for t in given)
+
+
+@pytest.mark.parametrize("unpack", UNPACK)
+@pytest.mark.parametrize("cut", ["shift", "vocab", "whole"])
+@pytest.mark.parametrize("mask", [False, True])
+def test_kl_backward_reads_what_the_hook_gave_back(recorder, unpack, cut, mask):
+    s, t = torch.randn(2, 2, 6, 7).unbind(0)
+    s, t = ({"shift": x[:, :-1], "vocab": x[..., 1:5], "whole": x}[cut] for x in (s, t))
+    s = s.requires_grad_(True)
+    m = torch.ones(s.shape[:2], dtype=torch.int64) if mask else None
+    hooks, given = held(UNPACK[unpack])
+    with hooks:
+        loss = kl.LogitsKLAlignFn.apply(s, t, m, _lib.LKL_MASK_I64, 1.0,
+                                        (_common.rows_of(s), _common.rows_of(t)))
+    (d,) = torch.autograd.grad(loss, s)
+    args = recorder.calls["lkl_logits_kl_backward"]
+    check_rows(args, 0, given, tuple(s.shape))
+    check_rows(args, 2, given, tuple(t.shape))
+    assert d.shape == s.shape and (args[4] is not None) == mask
+    if unpack != "strange":
+        for k in (7, 8):             # the two log-sum-exps
+            assert any(z.data_ptr() == args[k] and z.is_contiguous() for z in given)
+
+
+def test_logits_backward_refuses_other_types_from_a_hook(recorder):
+    x = torch.randn(2, 6, 8).requires_grad_(True)
+    ids = torch.zeros(2, 6, dtype=torch.int64)
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    for bad in (lambda t: t.half() if t.is_floating_point() else t, lambda t: t[..., :4],
+                lambda t: t if t.is_floating_point() else t.int()):
+        with hooks(lambda t: t, bad):
+            lp = token.TokenLogprobsFn.apply(x, _common.rows_of(x), ids, 0, -100)[0]
+            loss = kl.LogitsKLAlignFn.apply(x, x.detach(), ids, _lib.LKL_MASK_I64, 1.0,
+                                            (_common.rows_of(x),) * 2)
+        for y in (lp.sum(), loss):
+            with pytest.raises(AssertionError, match="saved"):
+                torch.autograd.grad(y, x)
+    assert not any("backward" in name for name in recorder.calls)

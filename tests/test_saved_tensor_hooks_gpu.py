@@ -5,6 +5,7 @@ import torch
 
 from gpu_util import check_device_status
 from linearard_b200.attention import attn
+from linearard_b200.logits import logits_kl_align, token_logprobs
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +59,46 @@ def test_attention(hook, layout, D):
     check_device_status()
     for name, a, b in zip("qkv", got, want):
         assert torch.equal(a, b), name
+
+
+CUTS = {"shift": lambda x: x[:, :-1], "vocab": lambda x: x[..., 3:998], "rows": lambda x: x[1],
+        "whole": lambda x: x}
+
+
+def logits(cut, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(3, 9, 1003, device="cuda", generator=g).to(dtype)
+    return CUTS[cut](x)
+
+
+@pytest.mark.parametrize("hook", HOOKS)
+@pytest.mark.parametrize("cut", CUTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_token_logprobs(hook, cut, dtype):
+    x = logits(cut, dtype, 1).requires_grad_(True)
+    ids = torch.arange(x.shape[:-1].numel(), device="cuda").view(x.shape[:-1]) * 7 % x.shape[-1]
+
+    def grads(context):
+        with context():
+            r = token_logprobs(x, ids)
+        return torch.autograd.grad(r.logprob.sum() + 0.3 * r.entropy.sum(), x)[0]
+    want = grads(lambda: torch.enable_grad())
+    assert torch.equal(grads(HOOKS[hook]), want)
+
+
+@pytest.mark.parametrize("hook", HOOKS)
+@pytest.mark.parametrize("cut", CUTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", [False, True])
+def test_logits_kl(hook, cut, dtype, mask):
+    s, t = logits(cut, dtype, 1).requires_grad_(True), logits(cut, dtype, 2)
+    m = torch.ones(s.shape[:-1], device="cuda", dtype=torch.int64) if mask else None
+    if mask:
+        m[..., 5:] = 0
+
+    def grads(context):
+        with context():
+            loss = logits_kl_align(s, t, m, 1.5)
+        return torch.autograd.grad(loss, s)[0]
+    want = grads(lambda: torch.enable_grad())
+    assert torch.equal(grads(HOOKS[hook]), want)
