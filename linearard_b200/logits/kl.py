@@ -47,7 +47,7 @@ def _forward(s, t, mask, mdt, temperature, rows):
     dev, shape = s.device, s.shape[:-1]
     L = _lib.lib()
     with on_device(dev):
-        lse_s, lse_t = torch.empty((2, *shape), device=dev, dtype=torch.float32).unbind(0)
+        lse_s, lse_t = (torch.empty(shape, device=dev, dtype=torch.float32) for _ in range(2))
         loss = torch.empty((), device=dev, dtype=torch.float32)
         rs, rt = ctypes.byref(rows[0]), ctypes.byref(rows[1])
         n = L.lkl_logits_kl_workspace_size(rs)

@@ -34,7 +34,9 @@ def _forward(logits, rows, targets, top_k, ignore_index):
     """(logprob, entropy, lse, top_logprobs, top_indices) of checked arguments."""
     dev, shape = logits.device, targets.shape
     with on_device(dev):
-        logprob, entropy, lse = torch.empty((3, *shape), device=dev, dtype=torch.float32).unbind(0)
+        # tensors of their own: views of one could not be changed in place
+        logprob, entropy, lse = (torch.empty(shape, device=dev, dtype=torch.float32)
+                                 for _ in range(3))
         top_v = top_i = None
         if top_k:
             top_v = torch.empty((*shape, top_k), device=dev, dtype=torch.float32)
@@ -88,7 +90,8 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100) -> TokenLogprobs
     ignore_index and NaN where it is any other number outside [0, V).
     top_k: up to 32 alternatives, largest first, equal logits by the lowest
     index.  logprob and entropy carry gradients to the logits; the
-    alternatives carry none."""
+    alternatives carry none.  logprob may be changed in place; the backward needs
+    entropy as it is (autograd raises where it was changed)."""
     check_logits(logits)
     assert isinstance(targets, torch.Tensor), "targets must be a torch.Tensor"
     assert targets.device == logits.device, "targets must be on the device of the logits"
