@@ -12,6 +12,7 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._marshal import on_device, once_when_recorded, raw_stream, same_as_saved
@@ -101,7 +102,9 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100) -> TokenLogprobs
         "top_k must be from 0 to min(V, 32)"
     assert isinstance(ignore_index, int), "ignore_index must be an integer"
     rows, targets = rows_of(logits), targets.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
+    # a dual tensor does not require grad: the function refuses it, its tangent is not lost
+    if (logits.requires_grad and torch.is_grad_enabled()
+            or forward_ad.unpack_dual(logits).tangent is not None):
         return TokenLogprobs(*TokenLogprobsFn.apply(logits, rows, targets, top_k, ignore_index))
     logprob, entropy, _, top_v, top_i = _forward(logits, rows, targets, top_k, ignore_index)
     return TokenLogprobs(logprob, entropy, top_v, top_i)

@@ -45,3 +45,15 @@ def test_outputs_share_no_storage():
     outs += kl._forward(x, x, None, _lib.LKL_MASK_U8, 1.0, (rows, rows))
     assert len({t.untyped_storage().data_ptr() for t in outs}) == len(outs)
     assert not any(t._is_view() for t in outs)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor does not require grad, and its tangent would be lost."""
+    import torch.autograd.forward_ad as fwad
+    monkeypatch.setattr(token, "check_logits", lambda x: None)
+    x, ids = torch.randn(3, 5), torch.zeros(3, dtype=torch.int64)
+    with fwad.dual_level():
+        with pytest.raises(RuntimeError, match="forward"):
+            token.token_logprobs(fwad.make_dual(x, torch.ones_like(x)), ids)
+        token.token_logprobs(x, ids)
+    token.token_logprobs(x, ids)
