@@ -62,6 +62,7 @@ def prepare_mask(attn_mask, B, T, device):
         assert attn_mask.is_contiguous(), "attn_mask must be contiguous"
         attn_mask = attn_mask.to(device=device)
     assert attn_mask.is_cuda, "attn_mask must be on CUDA"
+    assert attn_mask.device == device, "attn_mask must be on the device of the tensors"
     assert attn_mask.ndim == 2, "attn_mask shape must be [B,T]"
     assert attn_mask.shape[0] == B and attn_mask.shape[1] == T, "attn_mask shape must be [B,T]"
     assert attn_mask.dtype in _MASK_DT, "attn_mask dtype is invalid"
