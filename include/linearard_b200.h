@@ -326,7 +326,9 @@ int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, cons
  * every stride a positive multiple of 8 elements; everything else runs on
  * CUDA-core kernels.  lkl_last_path() tells which.  An output may not start
  * where an input does.
- * Sums and softmax statistics are fp32; P and dS are rounded to the tensors'
+ * Sums and softmax statistics are fp32, so a probability carries 2^-23 of its
+ * score's size (sm_scale q . k): scores beyond some 2^20 are not told apart.
+ * P and dS are rounded to the tensors'
  * type before their products on the tensor cores (in fp16 a dS beyond 65504
  * overflows: scale the loss so that dout . v stays below).  Results are reproducible
  * bit for bit: every output row has one writer.
@@ -336,7 +338,7 @@ typedef struct lkl_attn_problem {
   int32_t dtype;      /* LKL_F16 or LKL_BF16                                   */
   int32_t causal;     /* nonzero: keep j <= i                                  */
   int32_t mask_dtype; /* lkl_mask_dtype, ignored when mask == NULL             */
-  float sm_scale;     /* <= 0 selects 1/sqrt(D)                                */
+  float sm_scale;     /* <= 0 selects 1/sqrt(D); else from 2^-126 to below 2^127 */
 } lkl_attn_problem;
 
 enum lkl_attn_tensor {

@@ -49,7 +49,8 @@ def _check(q, k, v):
 def _problem(q, k, causal, mask_dtype, sm_scale):
     B, Hq, T, D = q.shape
     sc = scale_of(sm_scale, D, "sm_scale")
-    assert 0.0 < sc < float("inf"), "sm_scale must be positive"
+    # normal numbers of single precision, also when multiplied by log2(e)
+    assert 2.0 ** -126 <= sc < 2.0 ** 127, "sm_scale must be positive"
     return _lib.LKLAttnProblem(B, Hq, k.shape[1], T, D, _DT[q.dtype], 1 if causal else 0,
                                mask_dtype, sc)
 

@@ -52,7 +52,6 @@ constexpr int kFaProducer = 8, kFaMma = 9, kFaCleaner = 10;
 // stays below 2^slack, where its rounding is as exact as below 1.  fp16 ends at 2^16.
 template <bool BF16>
 constexpr float kFaSlack = BF16 ? 40.f : 8.f;
-constexpr float kMaskedScore = -1.0e30f;
 
 template <int D>
 struct FaLayout {
@@ -397,7 +396,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            if (!(c * 32 + k <= lim && ((tb.w[c] >> k) & 1u))) x[c][k] = kMaskedScore;
+            if (!(c * 32 + k <= lim && ((tb.w[c] >> k) & 1u))) x[c][k] = -CUDART_INF_F;
       }
       float mx[8];   // eight chains: a single one would wait 64 times for the last maximum
 #pragma unroll
@@ -412,7 +411,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
                                            fmax3(mx[5], mx[6], mx[7])) * cs);
       if (__any_sync(0xffffffffu, live && m_new > ref + kFaSlack<BF16>)) {
         if (n > 0) {
-          const float f = ex2(ref - m_new);
+          const float f = ref == m_new ? 1.f : ex2(ref - m_new);   // -inf both: nothing yet
           const uint64_t f2 = f2pack(f, f);
           l *= f;
 #pragma unroll
@@ -428,7 +427,8 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
         }
         ref = m_new;
       }
-      const uint64_t nref2 = f2pack(-ref, -ref);
+      const float nref = ref == -CUDART_INF_F ? 0.f : -ref;   // no score above -inf so far
+      const uint64_t nref2 = f2pack(nref, nref);
       uint64_t sum2[4] = {};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {

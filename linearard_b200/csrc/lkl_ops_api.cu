@@ -17,6 +17,9 @@ int32_t check_attn(const lkl_attn_problem* p) {
   if (!head_dim_ok(p->D)) return LKL_ERR_BAD_HEAD_DIM;
   if (p->dtype != LKL_F16 && p->dtype != LKL_BF16) return LKL_ERR_BAD_DTYPE;
   if (p->mask_dtype < LKL_MASK_BOOL || p->mask_dtype > LKL_MASK_I64) return LKL_ERR_BAD_DTYPE;
+  // single precision holds the scale and its multiple by log2(e)
+  if (!(p->sm_scale <= 0.f) && !(p->sm_scale >= 0x1p-126f && p->sm_scale < 0x1p127f))
+    return LKL_ERR_BAD_SHAPE;
   // block counts and 32-bit token arithmetic
   if ((long long)p->B * p->Hq * (((long long)p->T + 31) / 32) > INT32_MAX ||
       p->T > INT32_MAX - 256)
