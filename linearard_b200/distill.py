@@ -69,11 +69,36 @@ class Capture:
         self.q[layer], self.k[layer], self.v[layer] = q, k, v
 
 
+# Options of transformers' attention interface that change its result and that `attn`
+# does not have
+_NOT_COMPUTED = ("softcap", "s_aux", "head_mask", "position_bias", "cu_seq_lens_q",
+                 "cu_seq_lens_k")
+
+
+def _check_mask_function(f, batch, q_length, kv_length, device):
+    """Refuses a transformers mask function that removes more than the future (a window
+    narrower than the sequence, packed sequences).  One that is neither of the plain two
+    is evaluated, 1024 rows at a time."""
+    from transformers.masking_utils import bidirectional_mask_function, causal_mask_function
+    if f in (None, causal_mask_function, bidirectional_mask_function):
+        return
+    b, h, q, k = (torch.arange(n, device=device).view([-1 if i == d else 1 for i in range(4)])
+                  for d, n in enumerate((batch, 1, q_length, kv_length)))
+    causal = full = torch.ones((), dtype=torch.bool, device=device)
+    for rows in q.split(1024, dim=2):
+        keep = f(b, h, rows, k)
+        causal = causal & (keep == (k <= rows)).all()
+        full = full & keep.all()
+    assert bool(causal | full), \
+        "the attention takes causal or full masks, no windows or packed sequences"
+
+
 def register_capture_attention(name=None, attention="sdpa"):
     """Register an attention implementation that records q, k, v (after
     RoPE, as the reference hook sees them) and then runs SDPA, or this package's
     attention (``attention="own"``: fp16 or bf16 on CUDA; a [B, T] padding mask
-    removes tokens as queries and as keys)."""
+    removes tokens as queries and as keys; a sliding window narrower than the
+    sequence, packed sequences, soft caps and sinks are refused)."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
     from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
@@ -87,6 +112,10 @@ def register_capture_attention(name=None, attention="sdpa"):
         if attention == "sdpa":
             return sdpa_attention_forward(module, query, key, value, attention_mask, **kwargs)
         assert not kwargs.get("dropout"), "the attention has no dropout"
+        window = kwargs.get("sliding_window")
+        assert window is None or window >= key.shape[2], "the attention has no sliding window"
+        for option in _NOT_COMPUTED:
+            assert kwargs.get(option) is None, f"the attention has no {option}"
         assert attention_mask is None or attention_mask.ndim == 2, \
             "the attention takes [B, T] padding masks"
         causal = kwargs.get("is_causal")
@@ -96,7 +125,10 @@ def register_capture_attention(name=None, attention="sdpa"):
         out = attn(query, key, value, attention_mask, causal, kwargs.get("scaling"))
         return out.transpose(1, 2), None
 
-    def padding_mask(*args, attention_mask=None, **kwargs):
+    def padding_mask(*args, attention_mask=None, mask_function=None, batch_size=None,
+                     q_length=None, kv_length=None, device=None, **kwargs):
+        assert not args, "the arguments of a mask function go by name"
+        _check_mask_function(mask_function, batch_size, q_length, kv_length, device)
         return attention_mask            # [B, T]: the operator takes it as it is
 
     ALL_ATTENTION_FUNCTIONS.register(name, capture_attention)
