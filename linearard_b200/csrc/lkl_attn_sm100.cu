@@ -358,7 +358,9 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float cs = p.sc * kLog2e;
     const uint64_t cs2 = f2pack(cs, cs);
-    float ref = -CUDART_INF_F, l = 0.f;   // exponent offset and sum of 2^(x cs - ref)
+    // Exponent offset and sum of 2^(x cs - ref).  The offset starts finite: as long as a
+    // row has nothing above -inf, its exponents are -inf and not inf - inf.
+    float ref = -CUDART_MAX_NORMAL_F, l = 0.f;
     const int my_ct = t ? n_ct[1] : n_ct[0];
     // rows that are not written take no part in the warp's decisions
     const bool live = i < p.T && my_ct > 0 && token_valid(MASKED ? bits : nullptr, words, b, i);
@@ -411,7 +413,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
                                            fmax3(mx[5], mx[6], mx[7])) * cs);
       if (__any_sync(0xffffffffu, live && m_new > ref + kFaSlack<BF16>)) {
         if (n > 0) {
-          const float f = ref == m_new ? 1.f : ex2(ref - m_new);   // -inf both: nothing yet
+          const float f = ex2(ref - m_new);
           const uint64_t f2 = f2pack(f, f);
           l *= f;
 #pragma unroll
@@ -427,8 +429,7 @@ attn_sm100_forward_kernel(const __grid_constant__ CUtensorMap tm_q,
         }
         ref = m_new;
       }
-      const float nref = ref == -CUDART_INF_F ? 0.f : -ref;   // no score above -inf so far
-      const uint64_t nref2 = f2pack(nref, nref);
+      const uint64_t nref2 = f2pack(-ref, -ref);
       uint64_t sum2[4] = {};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
