@@ -1146,13 +1146,12 @@ attn_sm100_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
         tmem_ld32(row_addr + (which ? kColDk : kColDv) + col0 + c2, v);
         tmem_wait_ld_dep(v);
         if (c.parts > 1) {
-          if (key >= p.T) continue;
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            if (col0 + c2 + k >= p.D) break;
-            *reinterpret_cast<float4*>(sum_row + col0 + c2 + k) =
-                live ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0, 0, 0, 0);
-          }
+          for (int k = 0; k < 32; k += 4)
+            if (key < p.T && col0 + c2 + k < p.D)
+              *reinterpret_cast<float4*>(sum_row + col0 + c2 + k) =
+                  live ? make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]) : make_float4(0, 0, 0, 0);
+          __syncwarp();   // the next step's TMEM load takes the whole warp
           continue;
         }
         uint32_t u[16];
@@ -1396,6 +1395,7 @@ attn_sm100_dq_kernel(const __grid_constant__ CUtensorMap tm_k, const AttnProblem
 #pragma unroll
       for (int col = 0; col < D; col += 32) {
         float v[32];
+        __syncwarp();   // lanes past the last row leave a step early; the load takes the warp
         if (any) {
           tmem_ld32(taddr + col, v);
           tmem_wait_ld_dep(v);

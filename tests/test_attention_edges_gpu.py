@@ -18,3 +18,13 @@ def test_small_scales_keep_removed_keys_out(sm_scale, causal, D):
     check(q, k, v, g, None, causal, sm_scale, backward=False)
     if sm_scale > 1e-35:        # below, dq and dk are subnormal
         check(q, k, v, g, right_pad(2, 300, [300, 70]), causal, sm_scale)
+
+
+@pytest.mark.parametrize("D", [8, 32, 128])
+@pytest.mark.parametrize("Hq,Hkv,causal,mask", [(2, 1, True, False), (1, 1, False, True),
+                                                (4, 2, True, True)])
+def test_shared_key_tiles_of_every_head_dim(D, Hq, Hkv, causal, mask):
+    """Few long key tiles, each the work of several blocks, whose sums have D columns; the
+    last tile ends inside a warp."""
+    q, k, v, g = make(1, Hq, Hkv, 4300, D, "bf16")
+    check(q, k, v, g, right_pad(1, 4300, [4111]) if mask else None, causal)
