@@ -31,14 +31,50 @@ cudaError_t launch_attn_delta(const AttnProblem& p, const AttnTensors& t, const 
 // of P behind it.  dS_ij = P_ij (dP_ij - delta_i) is a small difference where one key has
 // most of a row, as in rows of few keys: with the rounded out, dk of two tokens was off by
 // 17% (bf16), and 1% at eight.  Rows that see at most this many keys (in a causal sequence
-// of any length, its first) therefore take the sum; beyond it rows of many keys carry the
+// of any length, the first of its tokens that the mask keeps; else all rows of a sequence
+// with no more tokens) therefore take the sum; beyond it rows of many keys carry the
 // gradient and the roundings of dS and of the result outweigh that of out (dq of 4096
-// tokens, bf16, emulated: 0.0025 of its size off with no row by the sum, 0.00240 with
-// the first 256, 0.00236 with all).
+// tokens, D 128, bf16, emulated: 0.0025 of its size off with no row by the sum, 0.00240
+// with the first 256, 0.00236 with all).
 constexpr int kExactDeltaKeys = 256;
-// The same into rows[] by that sum, for the rows below kExactDeltaKeys.
+// The same into rows[] by that sum, for the rows that see at most kExactDeltaKeys keys.
 cudaError_t launch_attn_exact_delta(const AttnProblem& p, const AttnTensors& t,
                                     const uint32_t* bits, float2* rows, cudaStream_t st);
+// Those rows are the first tokens of a sequence.  Under a mask that leaves room for more
+// (T > kExactDeltaKeys) they may stand anywhere, and a kernel finds them by their rank
+// among the tokens that the mask keeps.
+inline __host__ __device__ bool exact_delta_ranked(const AttnProblem& p, const uint32_t* bits) {
+  return bits != nullptr && p.T > kExactDeltaKeys;
+}
+
+// A block of 256 threads finds the tokens of batch b whose rows see at most
+// kExactDeltaKeys keys: their positions, ascending, in pos[] and their number in every
+// thread.  sums: one int a warp.
+__device__ __forceinline__ int few_key_tokens(const uint32_t* bits, const AttnProblem& p, int b,
+                                              int* pos, int* sums) {
+  const int words = (p.T + 31) >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int n = 0;   // tokens of the words before
+  for (int w0 = 0; w0 < words; w0 += 256) {
+    const int w = w0 + threadIdx.x;
+    uint32_t m = w < words ? bits[(size_t)b * words + w] : 0u;
+    int upto = __popc(m);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int at = n + upto - __popc(m);
+    for (int k = 0; k < 8; ++k) {
+      if (k < warp) at += sums[k];
+      n += sums[k];
+    }
+    for (; m && at < kExactDeltaKeys; m &= m - 1) pos[at++] = w * 32 + __ffs(m) - 1;
+    __syncthreads();
+    if (n > kExactDeltaKeys) return p.causal ? kExactDeltaKeys : 0;
+  }
+  return n;
+}
 cudaError_t launch_attn_generic_backward(const AttnProblem& p, const AttnTensors& t,
                                          const uint32_t* bits, const float2* rows,
                                          cudaStream_t st);

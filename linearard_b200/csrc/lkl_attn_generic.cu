@@ -145,43 +145,66 @@ __global__ void attn_delta_kernel(const AttnProblem p, const AttnTensors a,
   }
 }
 
-// delta_i = sum_j P_ij (dout_i . v_j) for rows that see few keys; a block takes 32.
+// Rows pos[r0 .. r0 + 32) of head h, zeros from rank n on.
+template <int D>
+__device__ __forceinline__ void attn_load_ranked(float* dst, const void* src,
+                                                 const TensorStrides& s, int b, int h, int r0,
+                                                 const int* pos, int n, int dtype) {
+  const size_t base = (size_t)b * s.b + (size_t)h * s.h;
+  for (int e = threadIdx.x; e < kABM * D; e += kAThreads) {
+    const int r = e / D, d = e % D;
+    dst[r * (D + 1) + d] =
+        r0 + r < n ? load_elem(src, base + (size_t)pos[r0 + r] * s.t + d, dtype) : 0.f;
+  }
+}
+
+// delta_i = sum_j P_ij (dout_i . v_j) for rows that see few keys; a block takes 32.  Rows
+// and keys are ranks among the tokens at pos[]: without a mask the first ones.
 template <int D>
 __global__ void __launch_bounds__(kAThreads)
 attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
                         const uint32_t* __restrict__ bits, float2* __restrict__ rows,
                         int n_rt) {
+  __shared__ int pos[kExactDeltaKeys], sums[8];
   extern __shared__ float smem[];
   float* sQ = smem;
   float* sG = sQ + kABM * (D + 1);
   float* sK = sG + kABM * (D + 1);
   float* sV = sK + kABM * (D + 1);
-  const int n_t = (p.T + kABM - 1) / kABM, words = (p.T + 31) >> 5;
   const int bh = blockIdx.x / n_rt, mt = blockIdx.x % n_rt;   // n_rt: row tiles to take
   const int b = bh / p.Hq, h = bh % p.Hq, g = h / (p.Hq / p.Hkv);
-  const int r = threadIdx.x >> 3, sub = threadIdx.x & 7, i = mt * kABM + r;
-  const bool row = i < p.T && token_valid(bits, words, b, i);
-  const float z = row ? -a.lse[(size_t)bh * p.T + i] * kLog2e : -CUDART_INF_F;
-  attn_load_tile<D>(sQ, a.q, a.sq, b, h, mt * kABM, p.T, p.dtype, bits);
-  attn_load_tile<D>(sG, a.dout, a.sdo, b, h, mt * kABM, p.T, p.dtype, bits);
+  int n = min(p.T, kExactDeltaKeys);
+  if (bits) {
+    n = few_key_tokens(bits, p, b, pos, sums);
+  } else {
+    pos[threadIdx.x] = threadIdx.x;
+    __syncthreads();
+  }
+  const int r = threadIdx.x >> 3, sub = threadIdx.x & 7, rank = mt * kABM + r;
+  if (mt * kABM >= n) return;
+  const bool row = rank < n;
+  const size_t at = (size_t)bh * p.T + (row ? pos[rank] : 0);
+  const float z = row ? -a.lse[at] * kLog2e : -CUDART_INF_F;
+  attn_load_ranked<D>(sQ, a.q, a.sq, b, h, mt * kABM, pos, n, p.dtype);
+  attn_load_ranked<D>(sG, a.dout, a.sdo, b, h, mt * kABM, pos, n, p.dtype);
   float delta = 0.f;
-  const int n_j = p.causal ? mt + 1 : n_t;
+  const int n_j = p.causal ? mt + 1 : (n + kABM - 1) / kABM;
   for (int j = 0; j < n_j; ++j) {
     __syncthreads();
-    attn_load_tile<D>(sK, a.k, a.sk, b, g, j * kABM, p.T, p.dtype, bits);
-    attn_load_tile<D>(sV, a.v, a.sv, b, g, j * kABM, p.T, p.dtype, bits);
+    attn_load_ranked<D>(sK, a.k, a.sk, b, g, j * kABM, pos, n, p.dtype);
+    attn_load_ranked<D>(sV, a.v, a.sv, b, g, j * kABM, pos, n, p.dtype);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int cl = sub + 8 * k, c = j * kABM + cl;
-      if (row && c < p.T && (!p.causal || c <= i) && token_valid(bits, words, b, c)) {
+      if (row && c < n && (!p.causal || c <= rank)) {
         const float s = attn_dot<D>(sQ + r * (D + 1), sK + cl * (D + 1)) * p.sc * kLog2e;
         delta = fmaf(exp2f(s + z), attn_dot<D>(sG + r * (D + 1), sV + cl * (D + 1)), delta);
       }
     }
   }
   delta = sum8(delta);
-  if (sub == 0 && i < p.T) rows[(size_t)bh * p.T + i] = make_float2(z, delta);
+  if (sub == 0 && row) rows[at] = make_float2(z, delta);
 }
 
 // dq_i = sc sum_j P_ij (dout_i . v_j - delta_i) k_j; query rows are stationary.

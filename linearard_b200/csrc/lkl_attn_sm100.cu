@@ -614,16 +614,21 @@ __device__ __forceinline__ void load_fragment_row(uint4 (&x)[NC], const void* ba
 // few for staging tiles and TMEM to pay.  The eight warps take 8 keys each in turn, at
 // most four times, and are joined in their order.  Bound by the latency of those
 // steps: 11.8 us for the 256 rows of 32 heads, D 128.
+//
+// pos == nullptr: rows and keys by position.  Otherwise they are ranks among the n
+// tokens at pos[], which the mask keeps.  stats: the head's.
 template <int D, bool BF16>
 __device__ __forceinline__ void exact_delta_rows(const AttnProblem& p, const AttnTensors& a,
                                                  const uint32_t* bits, int b, int h, int first,
-                                                 float* dst) {
+                                                 const int* pos, int n, float* stats) {
   constexpr int NC = D / 32;
   __shared__ float part[8][16];
   const int words = (p.T + 31) >> 5, lane = threadIdx.x & 31, quad = lane >> 2;
-  const int warp = threadIdx.x >> 5, i0 = first + quad, i1 = i0 + 8;
-  const bool on0 = i0 < p.T && token_valid(bits, words, b, i0);
-  const bool on1 = i1 < p.T && token_valid(bits, words, b, i1);
+  const int warp = threadIdx.x >> 5, r0 = first + quad, r1 = r0 + 8;
+  auto token = [&](int r) { return pos && r < n ? pos[r] : r; };
+  auto kept = [&](int r) { return r < n && (pos || token_valid(bits, words, b, r)); };
+  const int i0 = token(r0), i1 = token(r1);
+  const bool on0 = kept(r0), on1 = kept(r1);
   const float* lse = a.lse + ((size_t)b * p.Hq + h) * p.T;
   const float z0 = on0 ? -lse[i0] * kLog2e : -CUDART_INF_F;
   const float z1 = on1 ? -lse[i1] * kLog2e : -CUDART_INF_F;
@@ -637,14 +642,14 @@ __device__ __forceinline__ void exact_delta_rows(const AttnProblem& p, const Att
   const int kv = h / (p.Hq / p.Hkv);
   const size_t kb = (size_t)b * a.sk.b + (size_t)kv * a.sk.h;
   const size_t vb = (size_t)b * a.sv.b + (size_t)kv * a.sv.h;
-  const int keys = first >= p.T ? 0 : p.causal ? min(p.T, first + 16) : p.T;
+  const int keys = first >= n ? 0 : p.causal ? min(n, first + 16) : n;
   const float sl = p.sc * kLog2e;
   float d0 = 0.f, d1 = 0.f;
   for (int j = warp * 8; j < keys; j += 64) {
-    const int row = j + quad;
+    const int row = token(j + quad);
     uint4 k[NC], v[NC];
-    load_fragment_row(k, a.k, kb + (size_t)row * a.sk.t, row < p.T, p.D);
-    load_fragment_row(v, a.v, vb + (size_t)row * a.sv.t, row < p.T, p.D);
+    load_fragment_row(k, a.k, kb + (size_t)row * a.sk.t, j + quad < n, p.D);
+    load_fragment_row(v, a.v, vb + (size_t)row * a.sv.t, j + quad < n, p.D);
     float s[4] = {}, x[4] = {};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -656,47 +661,66 @@ __device__ __forceinline__ void exact_delta_rows(const AttnProblem& p, const Att
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int col = j + 2 * (lane & 3) + e;
-      if (col < p.T && token_valid(bits, words, b, col)) {
-        if (on0 && (!p.causal || col <= i0)) d0 = fmaf(exp2f(fmaf(s[e], sl, z0)), x[e], d0);
-        if (on1 && (!p.causal || col <= i1)) d1 = fmaf(exp2f(fmaf(s[e + 2], sl, z1)), x[e + 2], d1);
+      if (kept(col)) {
+        if (on0 && (!p.causal || col <= r0)) d0 = fmaf(exp2f(fmaf(s[e], sl, z0)), x[e], d0);
+        if (on1 && (!p.causal || col <= r1)) d1 = fmaf(exp2f(fmaf(s[e + 2], sl, z1)), x[e + 2], d1);
       }
     }
+    __syncwarp();   // the next step's products take the whole warp
   }
   for (int o = 1; o < 4; o <<= 1) {
     d0 += __shfl_xor_sync(0xffffffffu, d0, o);
     d1 += __shfl_xor_sync(0xffffffffu, d1, o);
   }
+  // by position, the tile's rows past T are set too: the dk/dv launch reads whole tiles
+  auto at = [&](int i) { return stats + (size_t)(i / kBM) * 2 * kBM + i % kBM; };
   if ((lane & 3) == 0) {
     part[warp][quad] = d0;
     part[warp][quad + 8] = d1;
     if (warp == 0) {
-      dst[quad] = z0;
-      dst[quad + 8] = z1;
+      if (!pos || on0) *at(i0) = z0;
+      if (!pos || on1) *at(i1) = z1;
     }
   }
   __syncthreads();
-  if (threadIdx.x < 16) {
+  if (threadIdx.x < 16 && (!pos || first + (int)threadIdx.x < n)) {
     float d = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) d += part[w][threadIdx.x];
-    dst[kBM + threadIdx.x] = d;
+    at(token(first + threadIdx.x))[kBM] = d;
   }
 }
 
-// Query tiles that see at most kExactDeltaKeys keys, the first of a head
-__host__ __device__ __forceinline__ int exact_delta_tiles(const AttnProblem& p) {
+// Query tiles that are known by position to see at most kExactDeltaKeys keys, the first of
+// a head.  None where they are found by rank: those rows replace what the launch below wrote.
+__host__ __device__ __forceinline__ int exact_delta_tiles(const AttnProblem& p, bool ranked) {
   const int n_t = (p.T + kBM - 1) / kBM;
-  return p.T <= kExactDeltaKeys ? n_t : p.causal ? kExactDeltaKeys / kBM : 0;
+  return ranked ? 0 : p.T <= kExactDeltaKeys ? n_t : p.causal ? kExactDeltaKeys / kBM : 0;
 }
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256, 2)
 attn_sm100_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
                               const uint32_t* __restrict__ bits, float* __restrict__ stats) {
-  const int n_t = (p.T + kBM - 1) / kBM, units = exact_delta_tiles(p) * (kBM / 16);
+  const int n_t = (p.T + kBM - 1) / kBM, units = exact_delta_tiles(p, false) * (kBM / 16);
   const int bh = blockIdx.x / units, first = blockIdx.x % units * 16;
-  exact_delta_rows<D, BF16>(p, a, bits, bh / p.Hq, bh % p.Hq, first,
-                            stats + ((size_t)bh * n_t + first / kBM) * 2 * kBM + first % kBM);
+  exact_delta_rows<D, BF16>(p, a, bits, bh / p.Hq, bh % p.Hq, first, nullptr, p.T,
+                            stats + (size_t)bh * n_t * 2 * kBM);
+}
+
+// The rows found by rank; a block takes 16 of a head's up to kExactDeltaKeys.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256, 2)
+attn_sm100_exact_delta_ranked_kernel(const AttnProblem p, const AttnTensors a,
+                                     const uint32_t* __restrict__ bits,
+                                     float* __restrict__ stats) {
+  constexpr int kUnits = kExactDeltaKeys / 16;
+  __shared__ int pos[kExactDeltaKeys], sums[8];
+  const int bh = blockIdx.x / kUnits, first = blockIdx.x % kUnits * 16, b = bh / p.Hq;
+  const int n = few_key_tokens(bits, p, b, pos, sums);
+  if (first >= n) return;
+  exact_delta_rows<D, BF16>(p, a, bits, b, bh % p.Hq, first, pos, n,
+                            stats + (size_t)bh * ((p.T + kBM - 1) / kBM) * 2 * kBM);
 }
 
 // The other tiles, one a block: delta_i = dout_i . out_i, D / 8 neighbouring lanes a row.
@@ -705,8 +729,8 @@ attn_sm100_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
 // few warps to read with: both in one launch took 34 us there.
 __global__ void __launch_bounds__(256)
 attn_sm100_delta_kernel(const AttnProblem p, const AttnTensors a,
-                        const uint32_t* __restrict__ bits, float* __restrict__ stats) {
-  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5, few = exact_delta_tiles(p);
+                        const uint32_t* __restrict__ bits, float* __restrict__ stats, int few) {
+  const int n_t = (p.T + kBM - 1) / kBM, words = (p.T + 31) >> 5;
   const int bh = blockIdx.x / (n_t - few), qt = few + blockIdx.x % (n_t - few);
   const int b = bh / p.Hq, h = bh % p.Hq, lanes = p.D / 8, sub = threadIdx.x % lanes;
   float* dst = stats + ((size_t)bh * n_t + qt) * 2 * kBM;
@@ -1515,12 +1539,16 @@ cudaError_t run_attn_backward(const AttnProblem& p, const AttnTensors& t, const 
       (e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
     return e;
   const int n_t = (p.T + kBM - 1) / kBM, G = p.Hq / p.Hkv, groups = p.B * p.Hkv;
-  const int few = exact_delta_tiles(p), heads = p.B * p.Hq;
+  const bool ranked = exact_delta_ranked(p, bits);
+  const int few = exact_delta_tiles(p, ranked), heads = p.B * p.Hq;
   if (few > 0)
     attn_sm100_exact_delta_kernel<D, BF16>
         <<<heads * few * (kBM / 16), 256, 0, st>>>(p, t, bits, stats);
   if (n_t > few)
-    attn_sm100_delta_kernel<<<heads * (n_t - few), 256, 0, st>>>(p, t, bits, stats);
+    attn_sm100_delta_kernel<<<heads * (n_t - few), 256, 0, st>>>(p, t, bits, stats, few);
+  if (ranked)
+    attn_sm100_exact_delta_ranked_kernel<D, BF16>
+        <<<heads * (kExactDeltaKeys / 16), 256, 0, st>>>(p, t, bits, stats);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const long long group_bytes = 4ll * G * p.T * p.D;   // queries and dO
   for (int g0 = 0; g0 < groups; g0 += plan.per)

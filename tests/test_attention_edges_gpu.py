@@ -3,6 +3,8 @@ few keys, memory orders, shared key tiles of every head dim."""
 import pytest
 import torch
 
+from linearard_b200.attention import attn_backward, attn_forward
+from operator_refs import assert_within
 from test_attention_gpu import check, make, right_pad
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +30,67 @@ def test_shared_key_tiles_of_every_head_dim(D, Hq, Hkv, causal, mask):
     last tile ends inside a warp."""
     q, k, v, g = make(1, Hq, Hkv, 4300, D, "bf16")
     check(q, k, v, g, right_pad(1, 4300, [4111]) if mask else None, causal)
+
+
+def sees_few(m, causal):
+    """[B, T] bool: kept rows that see at most 256 keys."""
+    seen = m.cumsum(1) if causal else m.sum(1, keepdim=True).expand_as(m)
+    return m & (seen <= 256)
+
+
+@pytest.mark.parametrize("kind", ["left", "short", "holes", "right"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("T,D", [(300, 64), (700, 16), (700, 128), (1100, 256), (9000, 32)])
+def test_rows_of_few_keys_under_a_mask(kind, causal, T, D):
+    """What decides is how many keys a row sees, not where it stands: rows of at most 256
+    keys take delta from the probabilities, so that their dq holds no more than the
+    roundings of dS and of the result, and so does dk where every row is one of them."""
+    B, H, Hkv = 3, 4, 2
+    # scores of a few units: the bound on their fp32 sums stays below what a rounded out costs
+    q, k, v, g = make(B, H, Hkv, T, D, "bf16", seed=T, scale=1.1)
+    m = torch.zeros(B, T, dtype=torch.bool, device="cuda")
+    for b, n in enumerate((2, 200, T - 20)):
+        if kind == "left":
+            m[b, T - n:] = True
+        elif kind == "holes":
+            m[b, torch.randperm(T, device="cuda", generator=torch.Generator("cuda").manual_seed(b))[:n]] = True
+        elif kind == "short":        # a short sequence behind a page of padding
+            m[b, T // 3:T // 3 + min(n, 9 + 100 * b)] = True
+        else:
+            m[b, :n] = True
+    out, lse = attn_forward(q, k, v, m, causal)
+    dq, dk, _ = attn_backward(g, q, k, v, out, lse, m, causal)
+    u = 2.0 ** -8
+    few = sees_few(m, causal)
+    for b in range(B):
+        rows = few[b].nonzero()[:, 0]
+        n = len(rows)
+        if n == 0:
+            continue
+        qq, gg = q[b][:, rows].double(), g[b][:, rows].double()
+        kk, vv = (t[b][:, rows].double().repeat_interleave(H // Hkv, 0) for t in (k, v))
+        keep = torch.ones(n, n, dtype=torch.bool, device="cuda")
+        keep = keep.tril() if causal else keep
+        P = ((qq @ kk.transpose(-1, -2)) * D ** -0.5).masked_fill(~keep, -torch.inf).softmax(-1)
+        dP = gg @ vv.transpose(-1, -2)
+        dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+        # fp32: the sums of D products behind S (twice: for delta and for dS) and dP, of n
+        # products behind delta and the results, on terms of size P |dout||v|
+        c = (2 * D + 2 * n) * 2.0 ** -24
+        mag = gg.abs() @ vv.abs().transpose(-1, -2)
+        size = (qq.abs() @ kk.abs().transpose(-1, -2)) * D ** -0.5
+        top = torch.where(keep, size, 0.0).amax(-1, keepdim=True)
+        tol = torch.where(keep, u * dS.abs() + P * (mag + (P * mag).sum(-1, keepdim=True))
+                          * (c * (2 + 2 * top) + 2.0 ** -18), 0.0) + 2.0 ** -126
+        sc = D ** -0.5
+        want = sc * dS @ kk
+        assert_within(dq[b][:, rows], want, sc * tol @ kk.abs() * (1 + u) + u * want.abs() + 1e-30,
+                      f"dq of sequence {b}")
+        if n == int(m[b].sum()):
+            def heads(x):
+                return x.view(Hkv, H // Hkv, n, D).sum(1)
+            want = heads(sc * dS.transpose(-1, -2) @ qq)
+            tol = heads(sc * tol.transpose(-1, -2) @ qq.abs()) * (1 + u) + u * want.abs() + 1e-30
+            assert_within(dk[b][:, rows], want, tol, f"dk of sequence {b}")
+    if T < 9000:                 # the whole result, in [T, T] maps of 64 bits
+        check(q, k, v, g, m, causal)
