@@ -398,8 +398,9 @@ int32_t lkl_token_logprobs(const void* logits, const lkl_logits* l, const int64_
 
 /* d_logits[j] = g (1[j = target] - p_j) - h p_j (log p_j + entropy), g =
  * d_logprob (0 for an ignored target, NaN for one outside [0, V)), h =
- * d_entropy; NULL means 0.  d_logits: contiguous [B, T, V] of the logits' type,
- * not the logits themselves (LKL_ERR_BAD_ALIAS). */
+ * d_entropy; NULL means 0.  A row whose target is ignored and whose d_entropy is
+ * 0 gets zeros, whatever its logits hold.  d_logits: contiguous [B, T, V] of the
+ * logits' type, not the logits themselves (LKL_ERR_BAD_ALIAS). */
 int32_t lkl_token_logprobs_backward(const void* logits, const lkl_logits* l,
                                     const int64_t* targets, int64_t ignore_index,
                                     const float* lse, const float* entropy,

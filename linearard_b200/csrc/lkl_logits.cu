@@ -807,6 +807,16 @@ struct LoadOne {
   }
 };
 
+// A row without gradient: zeros, with nothing read.
+struct Nothing {
+  __device__ __forceinline__ int operator()(long long) const { return 0; }
+  __device__ __forceinline__ int one(long long) const { return 0; }
+};
+template <typename T>
+__device__ __forceinline__ void zero_row(T* out, long long V, int share) {
+  map_row<T>(out, out, V, share, Nothing{}, [](int, int, long long) { return 0.f; });
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kGThreadsL)
 token_logprobs_backward_kernel(const LogitsView view, const int64_t* __restrict__ targets,
@@ -814,14 +824,20 @@ token_logprobs_backward_kernel(const LogitsView view, const int64_t* __restrict_
                                const float* __restrict__ entropy, const float* __restrict__ g_lp,
                                const float* __restrict__ g_en, T* __restrict__ dx, int shares) {
   const long long row = blockIdx.x / shares;
+  const int share = (int)(blockIdx.x % shares);
   const T* x = row_ptr<T>(view, row);
+  T* out = dx + row * view.V;
   const int64_t y = targets[row];
   float g = g_lp && y != ignore ? g_lp[row] : 0.f;
   if (g_lp && y != ignore && (y < 0 || y >= view.V)) g = CUDART_NAN_F;
   const float h = g_en ? g_en[row] : 0.f, z = lse[row], H = entropy[row];
+  if (y == ignore && h == 0.f) {   // whatever its logits hold: 0 x NaN is not 0
+    zero_row(out, view.V, share);
+    return;
+  }
   // -p (g + h (log p + H)) + g at the target
   const float gh = fmaf(h, H, g);
-  map_row<T>(x, dx + row * view.V, view.V, (int)(blockIdx.x % shares), LoadOne<T>{x},
+  map_row<T>(x, out, view.V, share, LoadOne<T>{x},
              [&](const uint4& v, int e, long long at) {
                // e^-200 is 0; 0 x -inf would not be
                const float lp = max_nan(Elem<T>::get(v, e) - z, -200.f);
@@ -856,11 +872,7 @@ logits_kl_backward_kernel(const LogitsView sv, const LogitsView tv, const void* 
   const T *s = row_ptr<T>(sv, row), *t = row_ptr<T>(tv, row);
   T* out = ds + row * sv.V;
   if (mask && !mask_elem(mask, row, mdt)) {
-    struct Nothing {
-      __device__ __forceinline__ int operator()(long long) const { return 0; }
-      __device__ __forceinline__ int one(long long) const { return 0; }
-    };
-    map_row<T>(out, out, sv.V, share, Nothing{}, [](int, int, long long) { return 0.f; });
+    zero_row(out, sv.V, share);
     return;
   }
   // the log probability first: a likely token's exponent is small and keeps its bits
