@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from linearard_b200.logits import logits_kl_align, logits_kl_forward, token_logprobs
-from operator_refs import TokenRef, assert_within
+from operator_refs import KLRef, assert_within
 from test_logits_gpu import logits
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +32,40 @@ def test_rows_without_a_target_have_no_gradient_whatever_they_hold(dtype, V, poi
     got, want = grad(x), grad(clean)
     assert (got[ids == -100] == 0).all()
     assert torch.equal(got[ids != -100], want[ids != -100])
+
+
+@pytest.mark.parametrize("rows,V", [(3, 7), (5, 1003), (2, 40000), (700, 9001), (2000, 32000)])
+@pytest.mark.parametrize("tau", [1.0, 1.7])
+@pytest.mark.parametrize("offsets", [(1024.0, 0.0), (-512.0, 1024.0), (100.0, 100.0)])
+def test_kl_loss_does_not_see_a_rows_offset(rows, V, tau, offsets):
+    """A constant added to a row changes no distribution.  The logits are multiples of 2^-9
+    below 64, so that the sums are exact and so are all differences from a row's maximum:
+    the loss keeps its bits."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    t = (torch.randn(rows, V, device="cuda", generator=g) * 2).mul(512).round().div(512)
+    s = t + (torch.randn(rows, V, device="cuda", generator=g) * 0.1).mul(512).round().div(512)
+    want = logits_kl_forward(s, t, temperature=tau)[0]
+    got = logits_kl_forward(s + offsets[0], t + offsets[1], temperature=tau)[0]
+    assert torch.equal((s + offsets[0]) - offsets[0], s) and torch.equal((t + offsets[1]) - offsets[1], t)
+    assert torch.equal(got, want)
+    ref = KLRef(s, t, None, tau)
+    assert_within(got, ref.loss, ref.loss_tol, "loss")
+
+
+def test_kl_masked_vocabulary():
+    """Entries that both models exclude by the type's lowest number, or by -inf, add nothing,
+    wherever they stand; neither does a run of them before the first real logit."""
+    for low in (torch.finfo(torch.float32).min, -torch.inf):
+        t, s = logits(4, 9000, dtype="fp32", seed=1), logits(4, 9000, dtype="fp32", seed=2)
+        kept = KLRef(s[:, 6000:], t[:, 6000:])
+        s[:, :6000] = t[:, :6000] = low
+        leaf = s.clone().requires_grad_(True)
+        loss = logits_kl_align(leaf, t)
+        tol = KLRef(s, t).loss_tol
+        assert_within(loss, kept.loss, tol, "loss")
+        d = torch.autograd.grad(loss, leaf)[0]
+        assert (d[:, :6000] == 0).all() and torch.isfinite(d).all()
+        # the teacher alone excludes them
+        s[:, :6000] = logits(4, 6000, dtype="fp32", seed=3)
+        ref = KLRef(s, t)
+        assert_within(logits_kl_forward(s, t)[0], ref.loss, ref.loss_tol, "loss")
