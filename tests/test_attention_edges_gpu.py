@@ -3,7 +3,7 @@ few keys, memory orders, shared key tiles of every head dim."""
 import pytest
 import torch
 
-from linearard_b200.attention import attn_backward, attn_forward
+from linearard_b200.attention import attn, attn_backward, attn_forward
 from operator_refs import assert_within
 from test_attention_gpu import check, make, right_pad
 
@@ -94,3 +94,26 @@ def test_rows_of_few_keys_under_a_mask(kind, causal, T, D):
             assert_within(dk[b][:, rows], want, tol, f"dk of sequence {b}")
     if T < 9000:                 # the whole result, in [T, T] maps of 64 bits
         check(q, k, v, g, m, causal)
+
+
+@pytest.mark.parametrize("layout", ["bhtd", "bthd", "fused", "odd"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_results_follow_the_memory_order_of_their_tensors(layout, D):
+    """out in the order of heads and tokens of q; dq, dk and dv in that of q, k and v."""
+    B, Hq, Hkv, T = 2, 4, 2, 150
+    q, k, v, g = make(B, Hq, Hkv, T, D, "bf16", layout)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    auto = attn(*leaves)
+    out, lse = attn_forward(q, k, v)
+
+    def order(H):
+        return (T * H * D, D, H * D, 1) if layout in ("bthd", "fused") else (H * T * D, T * D, D, 1)
+    assert out.stride() == auto.stride() == order(Hq)
+    for d, H in zip(attn_backward(g, q, k, v, out, lse), (Hq, Hkv, Hkv)):
+        assert d.stride() == order(H)
+    for d, H in zip(torch.autograd.grad(auto, leaves, g), (Hq, Hkv, Hkv)):
+        assert d.stride() == order(H)
+    # tensors of different orders at once: each keeps its own
+    mixed = attn_backward(g, q, k.contiguous(), v, out, lse)
+    assert mixed[0].stride() == order(Hq) and mixed[2].stride() == order(Hkv)
+    assert mixed[1].is_contiguous()

@@ -69,3 +69,17 @@ def test_kl_masked_vocabulary():
         s[:, :6000] = logits(4, 6000, dtype="fp32", seed=3)
         ref = KLRef(s, t)
         assert_within(logits_kl_forward(s, t)[0], ref.loss, ref.loss_tol, "loss")
+
+
+def test_token_outputs_changed_in_place():
+    x = logits(3, 4, 1003)
+    ids = torch.arange(12, device="cuda").view(3, 4)
+    keep = (ids % 3 != 0)
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, ids)
+    want = torch.autograd.grad((r.logprob * 2 * keep).sum() + r.entropy.sum(), leaf)[0]
+    r = token_logprobs(leaf, ids)
+    entropy = r.entropy.detach().clone()
+    loss = r.logprob.mul_(2.0).masked_fill_(~keep, 0.0).sum() + r.entropy.sum()
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+    assert torch.equal(r.entropy.detach(), entropy)
