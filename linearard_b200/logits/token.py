@@ -100,7 +100,8 @@ def token_logprobs(logits, targets, top_k=0, ignore_index=-100) -> TokenLogprobs
     assert targets.shape == logits.shape[:-1], "targets shape must be that of the logits' rows"
     assert isinstance(top_k, int) and 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]), \
         "top_k must be from 0 to min(V, 32)"
-    assert isinstance(ignore_index, int), "ignore_index must be an integer"
+    assert isinstance(ignore_index, int) and -2 ** 63 <= ignore_index < 2 ** 63, \
+        "ignore_index must be an integer of 64 bits"
     rows, targets = rows_of(logits), targets.contiguous()
     # a dual tensor does not require grad: the function refuses it, its tangent is not lost
     if (logits.requires_grad and torch.is_grad_enabled()

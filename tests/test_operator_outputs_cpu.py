@@ -57,3 +57,14 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
             token.token_logprobs(fwad.make_dual(x, torch.ones_like(x)), ids)
         token.token_logprobs(x, ids)
     token.token_logprobs(x, ids)
+
+
+def test_ignore_index_beyond_64_bits_is_refused(monkeypatch):
+    """It would wrap into another number on its way to the kernel: 2^64 - 100 into -100."""
+    monkeypatch.setattr(token, "check_logits", lambda x: None)
+    x, ids = torch.randn(3, 5), torch.zeros(3, dtype=torch.int64)
+    for n in (2 ** 64 - 100, 2 ** 63, -2 ** 63 - 1):
+        with pytest.raises(AssertionError, match="ignore_index"):
+            token.token_logprobs(x, ids, ignore_index=n)
+    for n in (2 ** 63 - 1, -2 ** 63, 0):
+        token.token_logprobs(x, ids, ignore_index=n)
