@@ -322,16 +322,16 @@ int32_t lkl_forward_noalloc(const void* qs, const void* ks, const void* qt, cons
  * order of its index below, each with a d stride of 1; NULL: all contiguous
  * [B, H, T, D].  Input strides may be any non-negative number (0 where a
  * tensor is broadcast), output strides are positive.  Head dims 8, 16, 32, 64
- * and 128 run on the tensor cores when every pointer is 16-byte aligned and
- * every stride a positive multiple of 8 elements; everything else runs on
- * CUDA-core kernels.  lkl_last_path() tells which.  An output may not start
- * where an input does.
+ * and 128 run on the tensor cores when every pointer is 16-byte aligned,
+ * every stride a positive multiple of 8 elements and T D above 512; everything
+ * else runs on CUDA-core kernels.  lkl_last_path() tells which.  An output may
+ * not start where an input does.
  * Sums and softmax statistics are fp32, so a probability carries 2^-23 of its
  * score's size (sm_scale q . k): scores beyond some 2^20 are not told apart.
- * P and dS are rounded to the tensors'
- * type before their products on the tensor cores (in fp16 a dS beyond 65504
- * overflows: scale the loss so that dout . v stays below).  Results are reproducible
- * bit for bit: every output row has one writer.
+ * P and dS are rounded to the tensors' type before their products on the tensor
+ * cores (in fp16 a dS beyond 65504 overflows: scale the loss so that dout . v
+ * stays below); on the CUDA cores they stay fp32.  Results are reproducible bit
+ * for bit: every output row has one writer.
  * May be captured into CUDA graphs. */
 typedef struct lkl_attn_problem {
   int32_t B, Hq, Hkv, T, D;

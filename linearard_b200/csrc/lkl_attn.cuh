@@ -80,7 +80,14 @@ cudaError_t launch_attn_generic_backward(const AttnProblem& p, const AttnTensors
                                          cudaStream_t st);
 
 // Tensor-core kernels: head dims up to 128, 16-byte aligned pointers, strides
-// that are positive multiples of 8 elements.
+// that are positive multiples of 8 elements, and more elements a head than this.  Up to it
+// the CUDA-core kernels take a head in one or two 32-row tiles, and keep P and dS in fp32:
+// dq and dk carry their own rounding alone (bf16 0.0017 of their size off instead of 0.0024;
+// in a handful of tokens up to 0.0028).  Forward / backward of 2 and of 2048 heads,
+// CUDA cores against tensor cores, us on the device: D 16, T 32: 4.9 / 16 against 5.5 / 13,
+// 19 / 71 against 60 / 168; D 64, T 8: 6.0 / 21 against 5.4 / 13, 30 / 109 against 60 / 162.
+// D 64, T 32 would take 10 / 39 against 5.6 / 13, 55 / 217 against 61 / 180.
+constexpr int kAttnFewElements = 512;
 bool attn_sm100_supports(const AttnProblem& p, const AttnTensors& t);
 cudaError_t launch_attn_sm100_forward(const AttnProblem& p, const AttnTensors& t,
                                       const uint32_t* bits, cudaStream_t st);

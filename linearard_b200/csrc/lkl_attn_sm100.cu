@@ -1590,8 +1590,8 @@ bool attn_readable(const void* x, const TensorStrides& s) {
 }  // namespace
 
 bool attn_sm100_supports(const AttnProblem& p, const AttnTensors& t) {
-  return p.D <= 128 && attn_readable(t.q, t.sq) && attn_readable(t.k, t.sk) &&
-         attn_readable(t.v, t.sv) && attn_readable(t.out, t.so);
+  return p.D <= 128 && (long long)p.T * p.D > kAttnFewElements && attn_readable(t.q, t.sq) &&
+         attn_readable(t.k, t.sk) && attn_readable(t.v, t.sv) && attn_readable(t.out, t.so);
 }
 
 bool attn_sm100_backward_supports(const AttnProblem& p, const AttnTensors& t) {

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from linearard_b200.attention import attn, attn_backward, attn_forward
-from operator_refs import assert_within
+from operator_refs import AttnRef, assert_within
 from test_attention_gpu import check, make, right_pad
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +117,24 @@ def test_results_follow_the_memory_order_of_their_tensors(layout, D):
     mixed = attn_backward(g, q, k.contiguous(), v, out, lse)
     assert mixed[0].stride() == order(Hq) and mixed[2].stride() == order(Hkv)
     assert mixed[1].is_contiguous()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("T,D", [(1, 128), (4, 128), (2, 64), (8, 64), (7, 32), (16, 32), (8, 16),
+                                 (32, 16), (64, 8)])
+@pytest.mark.parametrize("mask", [False, True])
+def test_sequences_of_few_elements_carry_their_results_rounding_alone(dtype, causal, T, D, mask):
+    """Up to 512 elements a head everything before the results is fp32: the bounds are those
+    of 32-bit inputs and half a step of each result."""
+    q, k, v, g = make(3, 4, 2, T, D, dtype, seed=T + D)
+    m = right_pad(3, T, [T, max(1, T // 2), max(1, T - 1)]) if mask else None
+    ref = AttnRef(*(t.float() for t in (q, k, v)), m, causal, None, g.float())
+    out, lse = attn_forward(q, k, v, m, causal)
+    grads = attn_backward(g, q, k, v, out, lse, m, causal)
+    u, tiny = (2.0 ** -11, 2.0 ** -25) if dtype == "fp16" else (2.0 ** -8, 2.0 ** -133)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        want = getattr(ref, name)
+        tol = getattr(ref, name + "_tol") * (1 + u) + u * want.abs() + tiny
+        assert_within(got, want, tol, name)
+    assert_within(lse, ref.lse, ref.lse_tol, "lse")
