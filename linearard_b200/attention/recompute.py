@@ -28,6 +28,9 @@ from ..attention_KL._common import (_DT, _MASK_DT, SUPPORTED_HEAD_DIMS, TC_HEAD_
 
 __all__ = ["attn", "attn_forward", "attn_backward", "AttnFn"]
 
+# element strides (b, h, t) of the tensors of a call, in the library's order
+_Strides4, _Strides8 = ctypes.c_int64 * 12, ctypes.c_int64 * 24
+
 
 def _check(q, k, v):
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -64,27 +67,28 @@ def _strides(t):
 def _readable(t):
     """(tensor, strides): t itself, or a contiguous copy where the tensor-core
     kernels cannot read it in place (the CUDA-core ones could, many times slower)."""
-    s = _strides(t)
-    unit = t.stride(3) == 1
-    if t.shape[3] in TC_HEAD_DIMS:
-        b, h, n = s
-        unit = (unit and b > 0 and h > 0 and n > 0 and (b | h | n) % 8 == 0
-                and t.data_ptr() % 16 == 0)
-    if unit:
-        return t, s
+    b, h, n, unit = t.stride()
+    B, H, T, D = t.shape
+    b, h, n = b if B != 1 else D, h if H != 1 else D, n if T != 1 else D    # as in _strides
+    if unit == 1 and (D not in TC_HEAD_DIMS or (b > 0 and h > 0 and n > 0 and not (b | h | n) % 8
+                                                and not t.data_ptr() % 16)):
+        return t, (b, h, n)
     t = t.clone(memory_format=torch.contiguous_format)
     return t, _strides(t)
 
 
 def _like(t):
-    """An uninitialised tensor of t's shape and type, in its order of heads and tokens."""
+    """(tensor, strides): uninitialised, of t's shape and type, in its order of heads
+    and tokens."""
     B, H, T, D = t.shape
     s = t.stride()
-    if s == (H * T * D, T * D, D, 1) or s == (T * H * D, D, H * D, 1):
-        return torch.empty_like(t)      # dense: keeps the strides
+    n = H * T * D
+    if s == (n, T * D, D, 1) or s == (n, D, H * D, 1):
+        return torch.empty_like(t), s[:3]      # dense: keeps the strides
     if s[1] < s[2]:
-        return torch.empty((B, T, H, D), device=t.device, dtype=t.dtype).transpose(1, 2)
-    return torch.empty((B, H, T, D), device=t.device, dtype=t.dtype)
+        return (torch.empty((B, T, H, D), device=t.device, dtype=t.dtype).transpose(1, 2),
+                (n, D, H * D))
+    return torch.empty((B, H, T, D), device=t.device, dtype=t.dtype), (n, T * D, D)
 
 
 def _workspace(n, device):
@@ -100,7 +104,7 @@ def _forward(q, k, v, mask, prob):
     L, dev = _lib.lib(), q.device
     with on_device(dev):
         (rq, sq), (rk, sk), (rv, sv) = _readable(q), _readable(k), _readable(v)
-        out = _like(rq)
+        out, so = _like(rq)
         lse = torch.empty((prob.B, prob.Hq, prob.T), device=dev, dtype=torch.float32)
         ref = ctypes.byref(prob)
         n, ws, at, m = 0, None, None, None
@@ -108,7 +112,7 @@ def _forward(q, k, v, mask, prob):
             n, m = L.lkl_attn_forward_workspace_size(ref, 1), mask.data_ptr()
             ws, at = _workspace(n, dev)
         st = L.lkl_attn_forward(rq.data_ptr(), rk.data_ptr(), rv.data_ptr(),
-                                (ctypes.c_int64 * 12)(*sq, *sk, *sv, *_strides(out)), m, ref,
+                                _Strides4(*sq, *sk, *sv, *so), m, ref,
                                 out.data_ptr(), lse.data_ptr(), at, n, raw_stream(dev))
     _lib.check(st, "lkl_attn_forward")
     return out, lse
@@ -117,7 +121,7 @@ def _forward(q, k, v, mask, prob):
 def _backward(dout, q, k, v, out, lse, mask, prob):
     L, dev = _lib.lib(), q.device
     with on_device(dev):
-        dq, dk, dv = _like(q), _like(k), _like(v)
+        (dq, sdq), (dk, sdk), (dv, sdv) = _like(q), _like(k), _like(v)
         (q, sq), (k, sk), (v, sv), (out, so) = (_readable(t) for t in (q, k, v, out))
         dout, sd = _readable(dout)
         ref = ctypes.byref(prob)
@@ -125,8 +129,7 @@ def _backward(dout, q, k, v, out, lse, mask, prob):
         ws, at = _workspace(n, dev)
         st = L.lkl_attn_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            dout.data_ptr(), (ctypes.c_int64 * 24)(*sq, *sk, *sv, *so, *sd, *_strides(dq),
-                                                   *_strides(dk), *_strides(dv)),
+            dout.data_ptr(), _Strides8(*sq, *sk, *sv, *so, *sd, *sdq, *sdk, *sdv),
             None if mask is None else mask.data_ptr(), ref, dq.data_ptr(), dk.data_ptr(),
             dv.data_ptr(), at, n, raw_stream(dev))
     _lib.check(st, "lkl_attn_backward")
@@ -160,17 +163,19 @@ class AttnFn(torch.autograd.Function):
     def forward(ctx, q, k, v, mask, prob):
         out, lse = _forward(q, k, v, mask, prob)
         ctx.save_for_backward(q, k, v, out, lse, mask)
-        ctx.prob = prob
+        ctx.prob, ctx.kv_shape = prob, k.shape
         return out
 
     @once_when_recorded
     def backward(ctx, dout):
         q, k, v, out, lse, mask = ctx.saved_tensors
-        p, dt, dev = ctx.prob, dout.dtype, dout.device
         # strides are read from what came back: a hook may have changed them
-        for t, H in ((q, p.Hq), (k, p.Hkv), (v, p.Hkv), (out, p.Hq)):
-            same_as_saved(t, (p.B, H, p.T, p.D), dt, dev)
-        lse = same_as_saved(lse, (p.B, p.Hq, p.T), torch.float32, dev).contiguous()
+        p, dt, dev, shape, kv = ctx.prob, dout.dtype, dout.device, dout.shape, ctx.kv_shape
+        same_as_saved(q, shape, dt, dev)
+        same_as_saved(k, kv, dt, dev)
+        same_as_saved(v, kv, dt, dev)
+        same_as_saved(out, shape, dt, dev)
+        lse = same_as_saved(lse, shape[:3], torch.float32, dev).contiguous()
         if mask is not None:
             assert _MASK_DT.get(mask.dtype) == p.mask_dtype, "a saved mask came back as another type"
             mask = same_as_saved(mask, (p.B, p.T), mask.dtype, dev).contiguous()

@@ -145,21 +145,20 @@ __global__ void attn_delta_kernel(const AttnProblem p, const AttnTensors a,
   }
 }
 
-// Rows pos[r0 .. r0 + 32) of head h, zeros from rank n on.
-template <int D>
-__device__ __forceinline__ void attn_load_ranked(float* dst, const void* src,
+// Rows token(r0 .. r0 + 32) of head h, zeros where that is -1.
+template <int D, typename Token>
+__device__ __forceinline__ void attn_load_tokens(float* dst, const void* src,
                                                  const TensorStrides& s, int b, int h, int r0,
-                                                 const int* pos, int n, int dtype) {
+                                                 Token token, int dtype) {
   const size_t base = (size_t)b * s.b + (size_t)h * s.h;
   for (int e = threadIdx.x; e < kABM * D; e += kAThreads) {
-    const int r = e / D, d = e % D;
-    dst[r * (D + 1) + d] =
-        r0 + r < n ? load_elem(src, base + (size_t)pos[r0 + r] * s.t + d, dtype) : 0.f;
+    const int r = e / D, d = e % D, t = token(r0 + r);
+    dst[r * (D + 1) + d] = t >= 0 ? load_elem(src, base + (size_t)t * s.t + d, dtype) : 0.f;
   }
 }
 
 // delta_i = sum_j P_ij (dout_i . v_j) for rows that see few keys; a block takes 32.  Rows
-// and keys are ranks among the tokens at pos[]: without a mask the first ones.
+// and keys go by position or, where exact_delta_ranked() says so, by their rank.
 template <int D>
 __global__ void __launch_bounds__(kAThreads)
 attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
@@ -172,39 +171,38 @@ attn_exact_delta_kernel(const AttnProblem p, const AttnTensors a,
   float* sK = sG + kABM * (D + 1);
   float* sV = sK + kABM * (D + 1);
   const int bh = blockIdx.x / n_rt, mt = blockIdx.x % n_rt;   // n_rt: row tiles to take
-  const int b = bh / p.Hq, h = bh % p.Hq, g = h / (p.Hq / p.Hkv);
-  int n = min(p.T, kExactDeltaKeys);
-  if (bits) {
-    n = few_key_tokens(bits, p, b, pos, sums);
-  } else {
-    pos[threadIdx.x] = threadIdx.x;
-    __syncthreads();
-  }
-  const int r = threadIdx.x >> 3, sub = threadIdx.x & 7, rank = mt * kABM + r;
+  const int b = bh / p.Hq, h = bh % p.Hq, g = h / (p.Hq / p.Hkv), words = (p.T + 31) >> 5;
+  const bool ranked = exact_delta_ranked(p, bits);
+  const int n = ranked ? few_key_tokens(bits, p, b, pos, sums) : min(p.T, kExactDeltaKeys);
   if (mt * kABM >= n) return;
-  const bool row = rank < n;
-  const size_t at = (size_t)bh * p.T + (row ? pos[rank] : 0);
-  const float z = row ? -a.lse[at] * kLog2e : -CUDART_INF_F;
-  attn_load_ranked<D>(sQ, a.q, a.sq, b, h, mt * kABM, pos, n, p.dtype);
-  attn_load_ranked<D>(sG, a.dout, a.sdo, b, h, mt * kABM, pos, n, p.dtype);
+  auto token = [&](int r) {   // -1: none there, or one that the mask removes
+    if (r >= n) return -1;
+    return ranked ? pos[r] : token_valid(bits, words, b, r) ? r : -1;
+  };
+  const int r = threadIdx.x >> 3, sub = threadIdx.x & 7, rank = mt * kABM + r, i = token(rank);
+  const float z = i >= 0 ? -a.lse[(size_t)bh * p.T + i] * kLog2e : -CUDART_INF_F;
+  attn_load_tokens<D>(sQ, a.q, a.sq, b, h, mt * kABM, token, p.dtype);
+  attn_load_tokens<D>(sG, a.dout, a.sdo, b, h, mt * kABM, token, p.dtype);
   float delta = 0.f;
   const int n_j = p.causal ? mt + 1 : (n + kABM - 1) / kABM;
   for (int j = 0; j < n_j; ++j) {
     __syncthreads();
-    attn_load_ranked<D>(sK, a.k, a.sk, b, g, j * kABM, pos, n, p.dtype);
-    attn_load_ranked<D>(sV, a.v, a.sv, b, g, j * kABM, pos, n, p.dtype);
+    attn_load_tokens<D>(sK, a.k, a.sk, b, g, j * kABM, token, p.dtype);
+    attn_load_tokens<D>(sV, a.v, a.sv, b, g, j * kABM, token, p.dtype);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int cl = sub + 8 * k, c = j * kABM + cl;
-      if (row && c < n && (!p.causal || c <= rank)) {
+      if (i >= 0 && (!p.causal || c <= rank) && token(c) >= 0) {
         const float s = attn_dot<D>(sQ + r * (D + 1), sK + cl * (D + 1)) * p.sc * kLog2e;
         delta = fmaf(exp2f(s + z), attn_dot<D>(sG + r * (D + 1), sV + cl * (D + 1)), delta);
       }
     }
   }
   delta = sum8(delta);
-  if (sub == 0 && row) rows[at] = make_float2(z, delta);
+  // by position, a removed token's row is written too
+  const int at = ranked ? i : rank < n ? rank : -1;
+  if (sub == 0 && at >= 0) rows[(size_t)bh * p.T + at] = make_float2(z, delta);
 }
 
 // dq_i = sc sum_j P_ij (dout_i . v_j - delta_i) k_j; query rows are stationary.
@@ -323,8 +321,11 @@ attn_generic_dkv_kernel(const AttnProblem p, const AttnTensors a,
 template <typename K, typename... A>
 cudaError_t attn_launch(K kernel, long long grid, int smem, cudaStream_t st, A... args) {
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
+  if (smem > (48 << 10)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
   kernel<<<(int)grid, kAThreads, smem, st>>>(args...);
   return cudaGetLastError();
 }

@@ -205,10 +205,10 @@ int32_t lkl_attn_backward(const void* q, const void* k, const void* v, const voi
         at.ds_bytes,
         reinterpret_cast<float*>(base + at.acc), st));
   float2* rows = reinterpret_cast<float2*>(stats);
-  // every row first, those that the mask removes too; then the rows of few keys
+  // every row of a long sequence first, then those that see few keys
   const bool few = a.T <= lkl::kExactDeltaKeys;
-  if ((bits || !few) && (s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;
-  if ((bits || few || a.causal) &&
+  if (!few && (s = launch_status(lkl::launch_attn_delta(a, t, bits, rows, st)))) return s;
+  if ((few || a.causal || bits) &&
       (s = launch_status(lkl::launch_attn_exact_delta(a, t, bits, rows, st))))
     return s;
   return launch_status(lkl::launch_attn_generic_backward(a, t, bits, rows, st));

@@ -25,10 +25,13 @@ def rows_of(x) -> _lib.LKLLogits:
     return _lib.LKLLogits(*x.shape, *x.stride()[:2], _DT[x.dtype])
 
 
-def saved_rows(x, shape, dtype, device):
+def saved_rows(x, shape, dtype, device, seen):
     """(tensor, its rows) of logits that autograd kept for a backward: the strides are
-    those that it came back with."""
+    those that it came back with.  seen: the forward's (rows, strides)."""
     same_as_saved(x, shape, dtype, device)
-    if x.stride(-1) != 1 and x.shape[-1] != 1:
+    strides = x.stride()
+    if strides == seen[1]:
+        return x, seen[0]
+    if strides[-1] != 1 and shape[-1] != 1:
         x = x.contiguous()
     return x, rows_of(x)

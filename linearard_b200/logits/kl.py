@@ -47,7 +47,8 @@ def _forward(s, t, mask, mdt, temperature, rows):
     dev, shape = s.device, s.shape[:-1]
     L = _lib.lib()
     with on_device(dev):
-        lse_s, lse_t = (torch.empty(shape, device=dev, dtype=torch.float32) for _ in range(2))
+        lse_s = torch.empty(shape, device=dev, dtype=torch.float32)
+        lse_t = torch.empty_like(lse_s)
         loss = torch.empty((), device=dev, dtype=torch.float32)
         rs, rt = ctypes.byref(rows[0]), ctypes.byref(rows[1])
         n = L.lkl_logits_kl_workspace_size(rs)
@@ -107,6 +108,7 @@ class LogitsKLAlignFn(torch.autograd.Function):
         loss, lse_s, lse_t = _forward(s_logits, t_logits, mask, mdt, temperature, rows)
         ctx.save_for_backward(s_logits, t_logits, lse_s, lse_t, mask)
         ctx.mdt, ctx.temperature = mdt, temperature
+        ctx.seen = (rows[0], s_logits.stride()), (rows[1], t_logits.stride())
         ctx.shape, ctx.dtype, ctx.device = s_logits.shape, s_logits.dtype, s_logits.device
         return loss
 
@@ -114,14 +116,14 @@ class LogitsKLAlignFn(torch.autograd.Function):
     def backward(ctx, dloss):
         s_logits, t_logits, lse_s, lse_t, mask = ctx.saved_tensors
         shape, dt, dev = ctx.shape, ctx.dtype, ctx.device
-        lse_s, lse_t = (same_as_saved(t, shape[:-1], torch.float32, dev).contiguous()
-                        for t in (lse_s, lse_t))
+        lse_s = same_as_saved(lse_s, shape[:-1], torch.float32, dev).contiguous()
+        lse_t = same_as_saved(lse_t, shape[:-1], torch.float32, dev).contiguous()
         if mask is not None:
             assert _MASK_DT.get(mask.dtype) == ctx.mdt, "a saved mask came back as another type"
             rows = shape[:-1] if len(shape) == 3 else (1, shape[0])
             mask = same_as_saved(mask, rows, mask.dtype, dev).contiguous()
-        (s_logits, s_rows), (t_logits, t_rows) = (saved_rows(x, shape, dt, dev)
-                                                  for x in (s_logits, t_logits))
+        s_logits, s_rows = saved_rows(s_logits, shape, dt, dev, ctx.seen[0])
+        t_logits, t_rows = saved_rows(t_logits, shape, dt, dev, ctx.seen[1])
         ds = _backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.mdt, ctx.temperature,
                        (s_rows, t_rows), dloss.to(torch.float32))
         return ds, None, None, None, None, None      # the teacher gets no gradient

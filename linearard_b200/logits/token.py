@@ -36,8 +36,8 @@ def _forward(logits, rows, targets, top_k, ignore_index):
     dev, shape = logits.device, targets.shape
     with on_device(dev):
         # tensors of their own: views of one could not be changed in place
-        logprob, entropy, lse = (torch.empty(shape, device=dev, dtype=torch.float32)
-                                 for _ in range(3))
+        logprob = torch.empty(shape, device=dev, dtype=torch.float32)
+        entropy, lse = torch.empty_like(logprob), torch.empty_like(logprob)
         top_v = top_i = None
         if top_k:
             top_v = torch.empty((*shape, top_k), device=dev, dtype=torch.float32)
@@ -58,7 +58,7 @@ class TokenLogprobsFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, targets, lse, entropy)
         ctx.shape, ctx.dtype, ctx.device = logits.shape, logits.dtype, logits.device
-        ctx.ignore_index = ignore_index
+        ctx.seen, ctx.ignore_index = (rows, logits.stride()), ignore_index
         if top_k:
             ctx.mark_non_differentiable(top_v, top_i)
         return logprob, entropy, top_v, top_i
@@ -69,11 +69,11 @@ class TokenLogprobsFn(torch.autograd.Function):
             return None, None, None, None, None
         logits, targets, lse, entropy = ctx.saved_tensors
         dev, shape = ctx.device, ctx.shape[:-1]
-        targets = same_as_saved(targets, shape, torch.int64, dev)
-        lse, entropy = (same_as_saved(t, shape, torch.float32, dev) for t in (lse, entropy))
         with on_device(dev):
-            logits, rows = saved_rows(logits, ctx.shape, ctx.dtype, dev)
-            targets, lse, entropy = (t.contiguous() for t in (targets, lse, entropy))
+            logits, rows = saved_rows(logits, ctx.shape, ctx.dtype, dev, ctx.seen)
+            targets = same_as_saved(targets, shape, torch.int64, dev).contiguous()
+            lse = same_as_saved(lse, shape, torch.float32, dev).contiguous()
+            entropy = same_as_saved(entropy, shape, torch.float32, dev).contiguous()
             g, h = (None if d is None else d.to(torch.float32).contiguous()
                     for d in (d_logprob, d_entropy))
             dx = torch.empty(ctx.shape, device=dev, dtype=ctx.dtype)
