@@ -43,7 +43,7 @@
 extern "C" {
 #endif
 
-#define LKL_ABI_VERSION 7
+#define LKL_ABI_VERSION 8
 
 /* element types of q/k tensors; LKL_F32 for logits only (ABI version 7) */
 enum lkl_dtype { LKL_F16 = 0, LKL_BF16 = 1, LKL_F32 = 2 };
@@ -377,6 +377,11 @@ typedef struct lkl_logits {
   int64_t B, T, V;
   int64_t sb, st;     /* element strides of the batch and token dims            */
   int32_t dtype;      /* lkl_dtype                                              */
+  float* lse_low;     /* fp32 [B, T] or NULL (ABI version 8): what the rounding
+                         of the rows' log-sum-exp to fp32 leaves.  A forward
+                         writes it, its backward takes p from the sum of the
+                         two; without it p carries 2^-24 of the log-sum-exp's
+                         size                                                    */
 } lkl_logits;
 
 #define LKL_MAX_TOP_K 32

@@ -75,7 +75,8 @@ class LKLAttnProblem(ctypes.Structure):
 class LKLLogits(ctypes.Structure):
     """Rows of logits, [B, T, V] with element strides (sb, st, 1) (struct lkl_logits)."""
     _fields_ = [("B", ctypes.c_int64), ("T", ctypes.c_int64), ("V", ctypes.c_int64),
-                ("sb", ctypes.c_int64), ("st", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+                ("sb", ctypes.c_int64), ("st", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("lse_low", ctypes.c_void_p)]
 
 
 class LKLError(RuntimeError):

@@ -5,11 +5,13 @@
 
 namespace lkl {
 
-// Rows of a [B, T, V] tensor with element strides (sb, st, 1).
+// Rows of a [B, T, V] tensor with element strides (sb, st, 1).  low: what the rows'
+// log-sum-exp in fp32 lacks, or nullptr.
 struct LogitsView {
   const void* x;
   long long T, V, sb, st;
   int dtype;
+  float* low;
 };
 
 cudaError_t launch_token_logprobs(const LogitsView& x, long long rows, const int64_t* targets,

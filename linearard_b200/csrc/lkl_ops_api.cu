@@ -94,11 +94,11 @@ int32_t check_logits(const void* x, const lkl_logits* l) {
     return LKL_ERR_TOO_LARGE;
   if (l->B * l->T == 0) return LKL_OK;
   if (!x) return LKL_ERR_NULL_POINTER;
-  return aligned(x, logits_elem(l->dtype)) ? LKL_OK : LKL_ERR_MISALIGNED;
+  return aligned(x, logits_elem(l->dtype)) && aligned(l->lse_low, 4) ? LKL_OK : LKL_ERR_MISALIGNED;
 }
 
 LogitsView to_view(const void* x, const lkl_logits* l) {
-  return LogitsView{x, l->T, l->V, l->sb, l->st, l->dtype};
+  return LogitsView{x, l->T, l->V, l->sb, l->st, l->dtype, l->lse_low};
 }
 
 int32_t check_kl(const void* sx, const lkl_logits* s, const void* tx, const lkl_logits* t,

@@ -43,33 +43,48 @@ def _mask(attn_mask, s):
     return prepare_mask(mask, mask.shape[0], mask.shape[1], s.device)
 
 
-def _forward(s, t, mask, mdt, temperature, rows):
+def _forward(s, t, mask, mdt, temperature, rows, keep=False):
+    """(loss, lse_s, lse_t).  keep: for the backward, one tensor [4, ...] in lse_s: the
+    student's log-sum-exp, what its fp32 value lacks, and the teacher's two."""
     dev, shape = s.device, s.shape[:-1]
     L = _lib.lib()
     with on_device(dev):
-        lse_s = torch.empty(shape, device=dev, dtype=torch.float32)
-        lse_t = torch.empty_like(lse_s)
+        if keep:
+            lse_s, lse_t = torch.empty((4, *shape), device=dev, dtype=torch.float32), None
+            at_s, at_t = _kept(lse_s, rows)
+        else:
+            lse_s = torch.empty(shape, device=dev, dtype=torch.float32)
+            lse_t = torch.empty_like(lse_s)
+            at_s, at_t = lse_s.data_ptr(), lse_t.data_ptr()
         loss = torch.empty((), device=dev, dtype=torch.float32)
         rs, rt = ctypes.byref(rows[0]), ctypes.byref(rows[1])
         n = L.lkl_logits_kl_workspace_size(rs)
         ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
         st = L.lkl_logits_kl_forward(s.data_ptr(), rs, t.data_ptr(), rt,
                                      None if mask is None else mask.data_ptr(), mdt, temperature,
-                                     lse_s.data_ptr(), lse_t.data_ptr(), loss.data_ptr(),
-                                     ws.data_ptr(), n, raw_stream(dev))
+                                     at_s, at_t, loss.data_ptr(), ws.data_ptr(), n,
+                                     raw_stream(dev))
     _lib.check(st, "lkl_logits_kl_forward")
     return loss, lse_s, lse_t
 
 
-def _backward(s, t, lse_s, lse_t, mask, mdt, temperature, rows, dloss):
+def _kept(lse, rows):
+    """Addresses of the two log-sum-exps in a [4, ...] tensor; the rows learn those of
+    what their fp32 values lack."""
+    at, n = lse.data_ptr(), lse.numel()     # a quarter of n elements of 4 bytes each
+    rows[0].lse_low, rows[1].lse_low = at + n, at + 3 * n
+    return at, at + 2 * n
+
+
+def _backward(s, t, at_s, at_t, mask, mdt, temperature, rows, dloss):
+    """at_s, at_t: addresses of the log-sum-exps."""
     dev = s.device
     with on_device(dev):
         ds = torch.empty(s.shape, device=dev, dtype=s.dtype)
         st = _lib.lib().lkl_logits_kl_backward(
             s.data_ptr(), ctypes.byref(rows[0]), t.data_ptr(), ctypes.byref(rows[1]),
-            None if mask is None else mask.data_ptr(), mdt, temperature, lse_s.data_ptr(),
-            lse_t.data_ptr(), None if dloss is None else dloss.data_ptr(), ds.data_ptr(),
-            raw_stream(dev))
+            None if mask is None else mask.data_ptr(), mdt, temperature, at_s, at_t,
+            None if dloss is None else dloss.data_ptr(), ds.data_ptr(), raw_stream(dev))
     _lib.check(st, "lkl_logits_kl_backward")
     return ds
 
@@ -98,15 +113,15 @@ def logits_kl_backward(s_logits, t_logits, lse_s, lse_t, attn_mask=None, tempera
         assert isinstance(dloss, torch.Tensor) and dloss.numel() == 1 and dloss.device == dev \
             and dloss.dtype == torch.float32, "dloss must be a float32 scalar on the device"
     mask, mdt = _mask(attn_mask, s_logits)
-    return _backward(s_logits, t_logits, lse_s, lse_t, mask, mdt, float(temperature),
-                     (rows_of(s_logits), rows_of(t_logits)), dloss)
+    return _backward(s_logits, t_logits, lse_s.data_ptr(), lse_t.data_ptr(), mask, mdt,
+                     float(temperature), (rows_of(s_logits), rows_of(t_logits)), dloss)
 
 
 class LogitsKLAlignFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, s_logits, t_logits, mask, mdt, temperature, rows):
-        loss, lse_s, lse_t = _forward(s_logits, t_logits, mask, mdt, temperature, rows)
-        ctx.save_for_backward(s_logits, t_logits, lse_s, lse_t, mask)
+        loss, lse, _ = _forward(s_logits, t_logits, mask, mdt, temperature, rows, keep=True)
+        ctx.save_for_backward(s_logits, t_logits, lse, mask)
         ctx.mdt, ctx.temperature = mdt, temperature
         ctx.seen = (rows[0], s_logits.stride()), (rows[1], t_logits.stride())
         ctx.shape, ctx.dtype, ctx.device = s_logits.shape, s_logits.dtype, s_logits.device
@@ -114,18 +129,18 @@ class LogitsKLAlignFn(torch.autograd.Function):
 
     @once_when_recorded
     def backward(ctx, dloss):
-        s_logits, t_logits, lse_s, lse_t, mask = ctx.saved_tensors
+        s_logits, t_logits, lse, mask = ctx.saved_tensors
         shape, dt, dev = ctx.shape, ctx.dtype, ctx.device
-        lse_s = same_as_saved(lse_s, shape[:-1], torch.float32, dev).contiguous()
-        lse_t = same_as_saved(lse_t, shape[:-1], torch.float32, dev).contiguous()
+        lse = same_as_saved(lse, (4, *shape[:-1]), torch.float32, dev).contiguous()
         if mask is not None:
             assert _MASK_DT.get(mask.dtype) == ctx.mdt, "a saved mask came back as another type"
             rows = shape[:-1] if len(shape) == 3 else (1, shape[0])
             mask = same_as_saved(mask, rows, mask.dtype, dev).contiguous()
         s_logits, s_rows = saved_rows(s_logits, shape, dt, dev, ctx.seen[0])
         t_logits, t_rows = saved_rows(t_logits, shape, dt, dev, ctx.seen[1])
-        ds = _backward(s_logits, t_logits, lse_s, lse_t, mask, ctx.mdt, ctx.temperature,
-                       (s_rows, t_rows), dloss.to(torch.float32))
+        rows = (s_rows, t_rows)
+        ds = _backward(s_logits, t_logits, *_kept(lse, rows), mask, ctx.mdt, ctx.temperature,
+                       rows, dloss.to(torch.float32))
         return ds, None, None, None, None, None      # the teacher gets no gradient
 
 

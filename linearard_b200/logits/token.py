@@ -31,13 +31,19 @@ class TokenLogprobs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
-def _forward(logits, rows, targets, top_k, ignore_index):
-    """(logprob, entropy, lse, top_logprobs, top_indices) of checked arguments."""
+def _forward(logits, rows, targets, top_k, ignore_index, keep=False):
+    """(logprob, entropy, lse, top_logprobs, top_indices) of checked arguments.
+    keep: lse for the backward, [2, ...]: its fp32 value and what that lacks."""
     dev, shape = logits.device, targets.shape
     with on_device(dev):
         # tensors of their own: views of one could not be changed in place
         logprob = torch.empty(shape, device=dev, dtype=torch.float32)
-        entropy, lse = torch.empty_like(logprob), torch.empty_like(logprob)
+        entropy = torch.empty_like(logprob)
+        if keep:
+            lse = torch.empty((2, *shape), device=dev, dtype=torch.float32)
+            rows.lse_low = lse.data_ptr() + 4 * logprob.numel()
+        else:
+            lse = torch.empty_like(logprob)
         top_v = top_i = None
         if top_k:
             top_v = torch.empty((*shape, top_k), device=dev, dtype=torch.float32)
@@ -54,7 +60,8 @@ def _forward(logits, rows, targets, top_k, ignore_index):
 class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rows, targets, top_k: int, ignore_index: int):
-        logprob, entropy, lse, top_v, top_i = _forward(logits, rows, targets, top_k, ignore_index)
+        logprob, entropy, lse, top_v, top_i = _forward(logits, rows, targets, top_k, ignore_index,
+                                                       keep=True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, targets, lse, entropy)
         ctx.shape, ctx.dtype, ctx.device = logits.shape, logits.dtype, logits.device
@@ -72,7 +79,8 @@ class TokenLogprobsFn(torch.autograd.Function):
         with on_device(dev):
             logits, rows = saved_rows(logits, ctx.shape, ctx.dtype, dev, ctx.seen)
             targets = same_as_saved(targets, shape, torch.int64, dev).contiguous()
-            lse = same_as_saved(lse, shape, torch.float32, dev).contiguous()
+            lse = same_as_saved(lse, (2, *shape), torch.float32, dev).contiguous()
+            rows.lse_low = lse.data_ptr() + 4 * entropy.numel()
             entropy = same_as_saved(entropy, shape, torch.float32, dev).contiguous()
             g, h = (None if d is None else d.to(torch.float32).contiguous()
                     for d in (d_logprob, d_entropy))

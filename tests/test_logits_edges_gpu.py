@@ -83,3 +83,42 @@ def test_token_outputs_changed_in_place():
     loss = r.logprob.mul_(2.0).masked_fill_(~keep, 0.0).sum() + r.entropy.sum()
     assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
     assert torch.equal(r.entropy.detach(), entropy)
+
+
+def grid(*shape, seed=0, scale=2.0):
+    """Multiples of 2^-9 below 64, so that adding 1024 is exact in fp32."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).mul(512).round().div(512)
+
+
+def p_error(x):
+    """How far p may be from itself under an exact offset: the log probability and its
+    multiple by log2(e) are rounded (2^-24 of their size, both times), so is e^ (2^-22)."""
+    lp = torch.log_softmax(x.double(), -1)
+    return lp.exp() * (lp.abs() * 2.0 ** -22 + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("rows,V", [(3, 7), (5, 1003), (40, 40000)])
+@pytest.mark.parametrize("tau", [1.0, 1.7])
+@pytest.mark.parametrize("offset", [1024.0, -512.0])
+def test_gradients_do_not_see_a_rows_offset(rows, V, tau, offset):
+    t, s = grid(rows, V), grid(rows, V, seed=1)
+
+    def kl(s, t):
+        leaf = s.clone().requires_grad_(True)
+        return torch.autograd.grad(logits_kl_align(leaf, t, temperature=tau), leaf)[0].double()
+    want = kl(s, t)
+    tol = (p_error(s / tau) + p_error(t / tau)) / tau + 2.0 ** -22 * want.abs() + 1e-38
+    assert_within(kl(s + offset, t), want, tol, "student shifted")
+    assert_within(kl(s, t + offset), want, tol, "teacher shifted")
+    ids = torch.arange(rows, device="cuda")
+
+    def token(x):
+        leaf = x.clone().requires_grad_(True)
+        r = token_logprobs(leaf, ids)
+        return torch.autograd.grad(r.logprob.sum() + 0.5 * r.entropy.sum(), leaf)[0].double()
+    want = token(s)
+    lp = torch.log_softmax(s.double(), -1)
+    size = 1.0 + 0.5 * (lp.abs() + 12.0)       # |g + h (log p + H)| with H below log V
+    tol = p_error(s) * size + lp.exp() * 2.0 ** -20 * size + 2.0 ** -22 * want.abs() + 1e-38
+    assert_within(token(s + offset), want, tol, "token logits shifted")

@@ -147,6 +147,9 @@ def test_token_backward_reads_what_the_hook_gave_back(recorder, unpack, cut):
     if unpack != "strange":
         for k in (2, 4, 5):          # targets, lse, entropy
             assert any(t.data_ptr() == args[k] and t.is_contiguous() for t in given)
+        n = ids.numel()
+        assert args[1]._obj.lse_low == args[4] + 4 * n
+        assert any(t.data_ptr() == args[4] and t.numel() == 2 * n for t in given)
 
 
 @pytest.mark.parametrize("unpack", UNPACK)
@@ -167,8 +170,11 @@ def test_kl_backward_reads_what_the_hook_gave_back(recorder, unpack, cut, mask):
     check_rows(args, 2, given, tuple(t.shape))
     assert d.shape == s.shape and (args[4] is not None) == mask
     if unpack != "strange":
-        for k in (7, 8):             # the two log-sum-exps
-            assert any(z.data_ptr() == args[k] and z.is_contiguous() for z in given)
+        n = s.shape[0] * s.shape[1]      # the two log-sum-exps, each with what it lacks
+        assert any(z.data_ptr() == args[7] and z.is_contiguous() and z.numel() == 4 * n
+                   for z in given)
+        assert args[8] == args[7] + 8 * n
+        assert args[1]._obj.lse_low == args[7] + 4 * n and args[3]._obj.lse_low == args[8] + 4 * n
 
 
 def test_logits_backward_refuses_other_types_from_a_hook(recorder):
