@@ -381,7 +381,7 @@ typedef struct lkl_logits {
                          of the rows' log-sum-exp to fp32 leaves.  A forward
                          writes it, its backward takes p from the sum of the
                          two; without it p carries 2^-24 of the log-sum-exp's
-                         size                                                    */
+                         size.  An array of its own (LKL_ERR_BAD_ALIAS)          */
 } lkl_logits;
 
 #define LKL_MAX_TOP_K 32

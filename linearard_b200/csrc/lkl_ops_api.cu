@@ -101,6 +101,20 @@ LogitsView to_view(const void* x, const lkl_logits* l) {
   return LogitsView{x, l->T, l->V, l->sb, l->st, l->dtype, l->lse_low};
 }
 
+// What a log-sum-exp lacks stands in an array of its own.
+inline bool low_aliases(const lkl_logits* l, const void* other) {
+  return l->lse_low && l->lse_low == other;
+}
+
+int32_t check_kl_lse(const lkl_logits* s, const lkl_logits* t, const float* lse_s,
+                     const float* lse_t) {
+  if (!lse_s || !lse_t) return LKL_ERR_NULL_POINTER;
+  if (low_aliases(s, t->lse_low) || low_aliases(s, lse_s) || low_aliases(s, lse_t) ||
+      low_aliases(t, lse_s) || low_aliases(t, lse_t))
+    return LKL_ERR_BAD_ALIAS;
+  return LKL_OK;
+}
+
 int32_t check_kl(const void* sx, const lkl_logits* s, const void* tx, const lkl_logits* t,
                  const void* mask, int32_t mdt, float temperature) {
   int32_t e;
@@ -226,6 +240,7 @@ int32_t lkl_token_logprobs(const void* logits, const lkl_logits* l, const int64_
   if (!aligned(targets, 8) || !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(lse, 4) ||
       !aligned(top_logprobs, 4) || !aligned(top_indices, 8))
     return LKL_ERR_MISALIGNED;
+  if (low_aliases(l, lse)) return LKL_ERR_BAD_ALIAS;
   if (!bind_device_of(logits) || !device_is_sm100()) return LKL_ERR_NO_DEVICE;
   return launch_status(lkl::launch_token_logprobs(
       to_view(logits, l), l->B * l->T, targets, ignore_index, top_k, logprob, entropy, lse,
@@ -241,7 +256,7 @@ int32_t lkl_token_logprobs_backward(const void* logits, const lkl_logits* l,
   if (s) return s;
   if (l->B * l->T == 0) return LKL_OK;
   if (!targets || !lse || !entropy || !d_logits) return LKL_ERR_NULL_POINTER;
-  if (d_logits == logits) return LKL_ERR_BAD_ALIAS;
+  if (d_logits == logits || low_aliases(l, lse)) return LKL_ERR_BAD_ALIAS;
   if (!aligned(targets, 8) || !aligned(lse, 4) || !aligned(entropy, 4) ||
       !aligned(d_logprob, 4) || !aligned(d_entropy, 4) ||
       !aligned(d_logits, logits_elem(l->dtype)))
@@ -270,7 +285,7 @@ int32_t lkl_logits_kl_forward(const void* s_logits, const lkl_logits* s, const v
     if (!bind_device_of(loss)) return LKL_ERR_NO_DEVICE;
     return launch_status(cudaMemsetAsync(loss, 0, sizeof(float), st));
   }
-  if (!lse_s || !lse_t) return LKL_ERR_NULL_POINTER;
+  if ((e = check_kl_lse(s, t, lse_s, lse_t))) return e;
   if ((e = check_workspace(lkl_logits_kl_workspace_size(s), ws, ws_bytes))) return e;
   if (!bind_device_of(s_logits) || !device_is_sm100()) return LKL_ERR_NO_DEVICE;
   return launch_status(lkl::launch_logits_kl_forward(
@@ -285,7 +300,8 @@ int32_t lkl_logits_kl_backward(const void* s_logits, const lkl_logits* s, const 
   int32_t e = check_kl(s_logits, s, t_logits, t, mask, mask_dtype, temperature);
   if (e) return e;
   if (s->B * s->T == 0) return LKL_OK;
-  if (!lse_s || !lse_t || !ds) return LKL_ERR_NULL_POINTER;
+  if (!ds) return LKL_ERR_NULL_POINTER;
+  if ((e = check_kl_lse(s, t, lse_s, lse_t))) return e;
   if (ds == s_logits || ds == t_logits) return LKL_ERR_BAD_ALIAS;
   if (!aligned(lse_s, 4) || !aligned(lse_t, 4) || !aligned(dloss, 4) ||
       !aligned(ds, logits_elem(s->dtype)))
