@@ -33,9 +33,17 @@ cudaError_t launch_attn_delta(const AttnProblem& p, const AttnTensors& t, const 
 // 17% (bf16), and 1% at eight.  Rows that see at most this many keys (in a causal sequence
 // of any length, the first of its tokens that the mask keeps; else all rows of a sequence
 // with no more tokens) therefore take the sum; beyond it rows of many keys carry the
-// gradient and the roundings of dS and of the result outweigh that of out (dq of 4096
-// tokens, D 128, bf16, emulated: 0.0025 of its size off with no row by the sum, 0.00240
-// with the first 256, 0.00236 with all).
+// gradient and the roundings of dS and of the result outweigh that of out.  By how much goes
+// by the head dim.  Error of dq in bf16, emulated, with these rows by the sum and with all
+// (the result's rounding alone: 0.0017), causal and not:
+//   D 128, T 4000: 0.00238 and 0.00235, 0.00239 and 0.00236
+//   D 64, T 1000:  0.00247 and 0.00241, 0.00252 and 0.00242
+//   D 32, T 3000:  0.00258 and 0.00246, 0.00269 and 0.00253
+//   D 16, T 3000:  0.00275 and 0.00258, 0.00285 and 0.00258
+//   D 8, T 6500:   0.0034 and 0.0027, 0.0033 and 0.0029
+// A 16-bit remainder of out from the forward would bring the first of each pair near the
+// second.  It has no place in the call: the backward takes what a forward returns, out and
+// lse, and gives the same bits through autograd and by itself.
 constexpr int kExactDeltaKeys = 256;
 // The same into rows[] by that sum, for the rows that see at most kExactDeltaKeys keys.
 cudaError_t launch_attn_exact_delta(const AttnProblem& p, const AttnTensors& t,

@@ -8,8 +8,9 @@
 // 8 KB of shared memory a step, all that an SM delivers in 64 cycles), so neither may
 // wait: while one tile's warpgroup computes P, the other tile's GEMMs run.
 //
-// Measured at 32 / 8 heads x 8192 tokens, D 128, bf16, causal: 453 us, 1213 TFLOP/s, 73%
-// of the measured burst peak; two tiles x 128 keys take some 3300 cycles: softmax 1900,
+// Measured at 32 / 8 heads x 8192 tokens, D 128, bf16, causal: 453 to 469 us in bursts
+// (1213 TFLOP/s, 73% of the measured burst peak), 530 back to back at the power cap (1.67 GHz:
+// 1037 TFLOP/s, 62%); two tiles x 128 keys take some 3300 cycles: softmax 1900,
 // own GEMMs 1370 behind it.  Tried and slower there: P through shared memory, so
 // that S is free early (384 KB of shared memory a period: 610 against 541 us then);
 // 64-key units with two score buffers a tile (766); an MMA thread a tile (679);
@@ -31,7 +32,7 @@
 // Roundings: scores, statistics and every sum are fp32 (products of 16-bit inputs are
 // exact in it).  P is rounded to the inputs' type because the second GEMM takes 16-bit
 // operands; the row sum adds the unrounded P.  That error and the output's own rounding
-// are alike in size: 0.0022 of the output in bf16, 0.0016 with the latter alone.
+// are alike in size: 0.0022 of the output in bf16, 0.0016 with the latter alone (D 128).
 #include <math_constants.h>
 
 #include "lkl_attn.cuh"
@@ -543,8 +544,8 @@ cudaError_t run_attn_forward(const AttnProblem& p, const AttnTensors& t, const u
 //
 // Roundings: P and dS are rounded to the inputs' type, the only one that the GEMMs take,
 // and dS is handed over as rounded, which halves the dq launch's bytes.  The gradients
-// carry that error beside their result's own: 0.0024 of their size in bf16 instead of
-// 0.0017, 0.0003 instead of 0.0002 in fp16.  dS as a sum of two 16-bit values would
+// carry that error beside their result's own: at D 64 and 128 0.0024 of their size in bf16
+// instead of 0.0017, 0.0003 instead of 0.0002 in fp16.  dS as a sum of two 16-bit values would
 // take that back for a third more MMA steps and twice the hand-over.
 //
 // Sixteen row warps, 32 queries of 128 each (eight warps with 64 queries left the

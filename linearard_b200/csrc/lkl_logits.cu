@@ -2,8 +2,8 @@
 // entropy and top alternatives) and the KL between two models' rows, each with
 // its gradient.
 //
-// All four kernels are bound by HBM: a forward reads each logit once, a backward
-// reads it once more and writes its gradient.  The forwards keep, per thread, a
+// With many rows all four kernels are bound by HBM: a forward reads each logit once, a
+// backward reads it once more and writes its gradient.  The forwards keep, per thread, a
 // running maximum m and sums relative to it,
 //   l = sum e^(x - m),  a = sum e^(x - m) (x - m)     (token: entropy = log l - a / l)
 //   A = sum e^(t - m_t) ((t - m_t) - (s - m_s))       (KL = A / l_t + log l_s - log l_t),
@@ -15,10 +15,15 @@
 // forward hands over the rest of it as a second one, which costs a backward next to nothing
 // (0 to 2%): the multiplication by log2(e) becomes a multiply-add.
 //
-// Measured at 16384 x 32000 bf16 (of 6561 GB/s, the copy rate): KL backward 6.5 TB/s, forward
-// 6.1; token forward 5.9, backward 5.5 TB/s.  Blocks of 128 threads let ten rows of an SM
+// Measured at 16384 x 32000 bf16 (of 6561 GB/s, the copy rate): KL backward 6.4 TB/s, forward
+// 6.0; token forward 5.9, backward 5.7 TB/s.  Blocks of 128 threads let ten rows of an SM
 // overlap their ends, and 128 bytes in flight a thread fill HBM (64 bytes: 5.4 and 5.3;
-// 256 threads and pairwise joins: 4.0 and 3.8; 64 threads: 3.8 and 3.7).
+// 256 threads and pairwise joins: 4.0 and 3.8; 64 threads: 3.8 and 3.7).  Fewer rows leave
+// it idle at their ends: at 2004 x 50257 bf16 the KL takes 4.8 (forward) and 5.8 TB/s, the
+// token operator 4.6 and 4.8; at 999 x 50257 fp16 4.0 and 5.4, 3.8 and 3.4.  There the
+// rows of an SM are too few (7 of 999) for one's end to hide under another's loads, and the
+// token backward, with two 16-byte loads in flight a thread, is short of issue slots as well
+// (81% busy at 4096 x 32000).
 //
 // A row belongs to a cluster of 1, 2, 4 or 8 blocks that join their sums
 // through distributed shared memory, so that few rows still fill the GPU and
