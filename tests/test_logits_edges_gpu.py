@@ -122,3 +122,27 @@ def test_gradients_do_not_see_a_rows_offset(rows, V, tau, offset):
     size = 1.0 + 0.5 * (lp.abs() + 12.0)       # |g + h (log p + H)| with H below log V
     tol = p_error(s) * size + lp.exp() * 2.0 ** -20 * size + 2.0 ** -22 * want.abs() + 1e-38
     assert_within(token(s + offset), want, tol, "token logits shifted")
+
+
+@pytest.mark.parametrize("V", [7, 1000, 9001])
+@pytest.mark.parametrize("tau", [1.0, 2.0])
+def test_fp32_kl_gradient_of_near_models(V, tau):
+    """Where the models are near, each element's gradient is exact relative to its own size but
+    for what the row's log-sum-exps carry: two sums of V fp32 terms, in practice 2^-22 of each
+    (their worst case, V / 128 + 7 roundings of 2^-24 and exponentials of 2^-20, in full)."""
+    t = grid(64, V, seed=5)
+    step = 2.0 ** -9 * torch.randint(-8, 9, (64, V), device="cuda",
+                                     generator=torch.Generator(device="cuda").manual_seed(6))
+    s = (t + step).requires_grad_(True)
+    got = torch.autograd.grad(logits_kl_align(s, t, temperature=tau), s)[0].double()
+    ps, pt = (torch.softmax(x.detach().double() / tau, -1) for x in (s, t))
+    want = (ps - pt) / tau
+    # relative: the probability, e^x - 1 and the product; absolute: the row's two sums
+    lp = torch.log_softmax(t.double() / tau, -1)
+    rel = lp.abs() * 2.0 ** -22 + 2.0 ** -19
+    rows = 2 * ((V / 128 + 7) * 2.0 ** -24 + 2.0 ** -20)
+    assert_within(got, want, rel * want.abs() + rows * pt / tau + 1e-38, "ds")
+    # what the row's sums carry is one factor for the row: without it the relative bound holds
+    shift = ((got - want) / (pt / tau)).median(-1, keepdim=True).values
+    assert_within(got - shift * pt / tau, want, rel * (want.abs() + 2.0 ** -8 * pt / tau) + 1e-38,
+                  "ds beside the row's common part")
