@@ -140,7 +140,7 @@ size_t lkl_attn_backward_workspace_size(const lkl_attn_problem* p, int32_t has_m
   if (check_attn(p) != LKL_OK || p->B == 0 || p->T == 0) return 0;
   const AttnProblem a = to_attn(p);
   const size_t n = attn_stats_end(p, has_mask != 0);
-  if (a.D > 128) return n;
+  if (a.D > 128 || (long long)a.T * a.D <= lkl::kAttnFewElements) return n;
   return attn_scratch(p, has_mask != 0, SIZE_MAX).ds + round256(lkl::attn_sm100_ds_bytes(a)) +
          round256(lkl::attn_sm100_sums_bytes(a));
 }

@@ -28,3 +28,17 @@ def test_scales_of_the_whole_range_are_taken():
     q = torch.empty(1, 2, 8, 16).half()
     for sc in (2.0 ** -126, 1e-30, 1, 1e38):
         assert recompute._problem(q, q, True, 1, sc).sm_scale == pytest.approx(sc, rel=1e-6)
+
+
+def test_few_elements_ask_for_no_tile_scratch():
+    """Heads of at most 512 elements never reach the kernels that hand over tiles: row
+    statistics alone, 1 KB a head."""
+    L = _lib.lib()
+
+    def need(**kw):
+        p = _lib.LKLAttnProblem(**{**dict(B=4, Hq=64, Hkv=64, T=8, D=64, dtype=1, causal=1,
+                                          mask_dtype=1, sm_scale=0.0), **kw})
+        return L.lkl_attn_backward_workspace_size(ctypes.byref(p), 0)
+    for T, D in ((8, 64), (4, 128), (64, 8)):
+        assert need(T=T, D=D) == 4 * 64 * 1024
+    assert need(T=9) >= 4 * 64 * (1024 + 32768)
